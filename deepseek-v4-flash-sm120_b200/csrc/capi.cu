@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "dsv4b.h"
 #include "dsv4b_kernels.h"
@@ -101,6 +102,48 @@ int check_prefill_params(const dsv4b_decode_params* p) {
   // KV rows: 16-byte aligned base and row stride (16-byte loads), a whole d_qk row each.
   if (!aligned(p->kv, 16) || p->num_blocks <= 0 || p->page_block_size != 1) return DSV4B_ERR_INVALID_ARGUMENT;
   if (p->stride_kv_block % 16 != 0 || p->stride_kv_block < (int64_t)p->d_qk * 2) return DSV4B_ERR_INVALID_ARGUMENT;
+  return DSV4B_OK;
+}
+
+// Rows of 16-bit values that kernels read and write 16 bytes at a time.
+inline bool rows16(const void* p, int64_t a, int64_t b = 0, int64_t c = 0) {
+  return p && aligned(p, 16) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0 && a >= 0 && b >= 0 && c >= 0;
+}
+
+constexpr int64_t kMaxMapStride = (int64_t)1 << 40;  // tensor maps' limit, bytes
+
+// One of the cache's tensors: every (block, row, head) of it 16-byte aligned.
+inline bool gqa_rows(const void* p, int64_t block, int64_t row, int64_t head, int d) {
+  for (int64_t s : {block, row, head})
+    if (s % 16 || s < d || s >= kMaxMapStride) return false;
+  return p && aligned(p, 16);
+}
+
+int check_gqa_cache(const dsv4b_gqa_cache* c, bool with_v) {
+  if (!c || c->b <= 0 || c->num_blocks <= 0 || c->h_kv <= 0 || c->table_width <= 0) return DSV4B_ERR_INVALID_ARGUMENT;
+  if (c->b > dsv4b::kMaxGqaRequests || c->h_kv > 65535) return DSV4B_ERR_UNSUPPORTED;
+  const int page = c->page_block_size;
+  if (page < 16 || page > 1024 || (page & (page - 1))) return DSV4B_ERR_UNSUPPORTED;
+  if (c->d != 64 && c->d != 128) return DSV4B_ERR_UNSUPPORTED;
+  if (!gqa_rows(c->k, c->stride_k_block, c->stride_k_row, c->stride_k_head, c->d)) return DSV4B_ERR_INVALID_ARGUMENT;
+  if (!c->k_scale || !aligned(c->k_scale, 4) || !c->block_table || !aligned(c->block_table, 4) || !c->context_lens ||
+      !aligned(c->context_lens, 4) || c->stride_block_table < 0)
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (with_v && (!c->v_scale || !aligned(c->v_scale, 4) ||
+                 !gqa_rows(c->v, c->stride_v_block, c->stride_v_row, c->stride_v_head, c->d)))
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  return DSV4B_OK;
+}
+
+inline bool positive(float x) { return x > 0.f && x <= 3.402823466e38f; }
+
+int check_gqa_query(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q) {
+  if (!q || q->s_q <= 0 || q->h_q <= 0 || q->h_q % c->h_kv || !positive(q->sm_scale)) return DSV4B_ERR_INVALID_ARGUMENT;
+  if (q->dtype != DSV4B_BF16 && q->dtype != DSV4B_FP16) return DSV4B_ERR_UNSUPPORTED;
+  if (!rows16(q->q, q->stride_q_b, q->stride_q_s, q->stride_q_h)) return DSV4B_ERR_INVALID_ARGUMENT;
+  // one int numbers the (sequence, head, group of 16 rows), one the rows of a head
+  const int64_t rows = (int64_t)(q->h_q / c->h_kv) * q->s_q;
+  if (rows > (1 << 20) || (int64_t)c->b * c->h_kv * ((rows + 15) / 16) > INT_MAX) return DSV4B_ERR_UNSUPPORTED;
   return DSV4B_OK;
 }
 
@@ -405,12 +448,14 @@ int dsv4b_sparse_decode_noalloc(const dsv4b_decode_params* p, const dsv4b_sched_
 }
 
 int dsv4b_set_test_stall(int kernels) {
-  if (kernels & ~(DSV4B_STALL_DECODE | DSV4B_STALL_KV_WRITE | DSV4B_STALL_MQA_LOGITS))
+  if (kernels & ~(DSV4B_STALL_DECODE | DSV4B_STALL_KV_WRITE | DSV4B_STALL_MQA_LOGITS | DSV4B_STALL_GQA))
     return DSV4B_ERR_INVALID_ARGUMENT;
   int rc = current_arch_ok();
   if (rc) return rc;
   if ((rc = cuda_rc(dsv4b::set_decode_test_stall((kernels & DSV4B_STALL_DECODE) != 0)))) return rc;
   if ((rc = cuda_rc(dsv4b::set_kv_write_test_stall((kernels & DSV4B_STALL_KV_WRITE) != 0)))) return rc;
+  if ((rc = cuda_rc(dsv4b::set_gqa_test_stall((kernels & DSV4B_STALL_GQA) != 0)))) return rc;
+  if ((rc = cuda_rc(dsv4b::set_gqa_prefill_test_stall((kernels & DSV4B_STALL_GQA) != 0)))) return rc;
   return cuda_rc(dsv4b::set_mqa_test_stall((kernels & DSV4B_STALL_MQA_LOGITS) != 0));
 }
 
@@ -427,6 +472,120 @@ int dsv4b_read_kernel_status(void* workspace, size_t workspace_bytes, int* flags
   if ((rc = cuda_rc(cudaMemcpyAsync(flags, workspace, sizeof(int), cudaMemcpyDeviceToHost, s)))) return rc;
   if ((rc = cuda_rc(cudaStreamSynchronize(s)))) return rc;
   return cuda_rc(cudaMemsetAsync(workspace, 0, sizeof(int), s));
+}
+
+int dsv4b_gqa_status(int* flags, void* stream) {
+  if (!flags) return DSV4B_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int cache = 0, prefill = 0, rc;
+  if ((rc = cuda_rc(dsv4b::read_gqa_status(&cache, s)))) return rc;
+  if ((rc = cuda_rc(dsv4b::read_gqa_prefill_status(&prefill, s)))) return rc;
+  *flags = cache | prefill;
+  return DSV4B_OK;
+}
+
+int dsv4b_gqa_prefill(const dsv4b_gqa_prefill_params* p, void* stream) {
+  if (!p || p->b <= 0 || p->h_q <= 0 || p->h_kv <= 0 || p->h_q % p->h_kv || p->total_q < 0 || p->total_k < 0 ||
+      !positive(p->sm_scale))
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (p->dtype != DSV4B_BF16 && p->dtype != DSV4B_FP16) return DSV4B_ERR_UNSUPPORTED;
+  if (!((p->d_qk == 64 && p->d_v == 64) || ((p->d_qk == 128 || p->d_qk == 192) && p->d_v == 128)))
+    return DSV4B_ERR_UNSUPPORTED;
+  // int tiles and rows, one grid column of tiles x heads
+  if (p->b > dsv4b::kMaxGqaRequests || p->total_q > (1 << 30) || p->total_k > (1 << 30) ||
+      (p->total_q / 256 + p->b) * p->h_q > INT_MAX)
+    return DSV4B_ERR_UNSUPPORTED;
+  if (p->total_q == 0) return DSV4B_OK;
+  auto map_ok = [](const void* x, int64_t st, int64_t sh) {
+    return rows16(x, st, sh) && st * 2 < kMaxMapStride && sh * 2 < kMaxMapStride;
+  };
+  if (!map_ok(p->q, p->stride_q_t, p->stride_q_h) || !rows16(p->out, p->stride_o_t, p->stride_o_h))
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (p->total_k && (!map_ok(p->k, p->stride_k_t, p->stride_k_h) || !map_ok(p->v, p->stride_v_t, p->stride_v_h)))
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (!p->lse || !aligned(p->lse, 4) || !p->cu_seqlens_q || !aligned(p->cu_seqlens_q, 4) || !p->cu_seqlens_k ||
+      !aligned(p->cu_seqlens_k, 4))
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  int rc = current_arch_ok();
+  if (rc) return rc;
+  int bad = 0;
+  const cudaError_t e = dsv4b::launch_gqa_prefill(*p, static_cast<cudaStream_t>(stream), &bad);
+  return bad ? DSV4B_ERR_INVALID_ARGUMENT : cuda_rc(e);
+}
+
+int dsv4b_gqa_cache_append(const dsv4b_gqa_cache* c, int dtype, const void* k, int64_t stride_k_t,
+                           int64_t stride_k_h, const void* v, int64_t stride_v_t, int64_t stride_v_h,
+                           const int32_t* cu_seqlens, int64_t n, void* stream) {
+  int rc = check_gqa_cache(c, true);
+  if (rc) return rc;
+  if (dtype != DSV4B_BF16 && dtype != DSV4B_FP16) return DSV4B_ERR_UNSUPPORTED;
+  if (n < 0 || !cu_seqlens || !aligned(cu_seqlens, 4)) return DSV4B_ERR_INVALID_ARGUMENT;
+  if (n > INT_MAX) return DSV4B_ERR_UNSUPPORTED;
+  if (n == 0) return DSV4B_OK;
+  if (!rows16(k, stride_k_t, stride_k_h) || !rows16(v, stride_v_t, stride_v_h)) return DSV4B_ERR_INVALID_ARGUMENT;
+  if ((rc = current_arch_ok())) return rc;
+  return cuda_rc(dsv4b::launch_gqa_append(*c, dtype, k, stride_k_t, stride_k_h, v, stride_v_t, stride_v_h,
+                                          cu_seqlens, (int)n, static_cast<cudaStream_t>(stream)));
+}
+
+int dsv4b_gqa_decode_workspace_bytes(int device, int d, size_t* bytes) {
+  if (!bytes || (d != 64 && d != 128)) return DSV4B_ERR_INVALID_ARGUMENT;
+  DevInfo* info = nullptr;
+  const int rc = dev_info(device, &info);
+  if (rc) return rc;
+  *bytes = dsv4b::gqa_decode_ws_bytes(info->sms, d);
+  return DSV4B_OK;
+}
+
+int dsv4b_gqa_decode(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, void* out, int64_t stride_o_b,
+                     int64_t stride_o_s, int64_t stride_o_h, float* lse, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  int rc = check_gqa_cache(c, true);
+  if (rc || (rc = check_gqa_query(c, q))) return rc;
+  if (!rows16(out, stride_o_b, stride_o_s, stride_o_h) || !lse || !aligned(lse, 4)) return DSV4B_ERR_INVALID_ARGUMENT;
+  int dev = 0;
+  DevInfo* info = nullptr;
+  if ((rc = current_arch_ok())) return rc;
+  if (cudaGetDevice(&dev) != cudaSuccess) return DSV4B_ERR_CUDA;
+  if ((rc = dev_info(dev, &info))) return rc;
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < dsv4b::gqa_decode_ws_bytes(info->sms, c->d))
+    return DSV4B_ERR_WORKSPACE;
+  int bad = 0;
+  const cudaError_t e = dsv4b::launch_gqa_decode(*c, *q, out, stride_o_b, stride_o_s, stride_o_h, lse, workspace,
+                                                 info->sms, static_cast<cudaStream_t>(stream), &bad);
+  return bad ? DSV4B_ERR_INVALID_ARGUMENT : cuda_rc(e);
+}
+
+int dsv4b_gqa_attention_weights(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, const float* lse, float* weights,
+                                int64_t stride_w_b, int64_t stride_w_h, int32_t width, int accumulate, void* stream) {
+  int rc = check_gqa_cache(c, false);
+  if (rc || (rc = check_gqa_query(c, q))) return rc;
+  if (!lse || !aligned(lse, 4) || !weights || !aligned(weights, 4) || width <= 0 || stride_w_b < 0 || stride_w_h < 0)
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  int dev = 0;
+  DevInfo* info = nullptr;
+  if ((rc = current_arch_ok())) return rc;
+  if (cudaGetDevice(&dev) != cudaSuccess) return DSV4B_ERR_CUDA;
+  if ((rc = dev_info(dev, &info))) return rc;
+  int bad = 0;
+  const cudaError_t e = dsv4b::launch_gqa_weights(*c, *q, lse, weights, stride_w_b, stride_w_h, width, accumulate != 0,
+                                                  info->sms, static_cast<cudaStream_t>(stream), &bad);
+  return bad ? DSV4B_ERR_INVALID_ARGUMENT : cuda_rc(e);
+}
+
+int dsv4b_gqa_cache_evict(const dsv4b_gqa_cache* c, const dsv4b_gqa_evict_params* e, void* stream) {
+  int rc = check_gqa_cache(c, true);
+  if (rc) return rc;
+  if (!e || e->budget <= 0 || e->recent < 0 || e->recent > e->budget || e->width <= 0 || e->new_width < e->budget)
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (!e->weights || !e->new_weights || !e->kept || !e->new_lens || !e->new_table || e->new_table_width <= 0 ||
+      e->stride_w_b < 0 || e->stride_w_h < 0 || e->stride_nw_b < 0 || e->stride_nw_h < 0 || e->stride_new_table < 0)
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if (!aligned(e->weights, 4) || !aligned(e->new_weights, 4) || !aligned(e->kept, 4) || !aligned(e->new_lens, 4) ||
+      !aligned(e->new_table, 4) || e->new_table == c->block_table)
+    return DSV4B_ERR_INVALID_ARGUMENT;
+  if ((rc = current_arch_ok())) return rc;
+  return cuda_rc(dsv4b::launch_gqa_evict(*c, *e, static_cast<cudaStream_t>(stream)));
 }
 
 size_t dsv4b_prefill_workspace_bytes(int rows) {

@@ -83,4 +83,27 @@ cudaError_t launch_mqa_logits(const dsv4b_mqa_logits_params& p, const int32_t* s
 cudaError_t read_mqa_status(int* flags, cudaStream_t stream);
 cudaError_t set_mqa_test_stall(int stall);  // test hook, see dsv4b_set_test_stall
 
+// Grouped-query attention (csrc/gqa_cache.cu, csrc/gqa_decode.cu,
+// csrc/gqa_prefill.cu).  *bad_arg is set where the driver refuses a tensor
+// map of the arguments.
+constexpr int kMaxGqaRequests = 65535;
+cudaError_t launch_gqa_append(const dsv4b_gqa_cache& c, int dtype, const void* k, int64_t stride_k_t,
+                              int64_t stride_k_h, const void* v, int64_t stride_v_t, int64_t stride_v_h,
+                              const int32_t* cu_seqlens, int n, cudaStream_t stream);
+cudaError_t launch_gqa_evict(const dsv4b_gqa_cache& c, const dsv4b_gqa_evict_params& e, cudaStream_t stream);
+size_t gqa_decode_ws_bytes(int sms, int d);
+cudaError_t launch_gqa_decode(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q, void* out, int64_t stride_o_b,
+                              int64_t stride_o_s, int64_t stride_o_h, float* lse, void* ws, int sms,
+                              cudaStream_t stream, int* bad_arg);
+cudaError_t launch_gqa_weights(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q, const float* lse, float* weights,
+                               int64_t stride_w_b, int64_t stride_w_h, int width, int accumulate, int sms,
+                               cudaStream_t stream, int* bad_arg);
+cudaError_t launch_gqa_prefill(const dsv4b_gqa_prefill_params& p, cudaStream_t stream, int* bad_arg);
+// Status words and test hooks (dsv4b_set_test_stall) of the cache's kernels
+// and of the prompts'.
+cudaError_t read_gqa_status(int* flags, cudaStream_t stream);
+cudaError_t set_gqa_test_stall(int stall);
+cudaError_t read_gqa_prefill_status(int* flags, cudaStream_t stream);
+cudaError_t set_gqa_prefill_test_stall(int stall);
+
 }  // namespace dsv4b

@@ -1,0 +1,579 @@
+// Attention over whole prompts of packed sequences, grouped heads
+// (include/dsv4b.h, dsv4b_gqa_prefill), on the tcgen05 tensor cores.
+//
+//   S = q k^T, P = exp(sm_scale S - m), O = P v, out = O / sum(P)
+// with the running maximum m and sum of an online softmax over tiles of 128
+// keys.  2 (d_qk + d_v) operations per (query, key) against a few bytes per
+// token: bound by the tensor cores, with the exponentials next (a 128 x 128
+// tile is 2 * 128^2 (d_qk + d_v) operations, about 1,000 cycles of the tensor
+// core at d = 128, and 128^2 exponentials, 1,024 cycles of an SM's 16 a
+// cycle).
+//
+// One CTA has 256 queries of one head, as two tiles of 128, and walks the
+// keys they see.  While the tensor core multiplies for one tile, four warps
+// do the softmax of the other:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, a thread per row: S comes from
+//                   TMEM, P goes back there over S (16 bits, the A operand
+//                   of O += P v).  O is rescaled only when a row's maximum
+//                   grew by more than 2^8 (the exact maximum is not needed:
+//                   any reference within fp32's reach gives the same
+//                   quotient), which after the first tiles is rare;
+//   warp 8          issues the MMAs: S_0 S_1, then per key tile O_0 S_0' O_1
+//                   S_1', so that each softmax has the other tile's MMAs to
+//                   hide behind;
+//   warp 9          loads Q once and the K, V ring by TMA (SWIZZLE_128B);
+//   warp 10         V's guard, below.
+// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 and O_1 from 256 on.
+//
+// Masked keys have P = 0, but 0 * NaN is NaN: a row of V behind the
+// sequence's end belongs to another sequence or to nobody, and one behind a
+// query's position may hold anything.  Only the last key tiles of a CTA hold
+// such rows; there the guard zeroes the rows behind the end and any value
+// that is not finite, before the MMA reads them, and notes the rows of the
+// latter: a query that does see one has the value added at the end.
+//
+// The list of CTAs needs no lengths on the host: sequence i has the tiles
+// from cu_i / 256 + i on, at least as many as it can fill.  The last tiles
+// of a sequence, which see most keys, come first.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "dsv4b.h"
+#include "dsv4b_kernels.h"
+#include "dsv4b_ptx.cuh"
+
+namespace dsv4b {
+
+__device__ int g_gqa_prefill_status;          // kErr* bits on this device
+__device__ int g_gqa_prefill_test_stall = 0;  // test hook: Q's first load is withheld
+
+namespace {
+
+constexpr int kM = 128;              // queries of a tile, keys of a tile
+constexpr int kQueries = 2 * kM;     // queries of a CTA
+constexpr int kThreads = 11 * 32;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
+constexpr int kChunk = kM * 128;     // 128 rows x 64 16-bit columns, swizzled
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxEdge = 4;          // key tiles that some row of a CTA does not see whole
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;      // log2 of how far a maximum may be outgrown
+
+struct PrefillArgs {
+  int b, h_q, g, causal, total_q, total_k, tiles;
+  float scale_log2;
+  const void* v;
+  int64_t stride_v_t, stride_v_h;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  void* out;
+  int64_t stride_o_t, stride_o_h;
+  float* lse;
+};
+
+// Ring depths that fit 227 KB beside Q.
+template <int DQK, int DV>
+struct Cfg {
+  static constexpr int kQ = 2 * (DQK / 64) * kChunk;
+  static constexpr int kK = (DQK / 64) * kChunk;
+  static constexpr int kV = (DV / 64) * kChunk;
+  static constexpr int kStagesK = DQK == 64 ? 4 : 2;
+  static constexpr int kStagesV = DQK == 64 ? 4 : DQK == 128 ? 2 : 1;
+};
+
+struct Shared {
+  uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], go[kMaxEdge], guard[kMaxEdge];
+  uint64_t s_full[2], p_full[2], o_full[2], done;
+  uint32_t bad[kMaxEdge][4];  // rows of V with a value that is not finite
+  uint32_t tmem;
+  int abort;
+};
+
+template <int DQK, int DV>
+constexpr int smem_bytes() {
+  using C = Cfg<DQK, DV>;
+  return 1024 + C::kQ + C::kStagesK * C::kK + C::kStagesV * C::kV + (int)sizeof(Shared);
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit operands, fp32 sums.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
+  constexpr uint32_t types = (1u << 7) | (1u << 10);  // A, B: bf16 (0: fp16)
+  return std::is_same_v<T, __half> ? (idesc_bf16_f32(kM, n, false, b_mn_major) & ~types)
+                                   : idesc_bf16_f32(kM, n, false, b_mn_major);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// 0xFFFF in the halves of a word that are infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7C007C00u : 0x7F807F80u;
+  return __vcmpeq2(w & e, e);
+}
+
+// What a CTA works on, the same in every thread.
+struct Work {
+  int q0, rows;       // first query (row of q) and how many, 1 .. 256
+  int k0, n_k;        // the sequence's keys
+  int see;            // keys that the first query sees if causal (may be < 0)
+  int head;
+  __device__ __forceinline__ int limit(int r, int causal) const { return causal ? min(n_k, see + r) : n_k; }
+};
+
+template <typename T, int DQK, int DV>
+__global__ void __launch_bounds__(kThreads, 1)
+gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, const PrefillArgs a) {
+  using C = Cfg<DQK, DV>;
+  constexpr int kStagesK = C::kStagesK, kStagesV = C::kStagesV;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + C::kQ, v_s = k_s + kStagesK * C::kK;
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kQ + kStagesK * C::kK + kStagesV * C::kV);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  Work w;
+  {
+    const int tile = a.tiles - 1 - (int)(blockIdx.x / a.h_q);
+    auto cq = [&](int i) { return min(max(__ldg(a.cu_q + i), 0), a.total_q); };
+    int seq = 0;  // the number of i in [1, b) with cu_i / 256 + i <= tile
+    for (int i0 = 1; i0 < a.b; i0 += kThreads) {
+      const int i = i0 + tid;
+      const int c = __syncthreads_count(i < a.b && cq(i) / kQueries + i <= tile);
+      seq += c;
+      if (c < kThreads) break;
+    }
+    const int lo = cq(seq), n_q = max(0, cq(seq + 1) - lo);
+    const int t0 = (tile - (lo / kQueries + seq)) * kQueries;
+    if (t0 < 0 || t0 >= n_q) return;  // (t0 < 0: offsets that do not ascend)
+    w.head = (int)(blockIdx.x % a.h_q);
+    w.q0 = lo + t0;
+    w.rows = min(kQueries, n_q - t0);
+    w.k0 = min(max(__ldg(a.cu_k + seq), 0), a.total_k);
+    w.n_k = max(0, min(__ldg(a.cu_k + seq + 1), a.total_k) - w.k0);
+    w.see = t0 + w.n_k - n_q + 1;
+  }
+  const int kvh = w.head / a.g;
+  // key tiles of each query tile, and the first that some row does not see whole
+  int n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min(w.rows, (i + 1) * kM) - 1;
+    n[i] = last >= i * kM ? (max(0, w.limit(last, a.causal)) + kM - 1) / kM : 0;
+  }
+  const int nt = max(n[0], n[1]);
+  const int edge = max(0, w.limit(0, a.causal)) / kM;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], kM);
+      mbar_init(&sh.o_full[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.go[i], 1);
+      mbar_init(&sh.guard[i], 1);
+    }
+    mbar_init(&sh.done, 1);
+    sh.abort = 0;
+    fence_mbarrier_init();
+  }
+  if (tid < 16) (&sh.bad[0][0])[tid] = 0;
+  if (warp == kMmaWarp) {
+    tmem_alloc(&sh.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  volatile int* abort = &sh.abort;
+  int* status = &g_gqa_prefill_status;
+
+  if (warp == kLoadWarp) {
+    // ---------------------------------------------------------------- loads
+    if (lane == 0 && nt > 0) {
+      const bool withhold = g_gqa_prefill_test_stall != 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (n[i] == 0) continue;
+        if (withhold && i == 0) continue;
+        mbar_arrive_expect_tx(&sh.q_full[i], C::kQ / 2);
+        for (int c = 0; c < DQK / 64; ++c)
+          tma_load_3d(q_s + i * (C::kQ / 2) + c * kChunk, &tq, c * 64, w.head, w.q0 + i * kM, &sh.q_full[i]);
+      }
+      int nk = 0, nv = 0;  // tiles issued
+      auto load_k = [&]() {
+        const int st = nk % kStagesK;
+        if (nk >= kStagesK && !mbar_wait(&sh.k_empty[st], (nk / kStagesK - 1) & 1, abort, status)) return false;
+        mbar_arrive_expect_tx(&sh.k_full[st], C::kK);
+        for (int c = 0; c < DQK / 64; ++c)
+          tma_load_3d(k_s + st * C::kK + c * kChunk, &tk, c * 64, kvh, w.k0 + nk * kM, &sh.k_full[st]);
+        ++nk;
+        return true;
+      };
+      auto load_v = [&]() {
+        const int st = nv % kStagesV;
+        if (nv >= kStagesV && !mbar_wait(&sh.v_empty[st], (nv / kStagesV - 1) & 1, abort, status)) return false;
+        mbar_arrive_expect_tx(&sh.v_full[st], C::kV);
+        for (int c = 0; c < DV / 64; ++c)
+          tma_load_3d(v_s + st * C::kV + c * kChunk, &tv, c * 64, kvh, w.k0 + nv * kM, &sh.v_full[st]);
+        if (nv >= edge) mbar_arrive(&sh.go[nv - edge]);
+        ++nv;
+        return true;
+      };
+      bool ok = load_k();
+      while (ok && nv < nt) {  // in the order of use: K_0 K_1 V_0 K_2 V_1 ...
+        if (nk < nt) ok = load_k();
+        if (ok) ok = load_v();
+      }
+      if (*abort) {  // what is in flight lands (or its wait runs out) before the CTA's shared memory goes
+        auto land = [&](uint64_t* bar, uint32_t parity) {
+          const long long t = clock64();
+          while (!mbar_try_wait(smem_u32(bar), parity, 1000u) && clock64() - t < kWaitLimitCycles) {
+          }
+        };
+        for (int x = max(0, nk - kStagesK); x < nk; ++x) land(&sh.k_full[x % kStagesK], (x / kStagesK) & 1);
+        for (int x = max(0, nv - kStagesV); x < nv; ++x) land(&sh.v_full[x % kStagesV], (x / kStagesV) & 1);
+        for (int i = 0; i < 2; ++i)
+          if (n[i] && !(withhold && i == 0)) land(&sh.q_full[i], 0);
+      }
+    }
+  } else if (warp == kGuardWarp) {
+    // ---------------------------------------------------------------- guard
+    for (int j = edge; j < nt; ++j) {
+      const int sv = j % kStagesV;
+      // `go`: the tile's load is on its way, so its stage's phase is this one
+      // (a parity alone does not tell it from the one before the last)
+      if (!mbar_wait(&sh.go[j - edge], 0, abort, status)) break;
+      if (!mbar_wait(&sh.v_full[sv], (j / kStagesV) & 1, abort, status)) break;
+      const int end = w.n_k - j * kM;                                      // rows from here on are no keys of ours
+      const int from = max(0, w.limit(0, a.causal) - j * kM);              // rows before it are seen by all
+      uint8_t* tile = smem + C::kQ + kStagesK * C::kK + sv * C::kV;
+      for (int c = 0; c < DV / 64; ++c) {
+        for (int r = (from & ~3) + (lane >> 3); r < kM; r += 4) {
+          uint4* p = reinterpret_cast<uint4*>(tile + c * kChunk + r * 128 + (lane & 7) * 16);
+          if (r >= end) {
+            *p = make_uint4(0, 0, 0, 0);
+          } else if (r >= from) {
+            uint4 x = *p;
+            const uint4 m = make_uint4(not_finite<T>(x.x), not_finite<T>(x.y), not_finite<T>(x.z), not_finite<T>(x.w));
+            if (m.x | m.y | m.z | m.w) {
+              *p = make_uint4(x.x & ~m.x, x.y & ~m.y, x.z & ~m.z, x.w & ~m.w);
+              atomicOr(&sh.bad[j - edge][r >> 5], 1u << (r & 31));
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.guard[j - edge]);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMAs
+    constexpr uint32_t idesc_s = idesc_of<T>(kM, false), idesc_o = idesc_of<T>(DV, true);
+    auto scores = [&](int i, int sk) {  // S_i = Q_i K^T
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < DQK / 64; ++c)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_bf16_ss(tmem + i * kM, sdesc_sw128(q_s + i * (C::kQ / 2) + c * kChunk + kk * 32, 16, 1024),
+                         sdesc_sw128(k_s + sk * C::kK + c * kChunk + kk * 32, 16, 1024), idesc_s, (c | kk) != 0);
+        umma_commit(&sh.s_full[i]);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int i, int sv, bool first) {  // O_i += P_i V
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kM / 16; ++kk)
+          umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8,
+                  sdesc_sw128(v_s + sv * C::kV + kk * 2048, kChunk, 1024), idesc_o, !(first && kk == 0));
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    bool ok = true;
+    for (int i = 0; i < 2 && ok; ++i)
+      if (n[i]) ok = mbar_wait(&sh.q_full[i], 0, abort, status);
+    if (nt > 0 && ok && (ok = mbar_wait(&sh.k_full[0], 0, abort, status))) {
+      for (int i = 0; i < 2; ++i)
+        if (n[i]) scores(i, 0);
+      commit(&sh.k_empty[0]);
+      for (int j = 0; j < nt && ok; ++j) {
+        const int sv = j % kStagesV, sk = (j + 1) % kStagesK;
+        ok = mbar_wait(&sh.v_full[sv], (j / kStagesV) & 1, abort, status);
+        if (ok && j >= edge) ok = mbar_wait(&sh.guard[j - edge], 0, abort, status);
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j >= n[i]) continue;
+          if (!(ok = mbar_wait(&sh.p_full[i], j & 1, abort, status))) break;
+          tc_fence_after();
+          values(i, sv, j == 0);
+          if (j + 1 < n[i]) {
+            if (!(ok = mbar_wait(&sh.k_full[sk], ((j + 1) / kStagesK) & 1, abort, status))) break;
+            scores(i, sk);
+          } else {
+            commit(&sh.o_full[i]);
+          }
+        }
+        commit(&sh.v_empty[sv]);
+        if (j + 1 < nt) commit(&sh.k_empty[sk]);
+      }
+    }
+    // every MMA has completed before TMEM is freed
+    commit(&sh.done);
+    const long long t = clock64();
+    while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int i = warp >> 2;  // query tile
+    const int r = i * kM + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + lanes + i * kM, o_t = tmem + lanes + 256 + i * DV;
+    const int lim = w.limit(r, a.causal), lim0 = w.limit(i * kM, a.causal);
+    const int mine = n[i];
+    const float c = a.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      if (!(ok = mbar_wait(&sh.s_full[i], j & 1, abort, status))) break;
+      tc_fence_after();
+      float s[kM];
+#pragma unroll
+      for (int x = 0; x < kM; x += 32) tmem_ld32(s_t + x, *reinterpret_cast<float(*)[32]>(&s[x]));
+      tc_wait_ld();
+      if (j * kM + kM > lim0) {
+        const int left = lim - j * kM;
+#pragma unroll
+        for (int x = 0; x < kM; ++x) s[x] = x < left ? s[x] : -INFINITY;
+      }
+      float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+#pragma unroll
+      for (int x = 4; x < kM; x += 4) {
+        t0 = fmaxf(t0, s[x]);
+        t1 = fmaxf(t1, s[x + 1]);
+        t2 = fmaxf(t2, s[x + 2]);
+        t3 = fmaxf(t3, s[x + 3]);
+      }
+      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+      const bool grew = (top - m) * c > kRescale;  // from -inf: always
+      if (__any_sync(0xffffffffu, grew)) {
+        const float f = grew ? fast_exp2((m - top) * c) : 1.f;
+        if (grew) m = top;
+        l *= f;
+        if (j > 0) {  // the MMAs of the tile before are complete: this tile's S came after them
+#pragma unroll
+          for (int x = 0; x < DV; x += 32) {
+            float o[32];
+            tmem_ld32(o_t + x, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tmem_st32(o_t + x, o);
+          }
+        }
+      }
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int x = 0; x < kM; x += 32) {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float u = fast_exp2(fmaf(s[x + 2 * e], c, -mc)), v = fast_exp2(fmaf(s[x + 2 * e + 1], c, -mc));
+          l0 += u;
+          l1 += v;
+          p[e] = __uint_as_float(pack16<T>(u, v));
+        }
+        tmem_st16(s_t + x / 2, p);
+      }
+      l += l0 + l1;
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&sh.p_full[i]);
+    }
+    if (mine > 0 && ok) ok = mbar_wait(&sh.o_full[i], 0, abort, status);
+    // rows of V that were kept out of the products, for those who see them
+    bool bad = false;
+    for (int j = edge; j < mine && ok; ++j) {
+      ok = mbar_wait(&sh.guard[j - edge], 0, abort, status);
+      bad |= (sh.bad[j - edge][0] | sh.bad[j - edge][1] | sh.bad[j - edge][2] | sh.bad[j - edge][3]) != 0;
+    }
+    tc_fence_after();
+    const bool live = r < w.rows;
+    const bool none = lim <= 0;
+    if (ok) {
+      const float inv = 1.f / l;
+      T* out = static_cast<T*>(a.out) + (int64_t)(w.q0 + r) * a.stride_o_t + (int64_t)w.head * a.stride_o_h;
+#pragma unroll
+      for (int x = 0; x < DV; x += 32) {
+        float o[32];
+        if (mine > 0) {
+          tmem_ld32(o_t + x, o);
+          tc_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = none ? 0.f : o[e] * inv;
+        if (bad) {
+          for (int j = edge; j < mine; ++j)
+            for (int k = 0; k < 4; ++k)
+              for (uint32_t bits = sh.bad[j - edge][k]; bits; bits &= bits - 1) {
+                const int t = j * kM + k * 32 + __ffs(bits) - 1;
+                if (t >= lim) continue;
+                const T* v = static_cast<const T*>(a.v) + (int64_t)(w.k0 + t) * a.stride_v_t +
+                             (int64_t)kvh * a.stride_v_h + x;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float f = static_cast<float>(v[e]);
+                  if (!(fabsf(f) < INFINITY)) o[e] += f;
+                }
+              }
+        }
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            *reinterpret_cast<uint4*>(out + x + e) = make_uint4(pack16<T>(o[e], o[e + 1]), pack16<T>(o[e + 2], o[e + 3]),
+                                                               pack16<T>(o[e + 4], o[e + 5]), pack16<T>(o[e + 6], o[e + 7]));
+          }
+        }
+      }
+      if (live) a.lse[(int64_t)(w.q0 + r) * a.h_q + w.head] = none ? -INFINITY : (m * c + log2f(l)) * kLn2;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// [tokens][heads][d] of 16 bits, boxes of 128 tokens x 64 columns of a head.
+bool make_map(CUtensorMap* m, const void* base, int64_t tokens, int heads, int d, int64_t stride_t, int64_t stride_h,
+              int dtype) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+  if (!enc) return false;
+  // strides of dims of size 1 (given as 0) are never used
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)(stride_h ? stride_h * 2 : d * 2), (cuuint64_t)(stride_t ? stride_t * 2 : d * 2)};
+  const cuuint32_t box[3] = {64, 1, kM};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return enc(m, dtype == DSV4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DQK, int DV>
+cudaError_t launch(const dsv4b_gqa_prefill_params& p, cudaStream_t stream, int* bad_arg) {
+  CUtensorMap tq, tk, tv;
+  // without a single key nothing is loaded: any valid map will do
+  const bool keys = p.total_k > 0;
+  if (!make_map(&tq, p.q, p.total_q, p.h_q, DQK, p.stride_q_t, p.stride_q_h, p.dtype) ||
+      !make_map(&tk, keys ? p.k : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DQK, keys ? p.stride_k_t : 0,
+                keys ? p.stride_k_h : 0, p.dtype) ||
+      !make_map(&tv, keys ? p.v : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DV, keys ? p.stride_v_t : 0,
+                keys ? p.stride_v_h : 0, p.dtype)) {
+    *bad_arg = 1;
+    return cudaErrorInvalidValue;
+  }
+  PrefillArgs a = {};
+  a.b = p.b;
+  a.h_q = p.h_q;
+  a.g = p.h_q / p.h_kv;
+  a.causal = p.causal;
+  a.total_q = (int)p.total_q;
+  a.total_k = (int)p.total_k;
+  a.tiles = (int)p.total_q / kQueries + p.b;
+  a.scale_log2 = p.sm_scale * kLog2e;
+  a.v = p.v;
+  a.stride_v_t = p.stride_v_t;
+  a.stride_v_h = p.stride_v_h;
+  a.cu_q = p.cu_seqlens_q;
+  a.cu_k = p.cu_seqlens_k;
+  a.out = p.out;
+  a.stride_o_t = p.stride_o_t;
+  a.stride_o_h = p.stride_o_h;
+  a.lse = p.lse;
+  constexpr int smem = smem_bytes<DQK, DV>();
+  static_assert(smem <= 227 * 1024, "prefill kernel shared memory");
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    e = cudaFuncSetAttribute(gqa_prefill_kernel<T, DQK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  gqa_prefill_kernel<T, DQK, DV><<<(unsigned)((int64_t)a.tiles * p.h_q), kThreads, smem, stream>>>(tq, tk, tv, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_gqa_prefill(const dsv4b_gqa_prefill_params& p, cudaStream_t stream, int* bad_arg) {
+  if (p.dtype == DSV4B_BF16) {
+    if (p.d_qk == 64) return launch<__nv_bfloat16, 64, 64>(p, stream, bad_arg);
+    if (p.d_qk == 128) return launch<__nv_bfloat16, 128, 128>(p, stream, bad_arg);
+    return launch<__nv_bfloat16, 192, 128>(p, stream, bad_arg);
+  }
+  if (p.d_qk == 64) return launch<__half, 64, 64>(p, stream, bad_arg);
+  if (p.d_qk == 128) return launch<__half, 128, 128>(p, stream, bad_arg);
+  return launch<__half, 192, 128>(p, stream, bad_arg);
+}
+
+cudaError_t read_gqa_prefill_status(int* flags, cudaStream_t stream) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(flags, g_gqa_prefill_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+  if (e != cudaSuccess) return e;
+  if ((e = cudaStreamSynchronize(stream)) != cudaSuccess) return e;
+  static const int zero = 0;
+  return cudaMemcpyToSymbolAsync(g_gqa_prefill_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+}
+
+cudaError_t set_gqa_prefill_test_stall(int stall) {
+  return cudaMemcpyToSymbol(g_gqa_prefill_test_stall, &stall, sizeof(stall));
+}
+
+}  // namespace dsv4b

@@ -4,8 +4,10 @@ Drop-in for the reference package's public surface
 (deepseek_v4_kernel/__init__.py:1-7): ``sparse_decode_fwd`` and
 ``patch_flash_mla``; plus the FlashMLA-compatible interface functions,
 the KV-cache writers that produce the FP8 pages (``cache_ops``), the
-indexer logits that produce ``indices`` (``indexer``) and the sparse
-prefill ``flash_mla_sparse_fwd`` (``prefill``).
+indexer logits that produce ``indices`` (``indexer``), the sparse
+prefill ``flash_mla_sparse_fwd`` (``prefill``), and grouped-query attention
+for the layers and draft models beside the latent ones (``gqa``): whole
+prompts, and an 8-bit cache with append, decode and eviction.
 
 The public names are resolved on first use (PEP 562), so importing a
 host-only submodule such as ``deepseek_v4_kernel.kvcache`` or
@@ -29,6 +31,11 @@ _EXPORTS = {
     "flash_mla_sparse_fwd": ("prefill", "flash_mla_sparse_fwd"),
     "flash_mla_with_kvcache": ("interface", "flash_mla_with_kvcache"),
     "get_mla_metadata": ("interface", "get_mla_metadata"),
+    "gqa_attention_weights": ("gqa", "gqa_attention_weights"),
+    "gqa_cache_append": ("gqa", "gqa_cache_append"),
+    "gqa_cache_evict": ("gqa", "gqa_cache_evict"),
+    "gqa_decode_fwd": ("gqa", "gqa_decode_fwd"),
+    "gqa_prefill_fwd": ("gqa", "gqa_prefill_fwd"),
     "gather_dequant": ("ops", "gather_dequant"),
     "read_kernel_status": ("ops", "read_kernel_status"),
     "sparse_decode_fwd": ("ops", "sparse_decode_fwd"),

@@ -38,12 +38,14 @@ EXPORTED = (
     "dsv4b_mqa_logits_metadata", "dsv4b_fp8_paged_mqa_logits", "dsv4b_mqa_logits_status",
     "dsv4b_set_test_stall", "dsv4b_prefill_workspace_bytes", "dsv4b_sparse_prefill",
     "dsv4b_mma_rate_probe", "dsv4b_gather_rate_probe",
+    "dsv4b_gqa_cache_append", "dsv4b_gqa_decode_workspace_bytes", "dsv4b_gqa_decode",
+    "dsv4b_gqa_attention_weights", "dsv4b_gqa_cache_evict", "dsv4b_gqa_prefill", "dsv4b_gqa_status",
 )
 
 NOALLOC_SCRATCH_BYTES = 32 * 1024 * 1024
 
 # dsv4b_set_test_stall bits
-STALL_DECODE, STALL_KV_WRITE, STALL_MQA_LOGITS = 1, 2, 4
+STALL_DECODE, STALL_KV_WRITE, STALL_MQA_LOGITS, STALL_GQA = 1, 2, 4, 16
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -118,6 +120,13 @@ def _load():
     lib.dsv4b_prefill_workspace_bytes.restype = ctypes.c_size_t
     lib.dsv4b_prefill_workspace_bytes.argtypes = [ctypes.c_int]
     lib.dsv4b_sparse_prefill.argtypes = [P, _vp, ctypes.c_size_t, _vp]
+    lib.dsv4b_gqa_cache_append.argtypes = [_vp, ctypes.c_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]
+    lib.dsv4b_gqa_decode_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]
+    lib.dsv4b_gqa_decode.argtypes = [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, ctypes.c_size_t, _vp]
+    lib.dsv4b_gqa_attention_weights.argtypes = [_vp, _vp, _vp, _vp, _i64, _i64, _i32, ctypes.c_int, _vp]
+    lib.dsv4b_gqa_cache_evict.argtypes = [_vp, _vp, _vp]
+    lib.dsv4b_gqa_prefill.argtypes = [_vp, _vp]
+    lib.dsv4b_gqa_status.argtypes = [ctypes.POINTER(ctypes.c_int), _vp]
     return lib
 
 

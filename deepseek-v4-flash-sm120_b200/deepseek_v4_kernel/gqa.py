@@ -1,0 +1,378 @@
+"""Grouped-query attention: whole prompts, and an 8-bit paged cache.
+
+For the layers and draft models that a serving engine runs beside the
+latent-attention ones (the reference has none of it), and for dense prompts
+of latent attention with its heads expanded (d_qk 192, d_v 128).  The
+functions make one serving path:
+
+* ``gqa_prefill_fwd``        attention over packed whole prompts;
+* ``gqa_cache_append``       their (or a decode step's) K and V into the cache;
+* ``gqa_decode_fwd``         attention of each sequence's last tokens over it;
+* ``gqa_attention_weights``  the weight that each cached position drew;
+* ``gqa_cache_evict``        keeps the heaviest and the newest positions.
+
+The cache: ``k_cache`` and ``v_cache`` float8_e4m3fn (or uint8) [num_blocks,
+P, h_kv, d] with any 16-byte aligned strides (a [num_blocks, h_kv, P, d]
+pool is passed as ``pool.transpose(1, 2)``), P a power of two from 16 to
+1024, d 64 or 128; ``k_scale`` and ``v_scale`` fp32 [num_blocks, h_kv]: a
+stored value stands for e4m3 * scale of its block and head.  Position t of
+sequence i lies in block ``block_table[i, t // P]``, row t % P;
+``context_lens`` int32 [b] counts each sequence's positions.  Block ids out
+of range hold nothing: reads leave them out, writes skip them.
+
+All run on the current stream without a host synchronisation and can be
+captured in CUDA graphs.  Errors raise RuntimeError.  See include/dsv4b.h
+for the exact contracts.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import check, lib
+from .ops import _on_device, _stream
+
+_i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_FP8 = (torch.float8_e4m3fn, torch.uint8)
+
+
+class GqaCache(ctypes.Structure):
+    """dsv4b_gqa_cache."""
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+        ("stride_k_block", _i64), ("stride_k_row", _i64), ("stride_k_head", _i64),
+        ("stride_v_block", _i64), ("stride_v_row", _i64), ("stride_v_head", _i64),
+        ("num_blocks", _i32), ("page_block_size", _i32), ("h_kv", _i32), ("d", _i32),
+        ("block_table", _vp), ("stride_block_table", _i64), ("table_width", _i32), ("b", _i32),
+        ("context_lens", _vp),
+    ]
+
+
+class GqaQuery(ctypes.Structure):
+    """dsv4b_gqa_query."""
+    _fields_ = [
+        ("dtype", _i32), ("s_q", _i32), ("h_q", _i32), ("sm_scale", _f32),
+        ("q", _vp), ("stride_q_b", _i64), ("stride_q_s", _i64), ("stride_q_h", _i64),
+    ]
+
+
+class GqaEvictParams(ctypes.Structure):
+    """dsv4b_gqa_evict_params."""
+    _fields_ = [
+        ("budget", _i32), ("recent", _i32), ("weights", _vp), ("stride_w_b", _i64), ("stride_w_h", _i64),
+        ("width", _i32), ("new_width", _i32), ("new_weights", _vp), ("stride_nw_b", _i64), ("stride_nw_h", _i64),
+        ("kept", _vp), ("new_lens", _vp), ("new_table", _vp), ("stride_new_table", _i64), ("new_table_width", _i32),
+    ]
+
+
+class GqaPrefillParams(ctypes.Structure):
+    """dsv4b_gqa_prefill_params."""
+    _fields_ = [
+        ("dtype", _i32), ("b", _i32), ("h_q", _i32), ("h_kv", _i32), ("d_qk", _i32), ("d_v", _i32), ("causal", _i32),
+        ("sm_scale", _f32), ("total_q", _i64), ("total_k", _i64),
+        ("q", _vp), ("stride_q_t", _i64), ("stride_q_h", _i64),
+        ("k", _vp), ("stride_k_t", _i64), ("stride_k_h", _i64),
+        ("v", _vp), ("stride_v_t", _i64), ("stride_v_h", _i64),
+        ("cu_seqlens_q", _vp), ("cu_seqlens_k", _vp),
+        ("out", _vp), ("stride_o_t", _i64), ("stride_o_h", _i64), ("lse", _vp),
+    ]
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise RuntimeError(message)
+
+
+def _int32(t: torch.Tensor, shape, name: str, dev: torch.device) -> int:
+    """Pointer of a contiguous int32 tensor of this shape."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {dev}, got "
+                           f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, b: int, name: str, dev: torch.device) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.size(0) != b or t.size(1) < 1 or t.device != dev or \
+            (t.size(1) > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name} must be int32 [{b}, blocks] on {dev} with a contiguous last dim")
+
+
+def _rows16(t: torch.Tensor, name: str) -> None:
+    """Rows that the kernels read or write 16 bytes at a time."""
+    st = t.stride()
+    if st[-1] != 1 or any(s % 8 and n > 1 for s, n in zip(st[:-1], t.shape)) or t.data_ptr() % 16:
+        raise RuntimeError(f"{name} needs a contiguous last dim, other strides in multiples of 8 elements and a "
+                           f"16-byte aligned base, got strides {st}")
+
+
+def _strides(t: torch.Tensor):
+    """Strides with those of size-1 dims (which no address uses) made 0."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+
+
+def _fp8_cache(t: torch.Tensor, scale: torch.Tensor, name: str, dev: torch.device):
+    """The three byte strides of a cache tensor, checked with its scales."""
+    if t.dtype not in _FP8 or t.dim() != 4 or t.device != dev:
+        raise RuntimeError(f"{name}_cache must be float8_e4m3fn / uint8 [num_blocks, P, h_kv, d] on {dev}")
+    nb, page, h, d = t.shape
+    _require(nb > 0 and h > 0, f"{name}_cache has no blocks or heads")
+    _require(page in (16, 32, 64, 128, 256, 512, 1024), f"block size {page}: a power of two from 16 to 1024 is supported")
+    _require(d in (64, 128), f"d = {d}: 64 or 128 is supported")
+    sb, sr, sh, sd = t.stride()
+    if nb == 1:  # size-1 dims: any stride will do
+        sb = max(page * sr, d)
+    if h == 1:
+        sh = max(sr, d)
+    if sd != 1 or sb % 16 or sr % 16 or sh % 16 or min(sb, sr, sh) < d or t.data_ptr() % 16:
+        raise RuntimeError(f"{name}_cache needs a contiguous last dim, other strides in multiples of 16 bytes and a "
+                           f"16-byte aligned base, got strides {t.stride()}")
+    if scale.dtype != torch.float32 or scale.shape != (nb, h) or not scale.is_contiguous() or scale.device != dev:
+        raise RuntimeError(f"{name}_scale must be contiguous float32 {[nb, h]} on {dev}")
+    return sb, sr, sh
+
+
+def _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens) -> GqaCache:
+    dev = k_cache.device
+    _require(k_cache.is_cuda, "the cache must be a CUDA tensor")
+    b = context_lens.numel()
+    _require(b > 0, "context_lens is empty")
+    ctx = _int32(context_lens, (b,), "context_lens", dev)
+    _table(block_table, b, "block_table", dev)
+    kb, kr, kh = _fp8_cache(k_cache, k_scale, "k", dev)
+    v = vs = None
+    vb = vr = vh = 0
+    if v_cache is not None:
+        _require(v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape")
+        vb, vr, vh = _fp8_cache(v_cache, v_scale, "v", dev)
+        v, vs = v_cache.data_ptr(), v_scale.data_ptr()
+    nb, page, h, d = k_cache.shape
+    return GqaCache(k_cache.data_ptr(), v, k_scale.data_ptr(), vs, kb, kr, kh, vb, vr, vh, nb, page, h, d,
+                    block_table.data_ptr(), block_table.stride(0), block_table.size(1), b, ctx)
+
+
+def _query(q, c: GqaCache, sm_scale: Optional[float], dev: torch.device) -> GqaQuery:
+    if q.dim() != 4 or q.dtype not in _DTYPES or q.device != dev:
+        raise RuntimeError("q must be bf16 / fp16 [b, s_q, h_q, d] on the cache's device")
+    b, s_q, h_q, d = q.shape
+    _require(b == c.b and d == c.d and s_q > 0, f"q {tuple(q.shape)} does not match {c.b} sequences of d {c.d}")
+    _require(h_q > 0 and h_q % c.h_kv == 0, f"{h_q} query heads are not a multiple of {c.h_kv} KV heads")
+    _rows16(q, "q")
+    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
+    _require(0.0 < scale < float("inf"), f"sm_scale must be positive, got {scale}")
+    sb, ss, sh, _ = _strides(q)
+    return GqaQuery(_DTYPES[q.dtype], s_q, h_q, scale, q.data_ptr(), sb, ss, sh)
+
+
+def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                    cu_seqlens_k: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+                    causal: bool = True, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention over whole prompts of packed sequences.
+
+    q [total_q, h_q, d_qk], k [total_k, h_kv, d_qk], v [total_k, h_kv, d_v],
+    bf16 or fp16, (d_qk, d_v) = (64, 64), (128, 128) or (192, 128), h_q a
+    multiple of h_kv; cu_seqlens int32 [b + 1] (``cu_seqlens_k`` defaults to
+    ``cu_seqlens_q``).  With ``causal`` the last query of a sequence sees
+    all its keys, the one before it one less, and so on.  Returns (out
+    [total_q, h_q, d_v], lse fp32 [total_q, h_q], natural log); a query that
+    sees no key gets 0 and -inf.  Rows behind the last sequence are not
+    written."""
+    dev = q.device
+    _require(q.is_cuda, "q must be a CUDA tensor")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 3 or t.dtype != q.dtype or t.dtype not in _DTYPES or t.device != dev:
+            raise RuntimeError(f"{name} must be bf16 / fp16 [tokens, heads, d], as q is, on {dev}")
+    total_q, h_q, d_qk = q.shape
+    total_k, h_kv, d_v = v.shape
+    _require(k.shape == (total_k, h_kv, d_qk), f"k {tuple(k.shape)} does not match q {tuple(q.shape)} and v {tuple(v.shape)}")
+    _require((d_qk, d_v) in ((64, 64), (128, 128), (192, 128)), f"(d_qk, d_v) = {(d_qk, d_v)}: (64, 64), (128, 128) "
+             "or (192, 128) is supported")
+    _require(h_kv > 0 and h_q > 0 and h_q % h_kv == 0, f"{h_q} query heads are not a multiple of {h_kv} KV heads")
+    scale = d_qk ** -0.5 if sm_scale is None else float(sm_scale)
+    _require(0.0 < scale < float("inf"), f"sm_scale must be positive, got {scale}")
+    b = cu_seqlens_q.numel() - 1
+    _require(b >= 1, "cu_seqlens_q must have b + 1 >= 2 entries")
+    cq = _int32(cu_seqlens_q, (b + 1,), "cu_seqlens_q", dev)
+    if cu_seqlens_k is None:
+        _require(total_k == total_q, "k and q have different lengths: pass cu_seqlens_k")
+        ck = cq
+    else:
+        ck = _int32(cu_seqlens_k, (b + 1,), "cu_seqlens_k", dev)
+    if out is None:
+        out = torch.empty((total_q, h_q, d_v), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != (total_q, h_q, d_v) or out.device != dev:
+        raise RuntimeError(f"out must be {q.dtype} {[total_q, h_q, d_v]} on {dev}")
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        _rows16(t, name)
+    lse = torch.empty((total_q, h_q), dtype=torch.float32, device=dev)
+    if total_q == 0:
+        return out, lse
+    qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _strides(out)
+    p = GqaPrefillParams(_DTYPES[q.dtype], b, h_q, h_kv, d_qk, d_v, 1 if causal else 0, scale, total_q, total_k,
+                         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cq, ck,
+                         out.data_ptr(), os_[0], os_[1], lse.data_ptr())
+    with _on_device(dev):
+        check("dsv4b_gqa_prefill", lib.dsv4b_gqa_prefill(ctypes.byref(p), _stream(dev)))
+    return out, lse
+
+
+def gqa_cache_append(k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
+                     block_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor) -> None:
+    """Appends tokens to the cache: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1
+    of k and v (bf16 / fp16 [n, h_kv, d]) become the last positions of
+    sequence i, whose ``context_lens`` counts them already.
+
+    A block and head's scale is the smallest power of two (at least 2^-100)
+    that holds its largest value; a block with earlier positions keeps a
+    larger scale, or has them rounded again to the new one.  Infinities are
+    stored as +-448 of the finite values' scale, NaN as NaN.  No block may
+    be written by two sequences of one call."""
+    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = k_cache.device
+    for t, name in ((k, "k"), (v, "v")):
+        if t.dim() != 3 or t.dtype != k.dtype or t.dtype not in _DTYPES or t.shape != k.shape or \
+                t.shape[1:] != (c.h_kv, c.d) or t.device != dev:
+            raise RuntimeError(f"{name} must be bf16 / fp16 [n, {c.h_kv}, {c.d}] on {dev}")
+        _rows16(t, name)
+    cu = _int32(cu_seqlens, (c.b + 1,), "cu_seqlens", dev)
+    ks, vs = _strides(k), _strides(v)
+    with _on_device(dev):
+        check("dsv4b_gqa_cache_append",
+              lib.dsv4b_gqa_cache_append(ctypes.byref(c), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                         vs[0], vs[1], cu, k.size(0), _stream(dev)))
+
+
+_ws_bytes: dict = {}  # (device index, d) -> bytes
+
+
+def _decode_workspace(dev: torch.device, d: int) -> torch.Tensor:
+    n = _ws_bytes.get((dev.index, d))
+    if n is None:
+        size = ctypes.c_size_t()
+        check("dsv4b_gqa_decode_workspace_bytes",
+              lib.dsv4b_gqa_decode_workspace_bytes(dev.index, d, ctypes.byref(size)))
+        n = _ws_bytes[(dev.index, d)] = int(size.value)
+    # each call's own: calls on several streams, or captured in several graphs, share none
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def gqa_decode_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+                   sm_scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of each sequence's last s_q positions over the cache.
+
+    q bf16 / fp16 [b, s_q, h_q, d]; ``context_lens`` counts the queries' own
+    positions, and query x sees those up to its own.  Returns (out [b, s_q,
+    h_q, d] in q's type, lse fp32 [b, h_q, s_q], natural log); a query that
+    sees no position gets 0 and -inf."""
+    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = k_cache.device
+    qq = _query(q, c, sm_scale, dev)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev:
+        raise RuntimeError(f"out must be {q.dtype} {list(q.shape)} on {dev}")
+    else:
+        _rows16(out, "out")
+    lse = torch.empty((c.b, qq.h_q, qq.s_q), dtype=torch.float32, device=dev)
+    so = _strides(out)
+    with _on_device(dev):
+        ws = _decode_workspace(dev, c.d)
+        check("dsv4b_gqa_decode",
+              lib.dsv4b_gqa_decode(ctypes.byref(c), ctypes.byref(qq), out.data_ptr(), so[0], so[1], so[2],
+                                   lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+    return out, lse
+
+
+def gqa_attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
+                          block_table: torch.Tensor, context_lens: torch.Tensor, sm_scale: Optional[float] = None,
+                          weights: Optional[torch.Tensor] = None, accumulate: bool = False,
+                          max_context: Optional[int] = None) -> torch.Tensor:
+    """The attention weight that each cached position drew from ``q``, summed
+    over the queries and over the query heads of a KV head.
+
+    q and lse as for / from ``gqa_decode_fwd`` (a prompt's last queries, or
+    a decode step's).  Returns fp32 [b, h_kv, width]: ``weights`` if given,
+    which ``accumulate`` adds to (behind the context it is left as it was;
+    without ``accumulate`` zeros go there), else a new tensor of width
+    ``max_context`` (default: the block table's)."""
+    c = _cache(k_cache, None, k_scale, None, block_table, context_lens)
+    dev = k_cache.device
+    qq = _query(q, c, sm_scale, dev)
+    if lse.dtype != torch.float32 or lse.shape != (c.b, qq.h_q, qq.s_q) or not lse.is_contiguous() or lse.device != dev:
+        raise RuntimeError(f"lse must be contiguous float32 {[c.b, qq.h_q, qq.s_q]} on {dev}")
+    if weights is None:
+        _require(not accumulate, "accumulate needs weights to add to")
+        width = c.table_width * c.page_block_size if max_context is None else int(max_context)
+        _require(width > 0, "max_context must be positive")
+        weights = torch.empty((c.b, c.h_kv, width), dtype=torch.float32, device=dev)
+    else:
+        _require(max_context is None, "max_context is for a new tensor: weights has a width already")
+        _weights(weights, c, "weights", dev)
+    sb, sh, _ = _strides(weights)
+    with _on_device(dev):
+        check("dsv4b_gqa_attention_weights",
+              lib.dsv4b_gqa_attention_weights(ctypes.byref(c), ctypes.byref(qq), lse.data_ptr(), weights.data_ptr(), sb,
+                                              sh, weights.size(2), 1 if accumulate else 0, _stream(dev)))
+    return weights
+
+
+def _weights(t: torch.Tensor, c: GqaCache, name: str, dev: torch.device) -> None:
+    if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (c.b, c.h_kv) or t.size(2) < 1 or \
+            t.stride(2) != 1 or t.device != dev:
+        raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width] on {dev} with a contiguous last dim")
+
+
+def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    block_table: torch.Tensor, context_lens: torch.Tensor, weights: torch.Tensor, budget: int,
+                    recent: int, new_block_table: torch.Tensor, new_weights: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Keeps ``budget`` positions of every sequence and KV head, each head
+    its own: the newest ``recent``, and of the others those of the largest
+    ``weights`` (fp32 [b, h_kv, width]; equal ones: the lowest position
+    first), all of them where there are no more.  They become, in order, the
+    first positions of the blocks of ``new_block_table`` [b, >= ceil(budget /
+    P)], which must be blocks that the call does not read, none twice.
+
+    Returns (kept int32 [b, h_kv, budget], -1 behind the new length;
+    new_weights fp32 [b, h_kv, >= budget], the kept positions' weights, 0
+    behind; new context_lens int32 [b]).  The old blocks keep what they
+    hold."""
+    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = k_cache.device
+    budget, recent = int(budget), int(recent)
+    _require(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}: 0 <= recent <= budget, 1 <= budget")
+    _weights(weights, c, "weights", dev)
+    _table(new_block_table, c.b, "new_block_table", dev)
+    _require(new_block_table.data_ptr() != block_table.data_ptr(), "new_block_table must not be block_table")
+    _require(new_block_table.size(1) * c.page_block_size >= min(budget, weights.size(2), c.table_width * c.page_block_size),
+             "new_block_table has fewer blocks than the budget needs")
+    if new_weights is None:
+        new_weights = torch.empty((c.b, c.h_kv, budget), dtype=torch.float32, device=dev)
+    else:
+        _weights(new_weights, c, "new_weights", dev)
+        _require(new_weights.size(2) >= budget, "new_weights is narrower than the budget")
+        _require(new_weights.data_ptr() != weights.data_ptr(), "new_weights must not be weights")
+    kept = torch.empty((c.b, c.h_kv, budget), dtype=torch.int32, device=dev)
+    new_lens = torch.empty((c.b,), dtype=torch.int32, device=dev)
+    ws, ns = _strides(weights), _strides(new_weights)
+    p = GqaEvictParams(budget, recent, weights.data_ptr(), ws[0], ws[1], weights.size(2), new_weights.size(2),
+                       new_weights.data_ptr(), ns[0], ns[1], kept.data_ptr(), new_lens.data_ptr(),
+                       new_block_table.data_ptr(), new_block_table.stride(0), new_block_table.size(1))
+    with _on_device(dev):
+        check("dsv4b_gqa_cache_evict", lib.dsv4b_gqa_cache_evict(ctypes.byref(c), ctypes.byref(p), _stream(dev)))
+    return kept, new_weights, new_lens
+
+
+def gqa_status(device: Optional[torch.device] = None) -> int:
+    """Status word of the grouped-query kernels (0 = no error; 1 = a wait
+    timed out and a call's outputs are invalid); clears it.  Synchronises."""
+    device = device or torch.device("cuda", torch.cuda.current_device())
+    flags = ctypes.c_int()
+    with torch.cuda.device(device):
+        check("dsv4b_gqa_status", lib.dsv4b_gqa_status(ctypes.byref(flags), _stream(device)))
+    return int(flags.value)

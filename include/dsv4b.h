@@ -303,6 +303,149 @@ DSV4B_API int dsv4b_fp8_paged_mqa_logits(const dsv4b_mqa_logits_params* p, const
  * (0 = no error; 1 = a kernel wait hit its time limit).  Synchronises. */
 DSV4B_API int dsv4b_mqa_logits_status(int* flags, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Grouped-query attention with an 8-bit paged cache (the layers and draft
+ * models beside the latent-attention ones; the reference has none of it).
+ *
+ * Heads: h_q query heads share h_kv KV heads, h_q % h_kv == 0; query head
+ * h reads KV head h / (h_q / h_kv).
+ *
+ * Cache: K and V are e4m3 values [num_blocks, page_block_size, h_kv, d]
+ * with any strides (bytes, multiples of 16; d values contiguous) and one
+ * fp32 scale per (block, head) [num_blocks, h_kv]; a stored value stands
+ * for e4m3 * scale.  Position t of sequence i lies in block
+ * block_table[i][t / page_block_size], row t % page_block_size.  A block id
+ * that is negative or >= num_blocks, or past the table's width, holds
+ * nothing: reads leave its positions out, writes to it are skipped. */
+typedef struct dsv4b_gqa_cache {
+  void* k;                   /* e4m3 */
+  void* v;
+  float* k_scale;            /* [num_blocks, h_kv], contiguous */
+  float* v_scale;
+  int64_t stride_k_block, stride_k_row, stride_k_head; /* bytes */
+  int64_t stride_v_block, stride_v_row, stride_v_head;
+  int32_t num_blocks, page_block_size; /* page_block_size: a power of two, 16 .. 1024 */
+  int32_t h_kv, d;                     /* d in {64, 128}; h_kv <= 65535 */
+  const int32_t* block_table;          /* [b, table_width] */
+  int64_t stride_block_table;          /* elements between rows */
+  int32_t table_width, b;
+  const int32_t* context_lens;         /* [b] positions of each sequence */
+} dsv4b_gqa_cache;
+
+/* 16-bit floating types of q, k, v and out. */
+#define DSV4B_BF16 0
+#define DSV4B_FP16 1
+
+/* Attention over whole prompts of packed sequences.  Sequence i has the
+ * queries cu_seqlens_q[i] .. cu_seqlens_q[i + 1] - 1 and likewise keys.
+ *   out[t][h] = softmax_j(sm_scale * q[t][h] . k[j][h']) v[j][h']
+ * over its own keys; with causal, query x of n_q sees key j if
+ * j <= x + n_k - n_q (the last query sees every key).  lse is the natural
+ * log of the softmax's denominator, fp32 [total_q, h_q]; a query that sees
+ * no key gets out = 0 and lse = -inf.  Rows of q behind the last sequence
+ * are not touched.  (d_qk, d_v) in {(64, 64), (128, 128), (192, 128)};
+ * sm_scale > 0.  Element strides, multiples of 8; 16-byte aligned bases. */
+typedef struct dsv4b_gqa_prefill_params {
+  int32_t dtype;             /* DSV4B_BF16 / DSV4B_FP16, of q, k, v and out */
+  int32_t b, h_q, h_kv, d_qk, d_v, causal;
+  float sm_scale;
+  int64_t total_q, total_k;  /* rows of q / of k and v */
+  const void* q;             /* [total_q, h_q, d_qk] */
+  int64_t stride_q_t, stride_q_h;
+  const void* k;             /* [total_k, h_kv, d_qk] */
+  int64_t stride_k_t, stride_k_h;
+  const void* v;             /* [total_k, h_kv, d_v] */
+  int64_t stride_v_t, stride_v_h;
+  const int32_t* cu_seqlens_q; /* [b + 1] */
+  const int32_t* cu_seqlens_k; /* [b + 1] */
+  void* out;                 /* [total_q, h_q, d_v] */
+  int64_t stride_o_t, stride_o_h;
+  float* lse;                /* [total_q, h_q], contiguous */
+} dsv4b_gqa_prefill_params;
+
+DSV4B_API int dsv4b_gqa_prefill(const dsv4b_gqa_prefill_params* p, void* stream);
+
+/* Appends new tokens to the cache.  k and v are [n, h_kv, d] (dtype as
+ * above, element strides, multiples of 8); rows cu_seqlens[i] ..
+ * cu_seqlens[i + 1] - 1 become the last positions of sequence i, whose
+ * context_lens[i] counts them.  The scale of a block and head is 2^e, e =
+ * max(-100, ceil(log2(amax / 448))) over the finite values that the call
+ * writes there; a block that holds earlier positions keeps its scale if
+ * that is larger, otherwise those rows are rounded again to the new scale
+ * (value * (old / new), to nearest even).  Values are x / scale clamped to
+ * +-448, to nearest even; NaN stays NaN.  Rows behind a sequence's last
+ * position keep their bytes.  No block may be written by two sequences of
+ * one call. */
+DSV4B_API int dsv4b_gqa_cache_append(const dsv4b_gqa_cache* c, int dtype, const void* k, int64_t stride_k_t,
+                                     int64_t stride_k_h, const void* v, int64_t stride_v_t, int64_t stride_v_h,
+                                     const int32_t* cu_seqlens, int64_t n, void* stream);
+
+/* Queries over the cache: q [b, s_q, h_q, d], the sequences' last s_q
+ * positions; query x sees the positions t <= context_lens[i] - s_q + x.
+ * Element strides, multiples of 8. */
+typedef struct dsv4b_gqa_query {
+  int32_t dtype, s_q, h_q;
+  float sm_scale;            /* > 0 */
+  const void* q;
+  int64_t stride_q_b, stride_q_s, stride_q_h;
+} dsv4b_gqa_query;
+
+/* Device workspace of dsv4b_gqa_decode on `device` (partial results of
+ * sequences that several SMs share; no initial contents). */
+DSV4B_API int dsv4b_gqa_decode_workspace_bytes(int device, int d, size_t* bytes);
+
+/* Attention over the cache.  out [b, s_q, h_q, d] in q's type (element
+ * strides, multiples of 8), lse fp32 [b, h_q, s_q]; a query that sees no
+ * position gets out = 0 and lse = -inf. */
+DSV4B_API int dsv4b_gqa_decode(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, void* out, int64_t stride_o_b,
+                               int64_t stride_o_s, int64_t stride_o_h, float* lse, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* The attention weight that each cached position drew:
+ *   weights[i][h][t] (+)= sum over the queries x and query heads of KV
+ *                         head h of exp(sm_scale * q . k[t] - lse)
+ * lse fp32 [b, h_q, s_q] as dsv4b_gqa_decode returns it (-inf: the query
+ * adds nothing).  weights fp32 [b, h_kv, width] (element strides, unit last
+ * stride); accumulate = 1 adds to it at t < context_lens[i] and leaves the
+ * rest, 0 stores, with zeros behind the context.  Only K is read: v and
+ * v_scale may be NULL. */
+DSV4B_API int dsv4b_gqa_attention_weights(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, const float* lse,
+                                          float* weights, int64_t stride_w_b, int64_t stride_w_h, int32_t width,
+                                          int accumulate, void* stream);
+
+/* Eviction by attention weight.  For every sequence and KV head: where
+ * context_lens exceeds `budget`, the newest `recent` positions and, of the
+ * others, the heaviest ones are kept, `budget` in all (equal weights: the
+ * lowest position first; NaN counts as the largest); otherwise all.  The
+ * kept positions, in order, become positions 0, 1, ... of the blocks of
+ * new_table; a new block's scale is the largest scale that its rows had,
+ * and each value is rounded to nearest even after e4m3 * (old / new).
+ * Writes kept int32 [b, h_kv, budget] (-1 behind the new length),
+ * new_weights fp32 [b, h_kv, new_width >= budget] (0 behind it) and
+ * new_lens int32 [b] = min(context_lens, budget).  No block of new_table
+ * may be one that the call reads, or be there twice.  weights fp32 [b,
+ * h_kv, width]: a sequence counts as at most `width` positions long. */
+typedef struct dsv4b_gqa_evict_params {
+  int32_t budget, recent;    /* 0 <= recent <= budget, budget >= 1 */
+  const float* weights;
+  int64_t stride_w_b, stride_w_h;
+  int32_t width, new_width;
+  float* new_weights;
+  int64_t stride_nw_b, stride_nw_h;
+  int32_t* kept;             /* contiguous */
+  int32_t* new_lens;
+  const int32_t* new_table;  /* [b, new_table_width] */
+  int64_t stride_new_table;
+  int32_t new_table_width;
+} dsv4b_gqa_evict_params;
+
+DSV4B_API int dsv4b_gqa_cache_evict(const dsv4b_gqa_cache* c, const dsv4b_gqa_evict_params* e, void* stream);
+
+/* Reads (and clears) this device's status word of the grouped-query
+ * kernels (0 = no error; 1 = a kernel wait hit its time limit and the
+ * call's outputs are invalid).  Synchronises `stream`. */
+DSV4B_API int dsv4b_gqa_status(int* flags, void* stream);
+
 /* Reads (and clears) the kernel status word kept in the workspace into
  * *flags (0 = no error; bit 0 = a bounded wait ran out of time, the call's
  * outputs are then invalid).  Synchronises `stream`.  workspace = NULL
@@ -325,7 +468,9 @@ DSV4B_API int dsv4b_read_kernel_status(void* workspace, size_t workspace_bytes,
  *   DSV4B_STALL_KV_WRITE    KV-cache writer: the first chunk's copies
  *                           (status: dsv4b_kv_cache_write_status);
  *   DSV4B_STALL_MQA_LOGITS  indexer logits: the first page-id batch
- *                           (status: dsv4b_mqa_logits_status).
+ *                           (status: dsv4b_mqa_logits_status);
+ *   DSV4B_STALL_GQA         grouped-query prefill and decode: the first
+ *                           load's arrival (status: dsv4b_gqa_status).
  * A test sets a bit, runs the call (about 2-4 s), checks the status, then
  * clears the hook (kernels = 0).  Replaces nothing in the reference, whose
  * kernels have no bounded waits (csrc/common/defines.h:11-21 aborts the
@@ -333,6 +478,7 @@ DSV4B_API int dsv4b_read_kernel_status(void* workspace, size_t workspace_bytes,
 #define DSV4B_STALL_DECODE 1
 #define DSV4B_STALL_KV_WRITE 2
 #define DSV4B_STALL_MQA_LOGITS 4
+#define DSV4B_STALL_GQA 16
 DSV4B_API int dsv4b_set_test_stall(int kernels);
 
 /* Size of the library's built-in device scratch used by
