@@ -496,10 +496,11 @@ int dsv4b_gqa_prefill(const dsv4b_gqa_prefill_params* p, void* stream) {
       (p->total_q / 256 + p->b) * p->h_q > INT_MAX)
     return DSV4B_ERR_UNSUPPORTED;
   if (p->total_q == 0) return DSV4B_OK;
+  // tensor maps: no stride 0 (nor for `out`, whose rows are written)
   auto map_ok = [](const void* x, int64_t st, int64_t sh) {
-    return rows16(x, st, sh) && st * 2 < kMaxMapStride && sh * 2 < kMaxMapStride;
+    return rows16(x, st, sh) && st > 0 && sh > 0 && st < kMaxMapStride / 2 && sh < kMaxMapStride / 2;
   };
-  if (!map_ok(p->q, p->stride_q_t, p->stride_q_h) || !rows16(p->out, p->stride_o_t, p->stride_o_h))
+  if (!map_ok(p->q, p->stride_q_t, p->stride_q_h) || !map_ok(p->out, p->stride_o_t, p->stride_o_h))
     return DSV4B_ERR_INVALID_ARGUMENT;
   if (p->total_k && (!map_ok(p->k, p->stride_k_t, p->stride_k_h) || !map_ok(p->v, p->stride_v_t, p->stride_v_h)))
     return DSV4B_ERR_INVALID_ARGUMENT;
@@ -542,7 +543,7 @@ int dsv4b_gqa_decode(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, void* o
                      void* stream) {
   int rc = check_gqa_cache(c, true);
   if (rc || (rc = check_gqa_query(c, q))) return rc;
-  if (!rows16(out, stride_o_b, stride_o_s, stride_o_h) || !lse || !aligned(lse, 4)) return DSV4B_ERR_INVALID_ARGUMENT;
+  if (!rows16(out, stride_o_b, stride_o_s, stride_o_h) || !stride_o_b || !stride_o_s || !stride_o_h || !lse || !aligned(lse, 4)) return DSV4B_ERR_INVALID_ARGUMENT;
   int dev = 0;
   DevInfo* info = nullptr;
   if ((rc = current_arch_ok())) return rc;

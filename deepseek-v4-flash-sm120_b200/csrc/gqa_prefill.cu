@@ -57,7 +57,8 @@ namespace {
 
 constexpr int kM = 128;              // queries of a tile, keys of a tile
 constexpr int kQueries = 2 * kM;     // queries of a CTA
-constexpr int kThreads = 11 * 32;
+constexpr int kThreads = 12 * 32;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 64;  // of 168 at launch: 2 * 216 + 64 <= 3 * 168
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10;
 constexpr int kChunk = kM * 128;     // 128 rows x 64 16-bit columns, swizzled
 constexpr uint32_t kTmemCols = 512;
@@ -122,6 +123,33 @@ __host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
   constexpr uint32_t types = (1u << 7) | (1u << 10);  // A, B: bf16 (0: fp16)
   return std::is_same_v<T, __half> ? (idesc_bf16_f32(kM, n, false, b_mn_major) & ~types)
                                    : idesc_bf16_f32(kM, n, false, b_mn_major);
+}
+
+// Two fp32 at once (Blackwell's packed forms; each half an ordinary fp32 operation).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <typename T>
@@ -226,6 +254,8 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   volatile int* abort = &sh.abort;
   int* status = &g_gqa_prefill_status;
 
+  if (warp >= kMmaWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ---------------------------------------------------------------- loads
     if (lane == 0 && nt > 0) {
@@ -365,7 +395,9 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const long long t = clock64();
     while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------------------------------------------------------- softmax
     const int i = warp >> 2;  // query tile
     const int r = i * kM + (warp & 3) * 32 + lane;
@@ -388,15 +420,15 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 #pragma unroll
         for (int x = 0; x < kM; ++x) s[x] = x < left ? s[x] : -INFINITY;
       }
-      float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+      float t[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int x = 4; x < kM; x += 4) {
-        t0 = fmaxf(t0, s[x]);
-        t1 = fmaxf(t1, s[x + 1]);
-        t2 = fmaxf(t2, s[x + 2]);
-        t3 = fmaxf(t3, s[x + 3]);
+      for (int x = 4; x + 8 <= kM; x += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = max3(t[e], s[x + 2 * e], s[x + 2 * e + 1]);
       }
-      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+      t[0] = max3(t[0], s[kM - 4], s[kM - 3]);
+      t[1] = max3(t[1], s[kM - 2], s[kM - 1]);
+      const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
       const bool grew = (top - m) * c > kRescale;  // from -inf: always
       if (__any_sync(0xffffffffu, grew)) {
         const float f = grew ? fast_exp2((m - top) * c) : 1.f;
@@ -414,21 +446,24 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.f : m * c;
-      float l0 = 0.f, l1 = 0.f;
+      const float mc = m == -INFINITY ? 0.f : -m * c;
+      const uint64_t cc = pair(c, c), mm = pair(mc, mc);
+      uint64_t l2[2] = {0, 0};  // two pairs of zeros
 #pragma unroll
       for (int x = 0; x < kM; x += 32) {
         float p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float u = fast_exp2(fmaf(s[x + 2 * e], c, -mc)), v = fast_exp2(fmaf(s[x + 2 * e + 1], c, -mc));
-          l0 += u;
-          l1 += v;
-          p[e] = __uint_as_float(pack16<T>(u, v));
+          float2 u = unpair(fma2(pair(s[x + 2 * e], s[x + 2 * e + 1]), cc, mm));
+          u.x = fast_exp2(u.x);
+          u.y = fast_exp2(u.y);
+          l2[e & 1] = add2(l2[e & 1], pair(u.x, u.y));
+          p[e] = __uint_as_float(pack16<T>(u.x, u.y));
         }
         tmem_st16(s_t + x / 2, p);
       }
-      l += l0 + l1;
+      const float2 sum = unpair(add2(l2[0], l2[1]));
+      l += sum.x + sum.y;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&sh.p_full[i]);
@@ -494,9 +529,8 @@ bool make_map(CUtensorMap* m, const void* base, int64_t tokens, int heads, int d
               int dtype) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
   if (!enc) return false;
-  // strides of dims of size 1 (given as 0) are never used
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
-  const cuuint64_t strides[2] = {(cuuint64_t)(stride_h ? stride_h * 2 : d * 2), (cuuint64_t)(stride_t ? stride_t * 2 : d * 2)};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride_h * 2, (cuuint64_t)stride_t * 2};
   const cuuint32_t box[3] = {64, 1, kM};
   const cuuint32_t es[3] = {1, 1, 1};
   return enc(m, dtype == DSV4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
@@ -511,10 +545,10 @@ cudaError_t launch(const dsv4b_gqa_prefill_params& p, cudaStream_t stream, int* 
   // without a single key nothing is loaded: any valid map will do
   const bool keys = p.total_k > 0;
   if (!make_map(&tq, p.q, p.total_q, p.h_q, DQK, p.stride_q_t, p.stride_q_h, p.dtype) ||
-      !make_map(&tk, keys ? p.k : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DQK, keys ? p.stride_k_t : 0,
-                keys ? p.stride_k_h : 0, p.dtype) ||
-      !make_map(&tv, keys ? p.v : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DV, keys ? p.stride_v_t : 0,
-                keys ? p.stride_v_h : 0, p.dtype)) {
+      !make_map(&tk, keys ? p.k : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DQK, keys ? p.stride_k_t : DQK,
+                keys ? p.stride_k_h : DQK, p.dtype) ||
+      !make_map(&tv, keys ? p.v : p.q, keys ? p.total_k : 1, keys ? p.h_kv : 1, DV, keys ? p.stride_v_t : DV,
+                keys ? p.stride_v_h : DV, p.dtype)) {
     *bad_arg = 1;
     return cudaErrorInvalidValue;
   }

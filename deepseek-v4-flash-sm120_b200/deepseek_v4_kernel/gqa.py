@@ -27,12 +27,13 @@ for the exact contracts.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from ._lib import check, lib
-from .ops import _on_device, _stream
+from .ops import _on_device
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
@@ -81,89 +82,127 @@ class GqaPrefillParams(ctypes.Structure):
     ]
 
 
+# The structures are packed in one call each (a ctypes structure filled field
+# by field took a fifth of a decode call's host time).
+_CODES = {_i32: "i", _i64: "q", _f32: "f", _vp: "P"}
+
+
+def _packer(cls) -> struct.Struct:
+    return struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_))
+
+
+_PACK_CACHE, _PACK_QUERY = _packer(GqaCache).pack, _packer(GqaQuery).pack
+_PACK_EVICT, _PACK_PREFILL = _packer(GqaEvictParams).pack, _packer(GqaPrefillParams).pack
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(dev: torch.device) -> int:
+    """The current stream's handle (the public accessor takes 2 us of a call)."""
+    return torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None else _raw_stream(dev.index)
+
+
 def _require(ok: bool, message: str) -> None:
     if not ok:
         raise RuntimeError(message)
 
 
-def _int32(t: torch.Tensor, shape, name: str, dev: torch.device) -> int:
-    """Pointer of a contiguous int32 tensor of this shape."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {dev}, got "
+def _int32(t: torch.Tensor, n: int, name: str, dev: torch.device) -> int:
+    """Pointer of a contiguous int32 tensor of n elements."""
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape {(n,)} on {dev}, got "
                            f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, b: int, name: str, dev: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.size(0) != b or t.size(1) < 1 or t.device != dev or \
-            (t.size(1) > 1 and t.stride(1) != 1):
-        raise RuntimeError(f"{name} must be int32 [{b}, blocks] on {dev} with a contiguous last dim")
+def _table(t: torch.Tensor, b: int, name: str, dev: torch.device):
+    """Pointer, row stride and width of a block table."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.device != dev:
+        raise RuntimeError(f"{name} must be int32 [b, blocks] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    n, width = t.shape
+    stride, unit = t.stride()
+    if n != b or width < 1 or (unit != 1 and width > 1):
+        raise RuntimeError(f"{name} must be int32 [{b}, blocks] with a contiguous last dim, got {tuple(t.shape)}")
+    return t.data_ptr(), stride, width
 
 
-def _rows16(t: torch.Tensor, name: str) -> None:
-    """Rows that the kernels read or write 16 bytes at a time."""
-    st = t.stride()
-    if st[-1] != 1 or any(s % 8 and n > 1 for s, n in zip(st[:-1], t.shape)) or t.data_ptr() % 16:
-        raise RuntimeError(f"{name} needs a contiguous last dim, other strides in multiples of 8 elements and a "
-                           f"16-byte aligned base, got strides {st}")
-
-
-def _strides(t: torch.Tensor):
-    """Strides with those of size-1 dims (which no address uses) made 0."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+def _rows16(t: torch.Tensor, name: str, distinct: bool = False):
+    """Pointer and strides of a tensor whose rows are read or written 16 bytes
+    at a time; ``distinct``: no two rows may be the same memory."""
+    ptr, st = t.data_ptr(), t.stride()
+    bits = 0
+    for x in st[:-1]:
+        bits |= x & 7
+    if bits or st[-1] != 1 or ptr & 15 or (distinct and 0 in st):
+        # strides of dims of one element are never used
+        st = [x if n > 1 else 8 for x, n in zip(st[:-1], t.shape)] + [st[-1]]
+        if st[-1] != 1 or any(x % 8 for x in st[:-1]) or ptr % 16 or (distinct and 0 in st):
+            raise RuntimeError(f"{name} needs a contiguous last dim, other strides in multiples of 8 elements (not 0, if "
+                               f"it is written to or loaded by tiles) and a 16-byte aligned base, got strides {t.stride()}")
+    return ptr, st
 
 
 def _fp8_cache(t: torch.Tensor, scale: torch.Tensor, name: str, dev: torch.device):
-    """The three byte strides of a cache tensor, checked with its scales."""
+    """The pointers and the three byte strides of a cache tensor and its scales."""
     if t.dtype not in _FP8 or t.dim() != 4 or t.device != dev:
         raise RuntimeError(f"{name}_cache must be float8_e4m3fn / uint8 [num_blocks, P, h_kv, d] on {dev}")
     nb, page, h, d = t.shape
-    _require(nb > 0 and h > 0, f"{name}_cache has no blocks or heads")
-    _require(page in (16, 32, 64, 128, 256, 512, 1024), f"block size {page}: a power of two from 16 to 1024 is supported")
-    _require(d in (64, 128), f"d = {d}: 64 or 128 is supported")
-    sb, sr, sh, sd = t.stride()
-    if nb == 1:  # size-1 dims: any stride will do
-        sb = max(page * sr, d)
-    if h == 1:
-        sh = max(sr, d)
-    if sd != 1 or sb % 16 or sr % 16 or sh % 16 or min(sb, sr, sh) < d or t.data_ptr() % 16:
+    ptr, (sb, sr, sh, sd) = t.data_ptr(), t.stride()
+    if nb <= 1 or h <= 1:  # dims of one element: any stride will do
+        _require(nb > 0 and h > 0, f"{name}_cache has no blocks or heads")
+        sb = sb if nb > 1 else max(page * sr, d)
+        sh = sh if h > 1 else max(sr, d)
+    if sd != 1 or (sb | sr | sh | ptr) & 15 or min(sb, sr, sh) < d:
         raise RuntimeError(f"{name}_cache needs a contiguous last dim, other strides in multiples of 16 bytes and a "
                            f"16-byte aligned base, got strides {t.stride()}")
     if scale.dtype != torch.float32 or scale.shape != (nb, h) or not scale.is_contiguous() or scale.device != dev:
         raise RuntimeError(f"{name}_scale must be contiguous float32 {[nb, h]} on {dev}")
-    return sb, sr, sh
+    return ptr, scale.data_ptr(), sb, sr, sh
 
 
-def _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens) -> GqaCache:
-    dev = k_cache.device
-    _require(k_cache.is_cuda, "the cache must be a CUDA tensor")
-    b = context_lens.numel()
-    _require(b > 0, "context_lens is empty")
-    ctx = _int32(context_lens, (b,), "context_lens", dev)
-    _table(block_table, b, "block_table", dev)
-    kb, kr, kh = _fp8_cache(k_cache, k_scale, "k", dev)
-    v = vs = None
-    vb = vr = vh = 0
-    if v_cache is not None:
-        _require(v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape")
-        vb, vr, vh = _fp8_cache(v_cache, v_scale, "v", dev)
-        v, vs = v_cache.data_ptr(), v_scale.data_ptr()
-    nb, page, h, d = k_cache.shape
-    return GqaCache(k_cache.data_ptr(), v, k_scale.data_ptr(), vs, kb, kr, kh, vb, vr, vh, nb, page, h, d,
-                    block_table.data_ptr(), block_table.stride(0), block_table.size(1), b, ctx)
+class _Cache:
+    """A checked cache: its packed structure, and the sizes that the calls need."""
+
+    __slots__ = ("packed", "dev", "b", "page", "h_kv", "d", "width", "table_ptr")
+
+    def __init__(self, k_cache, v_cache, k_scale, v_scale, block_table, context_lens):
+        dev = self.dev = k_cache.device
+        _require(k_cache.is_cuda, "the cache must be a CUDA tensor")
+        b = self.b = context_lens.numel()
+        _require(b > 0, "context_lens is empty")
+        ctx = _int32(context_lens, b, "context_lens", dev)
+        self.table_ptr, stride, self.width = _table(block_table, b, "block_table", dev)
+        k, ks, kb, kr, kh = _fp8_cache(k_cache, k_scale, "k", dev)
+        shape = k_cache.shape
+        if v_cache is None:
+            v = vs = vb = vr = vh = 0
+        else:
+            if v_cache.shape != shape:
+                raise RuntimeError("k_cache and v_cache must have one shape")
+            v, vs, vb, vr, vh = _fp8_cache(v_cache, v_scale, "v", dev)
+        nb, self.page, self.h_kv, self.d = shape
+        if self.page not in _PAGES or self.d not in (64, 128):
+            raise RuntimeError(f"blocks of {self.page} positions, d {self.d}: a power of two from 16 to 1024, and 64 or "
+                               "128, are supported")
+        self.packed = _PACK_CACHE(k, v, ks, vs, kb, kr, kh, vb, vr, vh, nb, self.page, self.h_kv, self.d,
+                                  self.table_ptr, stride, self.width, b, ctx)
 
 
-def _query(q, c: GqaCache, sm_scale: Optional[float], dev: torch.device) -> GqaQuery:
-    if q.dim() != 4 or q.dtype not in _DTYPES or q.device != dev:
-        raise RuntimeError("q must be bf16 / fp16 [b, s_q, h_q, d] on the cache's device")
+_PAGES = (16, 32, 64, 128, 256, 512, 1024)
+
+
+def _query(q, c: _Cache, sm_scale: Optional[float]):
+    """The packed query, s_q and h_q."""
+    if q.dim() != 4 or q.dtype not in _DTYPES or q.device != c.dev:
+        raise RuntimeError(f"q must be bf16 / fp16 [b, s_q, h_q, d] on {c.dev}")
     b, s_q, h_q, d = q.shape
-    _require(b == c.b and d == c.d and s_q > 0, f"q {tuple(q.shape)} does not match {c.b} sequences of d {c.d}")
-    _require(h_q > 0 and h_q % c.h_kv == 0, f"{h_q} query heads are not a multiple of {c.h_kv} KV heads")
-    _rows16(q, "q")
+    if b != c.b or d != c.d or s_q < 1 or h_q < 1 or h_q % c.h_kv:
+        raise RuntimeError(f"q {tuple(q.shape)} does not match {c.b} sequences, {c.h_kv} KV heads, d {c.d}")
+    ptr, st = _rows16(q, "q")
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
-    _require(0.0 < scale < float("inf"), f"sm_scale must be positive, got {scale}")
-    sb, ss, sh, _ = _strides(q)
-    return GqaQuery(_DTYPES[q.dtype], s_q, h_q, scale, q.data_ptr(), sb, ss, sh)
+    if not 0.0 < scale < float("inf"):
+        raise RuntimeError(f"sm_scale must be positive, got {scale}")
+    return _PACK_QUERY(_DTYPES[q.dtype], s_q, h_q, scale, ptr, st[0], st[1], st[2]), s_q, h_q
 
 
 def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -186,35 +225,37 @@ def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
             raise RuntimeError(f"{name} must be bf16 / fp16 [tokens, heads, d], as q is, on {dev}")
     total_q, h_q, d_qk = q.shape
     total_k, h_kv, d_v = v.shape
-    _require(k.shape == (total_k, h_kv, d_qk), f"k {tuple(k.shape)} does not match q {tuple(q.shape)} and v {tuple(v.shape)}")
-    _require((d_qk, d_v) in ((64, 64), (128, 128), (192, 128)), f"(d_qk, d_v) = {(d_qk, d_v)}: (64, 64), (128, 128) "
-             "or (192, 128) is supported")
-    _require(h_kv > 0 and h_q > 0 and h_q % h_kv == 0, f"{h_q} query heads are not a multiple of {h_kv} KV heads")
+    _require(k.shape == (total_k, h_kv, d_qk), "k does not match q and v")
+    if (d_qk, d_v) not in ((64, 64), (128, 128), (192, 128)):
+        raise RuntimeError(f"(d_qk, d_v) = {(d_qk, d_v)}: (64, 64), (128, 128) or (192, 128) is supported")
+    if h_kv < 1 or h_q < 1 or h_q % h_kv:
+        raise RuntimeError(f"{h_q} query heads are not a multiple of {h_kv} KV heads")
     scale = d_qk ** -0.5 if sm_scale is None else float(sm_scale)
-    _require(0.0 < scale < float("inf"), f"sm_scale must be positive, got {scale}")
+    if not 0.0 < scale < float("inf"):
+        raise RuntimeError(f"sm_scale must be positive, got {scale}")
     b = cu_seqlens_q.numel() - 1
     _require(b >= 1, "cu_seqlens_q must have b + 1 >= 2 entries")
-    cq = _int32(cu_seqlens_q, (b + 1,), "cu_seqlens_q", dev)
+    cq = _int32(cu_seqlens_q, b + 1, "cu_seqlens_q", dev)
     if cu_seqlens_k is None:
         _require(total_k == total_q, "k and q have different lengths: pass cu_seqlens_k")
         ck = cq
     else:
-        ck = _int32(cu_seqlens_k, (b + 1,), "cu_seqlens_k", dev)
+        ck = _int32(cu_seqlens_k, b + 1, "cu_seqlens_k", dev)
     if out is None:
-        out = torch.empty((total_q, h_q, d_v), dtype=q.dtype, device=dev)
+        out = q.new_empty((total_q, h_q, d_v))
     elif out.dtype != q.dtype or out.shape != (total_q, h_q, d_v) or out.device != dev:
         raise RuntimeError(f"out must be {q.dtype} {[total_q, h_q, d_v]} on {dev}")
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        _rows16(t, name)
     lse = torch.empty((total_q, h_q), dtype=torch.float32, device=dev)
     if total_q == 0:
         return out, lse
-    qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _strides(out)
-    p = GqaPrefillParams(_DTYPES[q.dtype], b, h_q, h_kv, d_qk, d_v, 1 if causal else 0, scale, total_q, total_k,
-                         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cq, ck,
-                         out.data_ptr(), os_[0], os_[1], lse.data_ptr())
+    qp, qs = _rows16(q, "q", True)
+    kp, ks = _rows16(k, "k", True)
+    vp, vs = _rows16(v, "v", True)
+    op, os_ = _rows16(out, "out", True)
+    p = _PACK_PREFILL(_DTYPES[q.dtype], b, h_q, h_kv, d_qk, d_v, 1 if causal else 0, scale, total_q, total_k, qp, qs[0],
+                      qs[1], kp, ks[0], ks[1], vp, vs[0], vs[1], cq, ck, op, os_[0], os_[1], lse.data_ptr())
     with _on_device(dev):
-        check("dsv4b_gqa_prefill", lib.dsv4b_gqa_prefill(ctypes.byref(p), _stream(dev)))
+        check("dsv4b_gqa_prefill", lib.dsv4b_gqa_prefill(p, _stream(dev)))
     return out, lse
 
 
@@ -230,19 +271,19 @@ def gqa_cache_append(k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
     larger scale, or has them rounded again to the new one.  Infinities are
     stored as +-448 of the finite values' scale, NaN as NaN.  No block may
     be written by two sequences of one call."""
-    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
-    dev = k_cache.device
-    for t, name in ((k, "k"), (v, "v")):
-        if t.dim() != 3 or t.dtype != k.dtype or t.dtype not in _DTYPES or t.shape != k.shape or \
-                t.shape[1:] != (c.h_kv, c.d) or t.device != dev:
-            raise RuntimeError(f"{name} must be bf16 / fp16 [n, {c.h_kv}, {c.d}] on {dev}")
-        _rows16(t, name)
-    cu = _int32(cu_seqlens, (c.b + 1,), "cu_seqlens", dev)
-    ks, vs = _strides(k), _strides(v)
+    c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = c.dev
+    n = k.size(0)
+    if k.dim() != 3 or k.dtype not in _DTYPES or v.dtype != k.dtype or k.shape != (n, c.h_kv, c.d) or \
+            v.shape != k.shape or k.device != dev or v.device != dev:
+        raise RuntimeError(f"k and v must be bf16 / fp16 [n, {c.h_kv}, {c.d}] on {dev}")
+    kp, ks = _rows16(k, "k")
+    vp, vs = _rows16(v, "v")
+    cu = _int32(cu_seqlens, c.b + 1, "cu_seqlens", dev)
     with _on_device(dev):
         check("dsv4b_gqa_cache_append",
-              lib.dsv4b_gqa_cache_append(ctypes.byref(c), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1], v.data_ptr(),
-                                         vs[0], vs[1], cu, k.size(0), _stream(dev)))
+              lib.dsv4b_gqa_cache_append(c.packed, _DTYPES[k.dtype], kp, ks[0], ks[1], vp, vs[0], vs[1], cu, n,
+                                         _stream(dev)))
 
 
 _ws_bytes: dict = {}  # (device index, d) -> bytes
@@ -269,22 +310,20 @@ def gqa_decode_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     positions, and query x sees those up to its own.  Returns (out [b, s_q,
     h_q, d] in q's type, lse fp32 [b, h_q, s_q], natural log); a query that
     sees no position gets 0 and -inf."""
-    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
-    dev = k_cache.device
-    qq = _query(q, c, sm_scale, dev)
+    c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = c.dev
+    qq, s_q, h_q = _query(q, c, sm_scale)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev:
         raise RuntimeError(f"out must be {q.dtype} {list(q.shape)} on {dev}")
-    else:
-        _rows16(out, "out")
-    lse = torch.empty((c.b, qq.h_q, qq.s_q), dtype=torch.float32, device=dev)
-    so = _strides(out)
+    op, so = _rows16(out, "out", True)
+    lse = torch.empty((c.b, h_q, s_q), dtype=torch.float32, device=dev)
     with _on_device(dev):
         ws = _decode_workspace(dev, c.d)
         check("dsv4b_gqa_decode",
-              lib.dsv4b_gqa_decode(ctypes.byref(c), ctypes.byref(qq), out.data_ptr(), so[0], so[1], so[2],
-                                   lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)))
+              lib.dsv4b_gqa_decode(c.packed, qq, op, so[0], so[1], so[2], lse.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   _stream(dev)))
     return out, lse
 
 
@@ -300,31 +339,35 @@ def gqa_attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Ten
     which ``accumulate`` adds to (behind the context it is left as it was;
     without ``accumulate`` zeros go there), else a new tensor of width
     ``max_context`` (default: the block table's)."""
-    c = _cache(k_cache, None, k_scale, None, block_table, context_lens)
-    dev = k_cache.device
-    qq = _query(q, c, sm_scale, dev)
-    if lse.dtype != torch.float32 or lse.shape != (c.b, qq.h_q, qq.s_q) or not lse.is_contiguous() or lse.device != dev:
-        raise RuntimeError(f"lse must be contiguous float32 {[c.b, qq.h_q, qq.s_q]} on {dev}")
+    c = _Cache(k_cache, None, k_scale, None, block_table, context_lens)
+    dev = c.dev
+    qq, s_q, h_q = _query(q, c, sm_scale)
+    if lse.dtype != torch.float32 or lse.shape != (c.b, h_q, s_q) or not lse.is_contiguous() or lse.device != dev:
+        raise RuntimeError(f"lse must be contiguous float32 {[c.b, h_q, s_q]} on {dev}")
     if weights is None:
         _require(not accumulate, "accumulate needs weights to add to")
-        width = c.table_width * c.page_block_size if max_context is None else int(max_context)
+        width = c.width * c.page if max_context is None else int(max_context)
         _require(width > 0, "max_context must be positive")
         weights = torch.empty((c.b, c.h_kv, width), dtype=torch.float32, device=dev)
     else:
         _require(max_context is None, "max_context is for a new tensor: weights has a width already")
-        _weights(weights, c, "weights", dev)
-    sb, sh, _ = _strides(weights)
+        width = _weights(weights, c, "weights", True)
+    sb, sh, _ = weights.stride()
     with _on_device(dev):
         check("dsv4b_gqa_attention_weights",
-              lib.dsv4b_gqa_attention_weights(ctypes.byref(c), ctypes.byref(qq), lse.data_ptr(), weights.data_ptr(), sb,
-                                              sh, weights.size(2), 1 if accumulate else 0, _stream(dev)))
+              lib.dsv4b_gqa_attention_weights(c.packed, qq, lse.data_ptr(), weights.data_ptr(), sb, sh, width,
+                                              1 if accumulate else 0, _stream(dev)))
     return weights
 
 
-def _weights(t: torch.Tensor, c: GqaCache, name: str, dev: torch.device) -> None:
+def _weights(t: torch.Tensor, c: _Cache, name: str, written: bool) -> int:
+    """The width of a weights tensor."""
     if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (c.b, c.h_kv) or t.size(2) < 1 or \
-            t.stride(2) != 1 or t.device != dev:
-        raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width] on {dev} with a contiguous last dim")
+            t.stride(2) != 1 or t.device != c.dev:
+        raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width] on {c.dev} with a contiguous last dim")
+    if written and any(s < t.size(2) and n > 1 for s, n in zip(t.stride()[:2], t.shape)):
+        raise RuntimeError(f"{name}'s rows overlap: strides {t.stride()}")
+    return t.size(2)
 
 
 def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -342,29 +385,30 @@ def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch
     new_weights fp32 [b, h_kv, >= budget], the kept positions' weights, 0
     behind; new context_lens int32 [b]).  The old blocks keep what they
     hold."""
-    c = _cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
-    dev = k_cache.device
+    c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
+    dev = c.dev
     budget, recent = int(budget), int(recent)
-    _require(budget >= 1 and 0 <= recent <= budget, f"budget {budget}, recent {recent}: 0 <= recent <= budget, 1 <= budget")
-    _weights(weights, c, "weights", dev)
-    _table(new_block_table, c.b, "new_block_table", dev)
-    _require(new_block_table.data_ptr() != block_table.data_ptr(), "new_block_table must not be block_table")
-    _require(new_block_table.size(1) * c.page_block_size >= min(budget, weights.size(2), c.table_width * c.page_block_size),
+    if budget < 1 or not 0 <= recent <= budget:
+        raise RuntimeError(f"budget {budget}, recent {recent}: 0 <= recent <= budget, 1 <= budget")
+    width = _weights(weights, c, "weights", False)
+    new_table, new_stride, new_blocks = _table(new_block_table, c.b, "new_block_table", dev)
+    _require(new_table != c.table_ptr, "new_block_table must not be block_table")
+    _require(new_blocks * c.page >= min(budget, width, c.width * c.page),
              "new_block_table has fewer blocks than the budget needs")
     if new_weights is None:
+        new_width = budget
         new_weights = torch.empty((c.b, c.h_kv, budget), dtype=torch.float32, device=dev)
     else:
-        _weights(new_weights, c, "new_weights", dev)
-        _require(new_weights.size(2) >= budget, "new_weights is narrower than the budget")
+        new_width = _weights(new_weights, c, "new_weights", True)
+        _require(new_width >= budget, "new_weights is narrower than the budget")
         _require(new_weights.data_ptr() != weights.data_ptr(), "new_weights must not be weights")
     kept = torch.empty((c.b, c.h_kv, budget), dtype=torch.int32, device=dev)
     new_lens = torch.empty((c.b,), dtype=torch.int32, device=dev)
-    ws, ns = _strides(weights), _strides(new_weights)
-    p = GqaEvictParams(budget, recent, weights.data_ptr(), ws[0], ws[1], weights.size(2), new_weights.size(2),
-                       new_weights.data_ptr(), ns[0], ns[1], kept.data_ptr(), new_lens.data_ptr(),
-                       new_block_table.data_ptr(), new_block_table.stride(0), new_block_table.size(1))
+    ws, ns = weights.stride(), new_weights.stride()
+    p = _PACK_EVICT(budget, recent, weights.data_ptr(), ws[0], ws[1], width, new_width, new_weights.data_ptr(), ns[0],
+                    ns[1], kept.data_ptr(), new_lens.data_ptr(), new_table, new_stride, new_blocks)
     with _on_device(dev):
-        check("dsv4b_gqa_cache_evict", lib.dsv4b_gqa_cache_evict(ctypes.byref(c), ctypes.byref(p), _stream(dev)))
+        check("dsv4b_gqa_cache_evict", lib.dsv4b_gqa_cache_evict(c.packed, p, _stream(dev)))
     return kept, new_weights, new_lens
 
 

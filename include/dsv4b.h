@@ -344,7 +344,8 @@ typedef struct dsv4b_gqa_cache {
  * log of the softmax's denominator, fp32 [total_q, h_q]; a query that sees
  * no key gets out = 0 and lse = -inf.  Rows of q behind the last sequence
  * are not touched.  (d_qk, d_v) in {(64, 64), (128, 128), (192, 128)};
- * sm_scale > 0.  Element strides, multiples of 8; 16-byte aligned bases. */
+ * sm_scale > 0.  Element strides, positive multiples of 8 (of a dim of one
+ * element too); 16-byte aligned bases. */
 typedef struct dsv4b_gqa_prefill_params {
   int32_t dtype;             /* DSV4B_BF16 / DSV4B_FP16, of q, k, v and out */
   int32_t b, h_q, h_kv, d_qk, d_v, causal;
@@ -395,7 +396,7 @@ typedef struct dsv4b_gqa_query {
 DSV4B_API int dsv4b_gqa_decode_workspace_bytes(int device, int d, size_t* bytes);
 
 /* Attention over the cache.  out [b, s_q, h_q, d] in q's type (element
- * strides, multiples of 8), lse fp32 [b, h_q, s_q]; a query that sees no
+ * strides, positive multiples of 8), lse fp32 [b, h_q, s_q]; a query that sees no
  * position gets out = 0 and lse = -inf. */
 DSV4B_API int dsv4b_gqa_decode(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, void* out, int64_t stride_o_b,
                                int64_t stride_o_s, int64_t stride_o_h, float* lse, void* workspace,
