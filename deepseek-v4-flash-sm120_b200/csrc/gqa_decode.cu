@@ -6,41 +6,46 @@
 //   out[r]  = sum_t exp(s[r][t] - lse[r]) * v_scale * v[t]
 // for the rows r = (query, head) that share a KV head: h_q / h_kv * s_q of
 // them, few against the positions.  Every cached byte is used for all rows
-// at once and only once, so the kernel is bound by the cache's bytes.
+// at once and only once, so the kernels are bound by the cache's bytes.
 //
-// Work.  A unit is 32 positions of one (sequence, KV head, group of 16
+// Work.  A unit is 32 positions of one (sequence, KV head, group of 8 or 16
 // rows).  All units stand in one list, and every warp of the grid (one CTA
-// of eight warps per SM) takes an equal, contiguous piece of it, so ragged
-// batches balance without a plan made ahead.  A warp runs the softmax of its
-// piece by itself: no barrier until its CTA's end, where pieces of one
-// (sequence, head, group) are joined; those that reach over CTAs are joined
-// by a second kernel.
+// per SM) takes an equal, contiguous piece of it, so ragged batches balance
+// without a plan made ahead.  A warp runs the softmax of its piece by
+// itself: no barrier until its CTA's end, where pieces of one (sequence,
+// head, group) are joined; those that reach over CTAs are joined by a second
+// kernel.
 //
-// Loads.  Each warp has its own ring of two stages (32 positions of K and of
-// V, 8 KB at d = 128), filled by TMA tiled loads that swizzle the rows and
-// counted on an mbarrier: 128 KB are in flight on an SM, without a register
-// or an issue slot spent on them.
+// Loads.  Each warp has its own ring of 32-position tiles, K and V in turn
+// (4 KB each at d = 128), filled by TMA tiled loads that swizzle the rows
+// and counted on mbarriers: up to 192 KB are in flight on an SM, without a
+// register or an issue slot spent on them.
 //
-// Products.  mma.sync m16n8k16 with fp16 operands, the 16 rows as M.  The
-// operands of tcgen05 would have to stand in shared memory in their final
-// type, so e4m3 would be widened into shared memory (twice its bytes written
-// and read again) for 16 useful rows of 128; mma.sync takes them from
+// Products.  mma.sync m16n8k16 with fp16 operands, positions (or dims of V)
+// as M and rows as N = 8: s^T = k q^T, out^T = v^T p^T.  The operands of
+// tcgen05 would have to stand in shared memory in their final type, so e4m3
+// would be widened into shared memory (twice its bytes written and read
+// again) for a tile of which 8 rows are used; mma.sync takes them from
 // registers, where an e4m3 pair becomes an fp16 pair (exactly) in one
-// instruction, and its rate is far above what the loads can feed.  The order
-// of d in q.k and of the positions in p.v is free, so the fragments are
-// built from 16-byte pieces of whole rows:
-//   K: thread (j, c) of a quad reads bytes [16c, 16c + 16) (and 64 further)
-//      of position perm(j): four k-steps, with q laid out to match;
-//   V: it reads 16 bytes of column piece col(j) of the four positions whose
-//      p it holds, and interleaves the bytes of two positions.
-// perm and col make every such read free of bank conflicts (below).
+// instruction, and its rate (974 multiply-adds a cycle and SM, measured) is
+// above what the loads can feed.  The order of d in q.k and of the positions
+// in p.v is free, so the fragments are built from 16-byte pieces of whole
+// rows, thread (g, c) = (lane / 4, lane % 4):
+//   K: it reads bytes [16c, 16c + 16) (and 64 further) of the positions
+//      perm(g) and 8 + perm(g): four k-steps, with q laid out to match;
+//   V: it reads the 16 dims from col(g) on of the four positions perm(2c),
+//      perm(2c + 1) and 8 further, and interleaves the bytes of two.
+// perm and col make every such read free of bank conflicts (below).  s^T
+// has a position per g and rows 2c, 2c + 1 in a thread; transposing its 8x8
+// blocks (movmatrix) gives p^T's fragments.
 //
 // Numbers.  q is scaled by a power of two per row so that fp16 holds it
 // (bf16 has fewer digits; what lies 2^-27 below the row's largest is lost).
-// p <= 1 is rounded to fp16 for p.v (2^-11 of each term), sums and the
+// The running maximum m is moved only when a score outgrows it by 2^8, so p
+// <= 2^8; p is rounded to fp16 for p.v (2^-11 of each term), sums and the
 // softmax's denominator are fp32 of the unrounded p.  The accumulator is
-// kept in units of the current block's v_scale and rescaled when that or
-// the running maximum changes, so that no scale enters an fp16.
+// kept in units of the current block's v_scale and rescaled when that or m
+// changes, so that no scale enters an fp16.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -64,17 +69,14 @@ __device__ int g_gqa_test_stall = 0;
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kUnit = 32;   // positions of a unit
-constexpr int kRows = 16;   // rows of a group (M of the MMA)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;  // log2 of how far m may be outgrown
 
 struct GqaArgs {
   const void* q;
   int64_t stride_q_b, stride_q_s, stride_q_h;
-  int s_q, h_q, h_kv, g, groups;  // g = h_q / h_kv; groups of 16 rows per KV head
+  int s_q, h_q, h_kv, g, groups;  // g = h_q / h_kv; groups of rows per KV head
   float scale_log2;               // sm_scale * log2(e)
   const float* k_scale;
   const float* v_scale;
@@ -94,13 +96,15 @@ struct GqaArgs {
   int width, accumulate;
 };
 
-// Positions of sequence i that the call reads, and its context length.
+// Positions of sequence i that the call reads.
 __device__ __forceinline__ int held_len(const GqaArgs& a, int i) {
   const int64_t room = (int64_t)a.table_width * a.page;
   return (int)min((int64_t)max(__ldg(a.ctx + i), 0), room);
 }
-__device__ __forceinline__ int units_of(const GqaArgs& a, int i) {
-  return max(1, (held_len(a, i) + kUnit - 1) / kUnit);  // an empty sequence has its outputs written too
+// Its units of U positions (one at least: an empty sequence has its outputs written too).
+template <int U>
+__device__ __forceinline__ int units_of(int len) {
+  return max(1, (len + U - 1) / U);
 }
 
 // ------------------------------------------------------------------ layouts
@@ -110,23 +114,23 @@ template <int D>
 struct Lay;
 template <>
 struct Lay<128> {
-  static constexpr int kStages = 2;
-  // A quarter of a warp's 16-byte reads (8 threads) is j, j + 1 with all c
-  // for K, and for V.  Rows that differ in bit 2 swap the halves of the row,
-  // so K wants perm(2j), perm(2j + 1) four apart and V wants col(2j),
-  // col(2j + 1) four pieces apart.
-  static __device__ __forceinline__ int perm(int j) { return (j >> 1) | ((j & 1) << 2); }
-  static __device__ __forceinline__ int col(int j) { return ((j >> 1) | ((j & 1) << 2)) * 16; }  // dims [col, col + 16)
+  // A quarter of a warp's 16-byte reads (8 threads) is g, g + 1 with all c,
+  // for K and for V.  Rows that differ in bit 2 swap the halves of the row,
+  // so K wants perm(2i), perm(2i + 1) four apart and V wants col(2i),
+  // col(2i + 1) four pieces apart.
+  static __device__ __forceinline__ int perm(int i) { return (i >> 1) | ((i & 1) << 2); }
+  static __device__ __forceinline__ int unperm(int t) { return ((t & 3) << 1) | (t >> 2); }
+  static __device__ __forceinline__ int col(int i) { return ((i >> 1) | ((i & 1) << 2)) * 16; }  // dims [col, col + 16)
   static __device__ __forceinline__ uint32_t piece(int row, int p) { return row * 128 + ((p ^ (row & 7)) << 4); }
 };
 template <>
 struct Lay<64> {
-  static constexpr int kStages = 4;
   // Two rows share 128 bytes, the odd one in the upper half: K wants
-  // perm(2j), perm(2j + 1) of different parity, V (8-byte reads, 16 threads
+  // perm(2i), perm(2i + 1) of different parity, V (8-byte reads, 16 threads
   // at once) wants perm(0), perm(2), perm(4), perm(6) of changing parity.
-  static __device__ __forceinline__ int perm(int j) { return j ^ ((j >> 1) & 1); }
-  static __device__ __forceinline__ int col(int j) { return j * 8; }  // dims [col, col + 8)
+  static __device__ __forceinline__ int perm(int i) { return i ^ ((i >> 1) & 1); }
+  static __device__ __forceinline__ int unperm(int t) { return t ^ ((t >> 1) & 1); }
+  static __device__ __forceinline__ int col(int i) { return i * 8; }  // dims [col, col + 8)
   static __device__ __forceinline__ uint32_t piece(int row, int p) { return row * 64 + ((p ^ ((row >> 1) & 3)) << 4); }
 };
 
@@ -140,21 +144,49 @@ __device__ __forceinline__ uint2 lds_v2(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+// The D / 8 bytes of V's dims from col(g) on, of one row of a tile.
+template <int D>
+__device__ __forceinline__ void lds_v_row(uint32_t tile, int row, int g, uint32_t (&w)[D / 32]) {
+  if constexpr (D == 128) {
+    const uint4 x = lds_v4(tile + Lay<D>::piece(row, Lay<D>::col(g) / 16));
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
+  } else {
+    const uint2 x = lds_v2(tile + Lay<D>::piece(row, g >> 1) + (g & 1) * 8);
+    w[0] = x.x;
+    w[1] = x.y;
+  }
+}
 
 // Two e4m3 (low byte first) as two fp16, exactly.
 __device__ __forceinline__ uint32_t widen(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The two pairs of a word.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8x8 block of 16-bit values (row g, columns 2c, 2c + 1 in a thread), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 // Four consecutive values of a 16-bit row.
@@ -171,89 +203,76 @@ __device__ __forceinline__ float4 load4(const T* p) {
   }
 }
 
-// A row's address in q (row r of the KV head: query r / g, head r % g).
-template <typename T>
-__device__ __forceinline__ const T* q_row(const GqaArgs& a, int b, int kvh, int r) {
-  return static_cast<const T*>(a.q) + (int64_t)b * a.stride_q_b + (int64_t)(r / a.g) * a.stride_q_s +
-         (int64_t)(kvh * a.g + r % a.g) * a.stride_q_h;
-}
-
-// The q fragments of 16 rows from row r0 on: thread (j, c) holds rows j and
-// j + 8, for k-step 4 h + s the dims 16 (4 h + c) + 4 s + {0, 1, 2, 3}, the
-// same that it reads of K.  Rows past `rows` are zero.  factor[i] is what a
-// product is multiplied by: the row's power of two and the softmax scale.
+// The q^T fragments of 8 rows from row r0 on: thread (g, c) holds row g, for
+// k-step 4 h + s the dims 16 (4 h + c) + 4 s + {0, 1, 2, 3}, the same that
+// it reads of K.  Rows from `rows` on are zero.  factor[k] is what the
+// products of row 2c + k are multiplied by: the row's power of two and the
+// softmax scale.
 template <typename T, int D>
-__device__ __forceinline__ void load_q(const GqaArgs& a, int b, int kvh, int r0, int rows, uint32_t (&q)[D / 16][4],
+__device__ __forceinline__ void load_q(const GqaArgs& a, int b, int kvh, int r0, int rows, uint32_t (&q)[D / 16][2],
                                        float (&factor)[2]) {
-  const int lane = threadIdx.x & 31, j = lane >> 2, c = lane & 3;
+  const int lane = threadIdx.x & 31, c = lane & 3, r = r0 + (lane >> 2);
+  const bool live = r < rows;
+  const T* p = static_cast<const T*>(a.q);
+  if (live)
+    p += (int64_t)b * a.stride_q_b + (int64_t)(r / a.g) * a.stride_q_s + (int64_t)(kvh * a.g + r % a.g) * a.stride_q_h;
+  float4 f[D / 16];
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = r0 + j + 8 * i;
-    const bool live = r < rows;
-    const T* p = live ? q_row<T>(a, b, kvh, r) : nullptr;
-    float4 f[D / 16];
-    float top = 0.f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      f[s] = live ? load4(p + (s >> 2) * 64 + c * 16 + (s & 3) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      top = fmaxf(top, fmaxf(fmaxf(fabsf(f[s].x), fabsf(f[s].y)), fmaxf(fabsf(f[s].z), fabsf(f[s].w))));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the row's largest value becomes 2^13 .. 2^14 (an infinite one stays so)
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 240) - 127 - 13;
-    const float up = __uint_as_float((uint32_t)(127 - e) << 23);
-    factor[i] = a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      q[s][i] = pack_half(f[s].x * up, f[s].y * up);
-      q[s][2 + i] = pack_half(f[s].z * up, f[s].w * up);
-    }
+  for (int s = 0; s < D / 16; ++s) {
+    f[s] = live ? load4(p + (s >> 2) * 64 + c * 16 + (s & 3) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    top = fmaxf(top, fmaxf(fmaxf(fabsf(f[s].x), fabsf(f[s].y)), fmaxf(fabsf(f[s].z), fabsf(f[s].w))));
   }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  // the row's largest value becomes 2^13 .. 2^14 (an infinite one stays so)
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 240) - 127 - 13;
+  const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+  const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    q[s][0] = pack_half(f[s].x * up, f[s].y * up);
+    q[s][1] = pack_half(f[s].z * up, f[s].w * up);
+  }
+  factor[0] = __shfl_sync(0xffffffffu, down, 8 * c);
+  factor[1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 }
 
-// q.k of the 16 rows with the 32 positions of a stage: s[nt][0, 1] row j,
-// s[nt][2, 3] row j + 8, positions 8 nt + perm(2 c), 8 nt + perm(2 c + 1).
+// K's fragments of 16 positions of a tile for k-steps 4 h .. 4 h + 3.
 template <int D>
-__device__ __forceinline__ void score_unit(uint32_t k_stage, const uint32_t (&q)[D / 16][4], float (&s)[4][4]) {
-  const int lane = threadIdx.x & 31, j = lane >> 2, c = lane & 3;
+__device__ __forceinline__ void k_frags(uint32_t tile, int mt, int h, uint32_t (&f)[4][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint4 x = lds_v4(tile + Lay<D>::piece(mt * 16 + Lay<D>::perm(g), 4 * h + c));
+  const uint4 y = lds_v4(tile + Lay<D>::piece(mt * 16 + 8 + Lay<D>::perm(g), 4 * h + c));
+  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-  for (int nt = 0; nt < 4; ++nt) {
-    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-    for (int h = 0; h < D / 64; ++h) {
-      const uint4 w = lds_v4(k_stage + Lay<D>::piece(nt * 8 + Lay<D>::perm(j), 4 * h + c));
-      mma_f16(s[nt], q[4 * h + 0], widen(w.x & 0xFFFFu), widen(w.x >> 16));
-      mma_f16(s[nt], q[4 * h + 1], widen(w.y & 0xFFFFu), widen(w.y >> 16));
-      mma_f16(s[nt], q[4 * h + 2], widen(w.z & 0xFFFFu), widen(w.z >> 16));
-      mma_f16(s[nt], q[4 * h + 3], widen(w.w & 0xFFFFu), widen(w.w >> 16));
-    }
+  for (int s = 0; s < 4; ++s) {
+    widen4(xs[s], f[s][0], f[s][2]);
+    widen4(ys[s], f[s][1], f[s][3]);
   }
 }
 
 // ------------------------------------------------------------------ the list
-struct Place {
-  int b, kvh, grp;  // sequence, KV head, group of rows
-  int u, nu;        // unit in it, and how many it has
-};
-
+template <int W>
 struct ListShared {
-  long long sum[kWarps];
+  long long sum[W];
   long long total;
-  int b[kWarps + 1];
-  long long u[kWarps + 1];
+  int b[W];
+  long long u[W];
 };
 
-// Every thread sums a run of sequences, the sums are scanned, and the thread
-// whose run holds a wanted position walks to it.  `want(i, total)` is the
-// i-th wanted position; one at or past the total is not placed (b = -1).
-template <typename Want>
-__device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n, ListShared& sh, Want want) {
+// Where n wanted positions of the list of all sequences' units (per_seq
+// times over for a sequence's heads and groups) lie: sh.b[k] the sequence
+// (-1: past the end), sh.u[k] the unit among all of the sequence's.  Every
+// thread sums a run of sequences, the sums are scanned, and the thread whose
+// run holds a wanted position walks to it.
+template <int W, int U, typename Want>
+__device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n, ListShared<W>& sh, Want want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int run = (a.b + kThreads - 1) / kThreads;
+  const int run = (a.b + W * 32 - 1) / (W * 32);
   const int i0 = min(a.b, tid * run), i1 = min(a.b, i0 + run);
   long long sum = 0;
-  for (int i = i0; i < i1; ++i) sum += units_of(a, i);
+  for (int i = i0; i < i1; ++i) sum += units_of<U>(held_len(a, i));
   sum *= per_seq;
   long long incl = sum;
   for (int o = 1; o < 32; o <<= 1) {
@@ -264,17 +283,19 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n
   if (tid < n) sh.b[tid] = -1;
   __syncthreads();
   long long pre = incl - sum, total = 0;
-  for (int i = 0; i < kWarps; ++i) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
     if (i < warp) pre += sh.sum[i];
     total += sh.sum[i];
   }
   if (tid == 0) sh.total = total;
-  for (int k = 0; k < n; ++k) {
-    const long long x = want(k, total);
-    if (x >= pre && x < pre + sum) {
+  if (sum > 0) {
+    for (int k = 0; k < n; ++k) {
+      const long long x = want(k, total);
+      if (x < pre || x >= pre + sum) continue;
       long long at = pre;
       for (int i = i0; i < i1; ++i) {
-        const long long m = (long long)units_of(a, i) * per_seq;
+        const long long m = (long long)units_of<U>(held_len(a, i)) * per_seq;
         if (x < at + m) {
           sh.b[k] = i;
           sh.u[k] = x - at;
@@ -287,8 +308,8 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n
   __syncthreads();
 }
 
-// Position x of `parts` equal pieces of a list: where piece i begins, and
-// which piece holds x.
+// Where piece i of `parts` equal pieces of a list begins, and which piece
+// holds position x.
 __device__ __forceinline__ long long piece_begin(long long total, long long i, long long parts) {
   return total * i / parts;
 }
@@ -297,122 +318,136 @@ __device__ __forceinline__ int piece_of(long long total, long long x, long long 
 }
 
 // ------------------------------------------------------------------ loading
-// A warp's ring: its own stages, one mbarrier each.  The load cursor runs
-// kStages units ahead of the one that computes.
-template <int D, bool WITH_V>
-struct Ring {
-  static constexpr int kStages = WITH_V ? Lay<D>::kStages : 2 * Lay<D>::kStages;
-  static constexpr int kTile = kUnit * D;                  // bytes of K (or V) of a unit
-  static constexpr int kStage = kTile * (WITH_V ? 2 : 1);
-  static constexpr int kBytes = kStages * kStage;
-};
-
-// The block ids of 16 units of a sequence, one per 16 positions, in the
-// lanes; `base` is the first unit's number (-1: none held).
+// The blocks of 512 positions of a (sequence, KV head), one per 16 of them,
+// in the lanes: ids and scales (a load per unit would have its latency waited
+// for in every unit).  `base` is the first unit's number (-1: none held).
 struct Pages {
-  int id, base, b;
+  int id, base, b, kvh;
+  float ks, vs;
 };
-
-__device__ __forceinline__ void fetch_pages(const GqaArgs& a, Pages& p, int b, int u, int len) {
-  if (p.b == b && p.base >= 0 && u >= p.base && u < p.base + 16) return;
+template <int U, bool WITH_V>
+__device__ __forceinline__ void fetch_pages(const GqaArgs& a, Pages& p, int b, int kvh, int u, int len) {
+  constexpr int kUnits = 512 / U;
+  if (p.base == (u & ~(kUnits - 1)) && p.b == b && p.kvh == kvh) return;
   const int lane = threadIdx.x & 31;
   p.b = b;
-  p.base = u & ~15;
-  const long long t = ((long long)p.base * 2 + lane) * 16;
+  p.kvh = kvh;
+  p.base = u & ~(kUnits - 1);
+  const long long t = (long long)p.base * U + lane * 16;
   p.id = -1;
+  p.ks = p.vs = 1.f;
   if (t < len) {
     const int id = __ldg(a.table + (int64_t)b * a.stride_table + (int)(t >> a.page_shift));
-    if (id >= 0 && id < a.num_blocks) p.id = id;
+    if (id >= 0 && id < a.num_blocks) {
+      p.id = id;
+      p.ks = __ldg(a.k_scale + (int64_t)id * a.h_kv + kvh);
+      if constexpr (WITH_V) p.vs = __ldg(a.v_scale + (int64_t)id * a.h_kv + kvh);
+    }
   }
 }
 
-// Issues the loads of unit u into a stage; returns, in every lane, which of
-// the unit's two halves of 16 positions are held (bits 0, 1) and, in lanes
-// 0-3, the scales of K (half 0, 1) and V (half 0, 1).
-template <int D, bool WITH_V>
-__device__ __forceinline__ int load_unit(const GqaArgs& a, const CUtensorMap* tk, const CUtensorMap* tv, Pages& pages,
-                                         int b, int kvh, int u, int len, uint32_t stage, uint64_t* bar, float& scale,
-                                         bool withhold) {
-  using R = Ring<D, WITH_V>;
-  const int lane = threadIdx.x & 31;
-  fetch_pages(a, pages, b, u, len);
-  const int i = (u - pages.base) * 2;
-  const int id0 = __shfl_sync(0xffffffffu, pages.id, i), id1 = __shfl_sync(0xffffffffu, pages.id, i + 1);
-  const int my = lane & 1 ? id1 : id0;
-  scale = 1.f;
-  if (lane < (WITH_V ? 4 : 2) && my >= 0)
-    scale = __ldg((lane < 2 ? a.k_scale : a.v_scale) + (int64_t)my * a.h_kv + kvh);
-  const int held = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
-  if (lane == 0 && !withhold) {
-    const int off = (u * kUnit) & (a.page - 1);
-    if (a.page >= kUnit) {  // one block holds the unit (its second half too, read or not)
-      mbar_arrive_expect_tx(bar, id0 >= 0 ? R::kStage : 0);
-      if (id0 >= 0) {
-        tma_load_4d(stage, tk, 0, off, kvh, id0, bar);
-        if constexpr (WITH_V) tma_load_4d(stage + R::kTile, tv, 0, off, kvh, id0, bar);
-      }
-    } else {
-      mbar_arrive_expect_tx(bar, __popc(held) * (R::kStage / 2));
-      if (id0 >= 0) {
-        tma_load_4d(stage, tk, 0, 0, kvh, id0, bar);
-        if constexpr (WITH_V) tma_load_4d(stage + R::kTile, tv, 0, 0, kvh, id0, bar);
-      }
-      if (id1 >= 0) {
-        tma_load_4d(stage + R::kTile / 2, tk, 0, 0, kvh, id1, bar);
-        if constexpr (WITH_V) tma_load_4d(stage + R::kTile + R::kTile / 2, tv, 0, 0, kvh, id1, bar);
-      }
+// What is known of a unit: which of its runs of 16 positions are there (one
+// bit each), and the scales of their K and V.
+template <int U>
+struct Info {
+  int held;
+  float ks[U / 16], vs[U / 16];
+};
+
+// A tile of U positions in a warp's ring: K's or V's of unit u.  The maps'
+// boxes have min(page, 64) rows (or 32, where U is); `ids` are the blocks of
+// its runs of 16 (< 0: not there, not loaded).  One lane's work.
+template <int D, int U>
+__device__ __forceinline__ void load_tile(const GqaArgs& a, const CUtensorMap* map, const int (&ids)[U / 16], int kvh,
+                                          int u, uint32_t tile, uint64_t* bar) {
+  constexpr int kBytes = U * D;
+  if (a.page >= U) {  // one block holds the unit (its last runs too, read or not)
+    mbar_arrive_expect_tx(bar, ids[0] >= 0 ? kBytes : 0);
+    if (ids[0] >= 0) tma_load_4d(tile, map, 0, (u * U) & (a.page - 1), kvh, ids[0], bar);
+  } else {
+    const int runs = a.page / 16;  // of a block: 1 or 2
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < U / 16; ++i) n += (i % runs == 0 && ids[i] >= 0) ? 1 : 0;
+    mbar_arrive_expect_tx(bar, n * a.page * D);
+#pragma unroll
+    for (int i = 0; i < U / 16; ++i)
+      if (i % runs == 0 && ids[i] >= 0) tma_load_4d(tile + i * 16 * D, map, 0, 0, kvh, ids[i], bar);
+  }
+}
+
+// After a wait gave up: a warp's loads in flight land (or their waits run
+// out) before its shared memory goes.
+__device__ __forceinline__ void drain(uint64_t* full, int slots, int slot, uint32_t phase, int flying) {
+  for (int i = 0; i < slots && i < flying; ++i) {
+    const int x = (slot + i) % slots;
+    const long long t = clock64();
+    while (!mbar_try_wait(smem_u32(&full[x]), phase ^ (x < slot ? 1u : 0u), 1000u) && clock64() - t < kWaitLimitCycles) {
     }
   }
-  return held;
 }
 
 // ------------------------------------------------------------------ decode
-template <int D>
-struct DecodeShared {
-  uint64_t full[kWarps][Ring<D, true>::kStages];
-  ListShared list;
-  // Pieces of one (sequence, head, group) that a warp began or ended with:
-  // [warp][first or last piece].  The values of a last one lie in the warp's
-  // ring, which it no longer needs.
-  int id[kWarps][2];        // (b, kvh, grp) as one number, -1: none
-  int from[kWarps][2], to[kWarps][2], nu[kWarps][2];
-  float m[kWarps][2][kRows], l[kWarps][2][kRows];
-  int abort;
+// A unit is 64 positions: what a unit costs beside its products (waits, the
+// cursors, page ids, the loads' issue) is about 250 instructions of a warp,
+// which at 32 positions took more issue slots than the products.  Up to 8
+// rows of a head (one n-tile) leave room for 12 warps of 168 registers, 16
+// rows for 8 of 255.
+template <int D, int NT>
+struct Dec {
+  static constexpr int kUnit = 64;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kTile = kUnit * D;
+  static constexpr int kSlots = NT == 1 && D == 128 ? 2 : 3;
 };
-template <int D>
-constexpr int decode_smem() {
-  return 1024 + kWarps * Ring<D, true>::kBytes + kWarps * kRows * D * 4 + (int)sizeof(DecodeShared<D>);
-}
 
-// Workspace: [CTA][2] records of {id, last CTA, begins here, rows},
-// m[16], l[16], o[16][D]; the first is a piece whose beginning lies in an
-// earlier CTA, the second one that goes on in the next.
-template <int D>
+// A piece of one (sequence, head, group of rows): id numbers these; begins
+// and ends: whether it holds the first and the last of its units; last: the
+// CTA that holds the last one.  o is not divided by l, both are relative to
+// 2^m.
+template <int D, int NT>
 struct Partial {
   int id, last, begins, ends;
-  float m[kRows], l[kRows];
-  float o[kRows * D];
+  float m[8 * NT], l[8 * NT];
+  float o[8 * NT * D];
 };
-
-__device__ __forceinline__ void store_row16(__nv_bfloat16* p, const float* v, int n) {
-  for (int i = 0; i < n; i += 8) {
-    uint4 w;
-    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[i + 2 * k], v[i + 2 * k + 1]);
-      x[k] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p + i) = w;
-  }
+// Workspace: the CTAs' joined pieces ([CTA][2]: one whose beginning lies in
+// an earlier CTA, one that goes on in the next), then the values of warps'
+// first pieces ([CTA][warp][rows][D]).
+template <int D, int NT>
+constexpr size_t ws_bytes(int ctas) {
+  return (size_t)ctas * (2 * sizeof(Partial<D, NT>) + (size_t)Dec<D, NT>::kWarps * 8 * NT * D * 4);
 }
-__device__ __forceinline__ void store_row16(__half* p, const float* v, int n) {
-  for (int i = 0; i < n; i += 8) {
-    uint4 w;
-    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = pack_half(v[i + 2 * k], v[i + 2 * k + 1]);
-    *reinterpret_cast<uint4*>(p + i) = w;
+
+template <int D, int NT>
+struct DecodeShared {
+  using C = Dec<D, NT>;
+  uint64_t full[C::kWarps][C::kSlots];
+  ListShared<C::kWarps> list;
+  // The pieces that a warp began ([0]) and ended ([1]) with, where they are
+  // not whole.  Values of one that a warp ends with lie in its ring, which
+  // it no longer needs; others in the workspace.
+  int id[2 * C::kWarps];  // -1: none
+  int from[2 * C::kWarps], to[2 * C::kWarps], nu[2 * C::kWarps], in_ring[2 * C::kWarps];
+  float ml[2 * C::kWarps][2 * C::kRows];  // m, l
+  int list_of[2 * C::kWarps];             // pieces of the one that is being joined
+  int abort;
+};
+template <int D, int NT>
+constexpr int decode_smem() {
+  using C = Dec<D, NT>;
+  return 1024 + C::kWarps * C::kSlots * C::kTile + (int)sizeof(DecodeShared<D, NT>);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    return pack_half(lo, hi);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
 
@@ -426,108 +461,96 @@ __device__ __forceinline__ float* lse_at(const GqaArgs& a, int b, int kvh, int r
 }
 
 // Joins n pieces of one (sequence, head, group), in order, by all threads:
-// piece i has maxima and sums ml(i) (m[16] then l[16]) and values o(i)
-// [16][D].  Writes the result, or the joined piece to `part`.
-template <typename T, int D, typename ML, typename O>
-__device__ __forceinline__ void join(const GqaArgs& a, int n, int id, ML m_of, O o_of, Partial<D>* part) {
-  constexpr int kPerThread = kRows * D / kThreads;  // 8 or 4 consecutive dims of one row
-  const int row = threadIdx.x / (D / kPerThread), d0 = (threadIdx.x % (D / kPerThread)) * kPerThread;
+// piece i has maxima and sums ml[i] (m, then l) and values o_of(i) [rows][D].
+// Writes the result, or the joined piece to `part`.
+template <typename T, int D, int NT, int THREADS, typename O>
+__device__ __forceinline__ void join(const GqaArgs& a, int n, int id, const float (*ml)[16 * NT], O o_of,
+                                     Partial<D, NT>* part) {
+  constexpr int kRows = 8 * NT;
   const int grp = id % a.groups, kvh = id / a.groups % a.h_kv, b = id / a.groups / a.h_kv;
-  const int r = grp * kRows + row;
-  if (r >= a.g * a.s_q) return;
-  float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, m_of(i)[row]);
-  float l = 0.f, o[kPerThread];
+  for (int e = threadIdx.x * 4; e < kRows * D; e += THREADS * 4) {
+    const int row = e / D, d0 = e % D;
+    const int r = grp * kRows + row;
+    if (r >= a.g * a.s_q) continue;
+    float m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, ml[i][row]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kDeep = 8;  // loads in flight
+    for (int i0 = 0; i0 < n; i0 += kDeep) {
+      float4 x[kDeep];
 #pragma unroll
-  for (int k = 0; k < kPerThread; ++k) o[k] = 0.f;
-  const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float f = fast_exp2(m_of(i)[row] - base);  // 0 where nothing was seen
-    l += f * m_of(i)[kRows + row];
-    const float* v = o_of(i) + row * D + d0;
+      for (int i = 0; i < kDeep; ++i)
+        x[i] = *reinterpret_cast<const float4*>(o_of(min(i0 + i, n - 1)) + e);
 #pragma unroll
-    for (int k = 0; k < kPerThread; k += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(v + k);
-      o[k] += f * x.x;
-      o[k + 1] += f * x.y;
-      o[k + 2] += f * x.z;
-      o[k + 3] += f * x.w;
+      for (int i = 0; i < kDeep; ++i) {
+        if (i0 + i < n) {
+          const float f = fast_exp2(ml[i0 + i][row] - base);  // 0 where nothing was seen
+          l += f * ml[i0 + i][kRows + row];
+          o.x += f * x[i].x;
+          o.y += f * x[i].y;
+          o.z += f * x[i].z;
+          o.w += f * x[i].w;
+        }
+      }
     }
-  }
-  if (part) {
-    if (d0 == 0) {
-      part->m[row] = m;
-      part->l[row] = l;
+    if (part) {
+      if (d0 == 0) {
+        part->m[row] = m;
+        part->l[row] = l;
+      }
+      *reinterpret_cast<float4*>(part->o + e) = o;
+      continue;
     }
-#pragma unroll
-    for (int k = 0; k < kPerThread; k += 4)
-      *reinterpret_cast<float4*>(part->o + row * D + d0 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-    return;
+    const bool none = m == -INFINITY;
+    const float inv = none ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) =
+        make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
+    if (d0 == 0) *lse_at(a, b, kvh, r) = none ? -INFINITY : (m + log2f(l)) * kLn2;
   }
-  const bool none = m == -INFINITY;
-  const float inv = none ? 0.f : 1.f / l;
-  T* p = out_row<T>(a, b, kvh, r) + d0;
-#pragma unroll
-  for (int k = 0; k < kPerThread; ++k) o[k] *= inv;
-  if constexpr (kPerThread == 8) {
-    store_row16(p, o, 8);
-  } else {
-    uint2 w;
-    if constexpr (std::is_same_v<T, __half>) {
-      w = make_uint2(pack_half(o[0], o[1]), pack_half(o[2], o[3]));
-    } else {
-      const __nv_bfloat162 x = __floats2bfloat162_rn(o[0], o[1]), y = __floats2bfloat162_rn(o[2], o[3]);
-      w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    }
-    *reinterpret_cast<uint2*>(p) = w;
-  }
-  if (d0 == 0) *lse_at(a, b, kvh, r) = none ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Dec<D, NT>::kThreads, 1)
 gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const GqaArgs a) {
-  using R = Ring<D, true>;
-  constexpr int kStages = R::kStages;
-  constexpr int kTiles = D / 8;  // n tiles of the output
+  using C = Dec<D, NT>;
+  constexpr int kWarps = C::kWarps, kSlots = C::kSlots, kRows = C::kRows, kTile = C::kTile;
+  constexpr int kUnit = C::kUnit, kRuns = kUnit / 16;
+  constexpr int kSteps = D / 16;  // k-steps of q.k, m-tiles of the output
   asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* first_o = reinterpret_cast<float*>(smem + kWarps * R::kBytes);  // [warp][16][D]
-  DecodeShared<D>& sh = *reinterpret_cast<DecodeShared<D>*>(first_o + kWarps * kRows * D);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane >> 2, c = lane & 3;
-  float* ring_o = reinterpret_cast<float*>(smem + warp * R::kBytes);
-  const uint32_t ring = smem_u32(ring_o);
+  DecodeShared<D, NT>& sh = *reinterpret_cast<DecodeShared<D, NT>*>(smem + kWarps * kSlots * kTile);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(smem + warp * kSlots * kTile);
   uint64_t* full = sh.full[warp];
+  // in the workspace: the values of a warp's first piece
+  auto first_o = [&](int w) {
+    return reinterpret_cast<float*>(reinterpret_cast<Partial<D, NT>*>(a.ws) + (int64_t)gridDim.x * 2) +
+           ((int64_t)blockIdx.x * kWarps + w) * kRows * D;
+  };
 
   if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], 1);
     fence_mbarrier_init();
-    sh.id[warp][0] = sh.id[warp][1] = -1;
+    sh.id[2 * warp] = sh.id[2 * warp + 1] = -1;
   }
   if (tid == 0) sh.abort = 0;
-  const int per_seq = a.h_kv * a.groups;
   const long long parts = (long long)gridDim.x * kWarps, first_part = (long long)blockIdx.x * kWarps;
-  find_places(a, per_seq, kWarps, sh.list,
-              [&](int k, long long total) { return piece_begin(total, first_part + k, parts); });
+  find_places<kWarps, kUnit>(a, a.h_kv * a.groups, kWarps, sh.list,
+                      [&](int k, long long total) { return piece_begin(total, first_part + k, parts); });
   const long long total = sh.list.total;
-  long long left = piece_begin(total, first_part + warp + 1, parts) - piece_begin(total, first_part + warp, parts);
-  const bool withhold = g_gqa_test_stall != 0 && tid == 0;
+  int left = (int)(piece_begin(total, first_part + warp + 1, parts) - piece_begin(total, first_part + warp, parts));
 
   // the two cursors: where loads and where products are
   struct Cursor {
     int b, kvh, grp, u, nu, len, end;  // end: the first query sees the positions below it
   };
-  auto place = [&](Cursor& x, int b, long long u) {
-    x.b = b;
-    x.len = held_len(a, b);
-    x.end = __ldg(a.ctx + b) - a.s_q + 1;
-    x.nu = max(1, (x.len + kUnit - 1) / kUnit);
-    const int pair = (int)(u / x.nu);
-    x.u = (int)(u - (long long)pair * x.nu);
-    x.kvh = pair / a.groups;
-    x.grp = pair % a.groups;
+  auto enter = [&](Cursor& x) {
+    x.len = held_len(a, x.b);
+    x.end = __ldg(a.ctx + x.b) - a.s_q + 1;
+    x.nu = units_of<kUnit>(x.len);
   };
   auto advance = [&](Cursor& x) {
     if (++x.u < x.nu) return;
@@ -536,340 +559,378 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     x.grp = 0;
     if (++x.kvh < a.h_kv) return;
     x.kvh = 0;
-    if (++x.b < a.b) {
-      x.len = held_len(a, x.b);
-      x.end = __ldg(a.ctx + x.b) - a.s_q + 1;
-      x.nu = max(1, (x.len + kUnit - 1) / kUnit);
+    if (++x.b < a.b) enter(x);
+  };
+  Cursor cur = {};
+  if (left > 0) {
+    cur.b = sh.list.b[warp];
+    enter(cur);
+    const long long u = sh.list.u[warp];
+    const int pair = (int)(u / cur.nu);
+    cur.u = (int)(u - (long long)pair * cur.nu);
+    cur.kvh = pair / a.groups;
+    cur.grp = pair % a.groups;
+  }
+  Cursor ld = cur;
+  int tiles = 2 * left;  // to be loaded
+  int ids[kRuns];
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) ids[i] = -1;
+  bool ld_v = false, withhold = g_gqa_test_stall != 0 && tid == 0;
+  Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
+  Info<kUnit> now, next;  // of the unit at `cur`, and of the one behind it
+  auto load_next = [&](int slot) {  // K of the unit at `ld`, the next time its V
+    if (tiles == 0) return;
+    --tiles;
+    if (!ld_v) {
+      fetch_pages<kUnit, true>(a, pages, ld.b, ld.kvh, ld.u, ld.len);
+      next.held = 0;
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {
+        const int from = (ld.u - pages.base) * kRuns + i;
+        ids[i] = __shfl_sync(0xffffffffu, pages.id, from);
+        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, from);
+        next.vs[i] = __shfl_sync(0xffffffffu, pages.vs, from);
+        next.held |= (ids[i] >= 0 ? 1 : 0) << i;
+      }
+      if (lane == 0 && !withhold) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + slot * kTile, &full[slot]);
+      withhold = false;
+    } else {
+      if (lane == 0) load_tile<D, kUnit>(a, &tv, ids, ld.kvh, ld.u, ring + slot * kTile, &full[slot]);
+      advance(ld);
+    }
+    ld_v = !ld_v;
+  };
+  load_next(0);
+  now = next;
+#pragma unroll
+  for (int s = 1; s < kSlots; ++s) load_next(s);
+
+  uint32_t q[NT][kSteps][2];
+  float factor[NT][2];
+  float o[kSteps][NT][4];  // (dim col(g) + 2 i, rows 2c, 2c + 1), (dim col(g) + 2 i + 1, the same), in units of v_unit
+  float m[NT][2], l[NT][2], v_unit = 1.f;
+  int from = 0, q_first = 0, q_of[NT][2];  // the first row's query, and those of rows 2c, 2c + 1
+  bool fresh = true, ok = true, first = true;
+  const int rows = a.g * a.s_q;
+  int slot = 0;
+  uint32_t phase = 0;
+  auto next_slot = [&]() {
+    if (++slot == kSlots) {
+      slot = 0;
+      phase ^= 1;
     }
   };
-  Cursor ld = {}, cur = {};
-  if (left > 0) {
-    place(ld, sh.list.b[warp], sh.list.u[warp]);
-    cur = ld;
-  }
-  long long to_load = left;
-  Pages pages = {-1, -1, -1};
-  float scales[kStages];
-  int held[kStages];
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) {
-    scales[s] = 1.f;
-    held[s] = 0;
-    if (to_load > 0) {
-      held[s] = load_unit<D, true>(a, &tk, &tv, pages, ld.b, ld.kvh, ld.u, ld.len, ring + s * R::kStage, &full[s],
-                                   scales[s], withhold && s == 0);
-      advance(ld);
-      --to_load;
-    }
-  }
 
-  uint32_t q[D / 16][4];
-  float factor[2] = {0.f, 0.f};
-  float o[kTiles][4], m[2], l[2], v_unit = 1.f;  // o is in units of v_unit
-  int from = 0, slot = 0;
-  bool fresh = true, ok = true;
-  uint32_t phase = 0;
-  const int rows = a.g * a.s_q;
-
-  int st = 0;
   while (left > 0) {
     const int r0 = cur.grp * kRows;
     if (fresh) {
-      load_q<T, D>(a, cur.b, cur.kvh, r0, rows, q, factor);
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+      for (int n = 0; n < NT; ++n) load_q<T, D>(a, cur.b, cur.kvh, r0 + 8 * n, rows, q[n], factor[n]);
+      q_first = r0 / a.g;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          m[n][k] = -INFINITY;
+          l[n][k] = 0.f;
+          q_of[n][k] = (r0 + 8 * n + 2 * c + k) / a.g;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
       v_unit = 1.f;
       from = cur.u;
       fresh = false;
     }
-    const uint32_t k_stage = ring + st * R::kStage, v_stage = k_stage + R::kTile;
     // positions below `all` are seen by every row, those from `len` on by none
     const int t0 = cur.u * kUnit;
-    const int all = min(cur.len, cur.end);
-    int held_now = held[0];
-    float scale_now = scales[0];
+    const int all = min(cur.len, cur.end + q_first);
+    bool edge = t0 + kUnit > all || now.held != (1 << kRuns) - 1;
 #pragma unroll
-    for (int i = 1; i < kStages; ++i) {
-      held_now = st == i ? held[i] : held_now;
-      scale_now = st == i ? scales[i] : scale_now;
-    }
-    const float ks[2] = {__shfl_sync(0xffffffffu, scale_now, 0), __shfl_sync(0xffffffffu, scale_now, 1)};
-    const float vs[2] = {__shfl_sync(0xffffffffu, scale_now, 2), __shfl_sync(0xffffffffu, scale_now, 3)};
-    const bool edge = t0 + kUnit > all || held_now != 3 || vs[0] == 0.f || vs[1] == 0.f;
-    const int lim[2] = {min(cur.len, cur.end + (r0 + j) / a.g), min(cur.len, cur.end + (r0 + j + 8) / a.g)};
-    ok = mbar_wait(&full[st], phase, &sh.abort, &g_gqa_status);
-    if (!ok) break;
-    {
-      float s[4][4];
-      score_unit<D>(k_stage, q, s);
-      float top[2] = {-INFINITY, -INFINITY};
+    for (int i = 0; i < kRuns; ++i) edge |= now.vs[i] == 0.f;
+    if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+
+    // s^T: s[mt][n]: positions 16 mt + perm(g) (0, 1) and 8 further (2, 3), rows 2c, 2c + 1
+    float s[kRuns][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
+    for (int mt = 0; mt < kRuns; ++mt) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float f = factor[i] * ks[nt >> 1];
-          s[nt][2 * i] *= f;
-          s[nt][2 * i + 1] *= f;
-        }
+      for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        uint32_t f[4][4];
+        k_frags<D>(ring + slot * kTile, mt, h, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma_f16(s[mt][n], f[k][0], f[k][1], f[k][2], f[k][3], q[n][4 * h + k][0], q[n][4 * h + k][1]);
       }
+    }
+    __syncwarp();
+    load_next(slot);
+    next_slot();
+
+#pragma unroll
+    for (int mt = 0; mt < kRuns; ++mt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float f = factor[n][k] * now.ks[mt];
+          s[mt][n][k] *= f;
+          s[mt][n][2 + k] *= f;
+        }
+    if (edge) {
+#pragma unroll
+      for (int mt = 0; mt < kRuns; ++mt) {
+        const bool there = (now.held >> mt) & 1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int lim = min(cur.len, cur.end + q_of[n][k]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!there || t0 + mt * 16 + h * 8 + Lay<D>::perm(g) >= lim) s[mt][n][2 * h + k] = -INFINITY;
+          }
+      }
+    }
+    // the running maxima, moved only where a score outgrows one by 2^8
+    float top[NT][2];
+    bool grew = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        top[n][k] = fmaxf(s[0][n][k], s[0][n][2 + k]);
+#pragma unroll
+        for (int mt = 1; mt < kRuns; ++mt) top[n][k] = fmaxf(top[n][k], fmaxf(s[mt][n][k], s[mt][n][2 + k]));
+        grew |= top[n][k] > m[n][k] + kRescale;
+      }
+    if (__any_sync(0xffffffffu, grew)) {
+      float alpha[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float t = top[n][k];
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+          alpha[n][k] = 1.f;
+          if (t > m[n][k]) {
+            alpha[n][k] = fast_exp2(m[n][k] - t);
+            m[n][k] = t;
+            l[n][k] *= alpha[n][k];
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][n][k] *= alpha[n][k & 1];
+    }
+    uint32_t p[kRuns][NT][2];  // p^T: rows g, positions 2c, 2c + 1 (of 8 and of the 8 further)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float base[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+      for (int mt = 0; mt < kRuns; ++mt) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[mt][n][k] = fast_exp2(s[mt][n][k] - base[k & 1]);
+        l[n][0] += s[mt][n][0] + s[mt][n][2];
+        l[n][1] += s[mt][n][1] + s[mt][n][3];
+        p[mt][n][0] = transpose8(pack_half(s[mt][n][0], s[mt][n][1]));
+        p[mt][n][1] = transpose8(pack_half(s[mt][n][2], s[mt][n][3]));
+      }
+    }
+    if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+    const uint32_t v_tile = ring + slot * kTile;
+#pragma unroll
+    for (int mt = 0; mt < kRuns; ++mt) {
+      // o into units of these positions' v_scale (0: they add nothing)
+      const bool there = (now.held >> mt) & 1 && now.vs[mt] != 0.f;
+      if (there && now.vs[mt] != v_unit) {  // the same in all lanes
+        const float r = v_unit / now.vs[mt];
+        v_unit = now.vs[mt];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[i][n][k] *= r;
+      }
+      // the four positions whose p this thread holds
+      const int row[4] = {16 * mt + Lay<D>::perm(2 * c), 16 * mt + Lay<D>::perm(2 * c + 1),
+                          16 * mt + 8 + Lay<D>::perm(2 * c), 16 * mt + 8 + Lay<D>::perm(2 * c + 1)};
+      uint32_t w[4][D / 32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) lds_v_row<D>(v_tile, row[k], g, w[k]);
+      // A position that some row does not see stays out of the product:
+      // 0 * NaN of a stale or masked value would reach that row.  Zero
+      // values here, added below for the rows that see them.
       if (edge) {
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const bool there = (held_now >> (nt >> 1)) & 1;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int t = t0 + nt * 8 + Lay<D>::perm(2 * c + k);
-            if (!there || t >= lim[0]) s[nt][k] = -INFINITY;
-            if (!there || t >= lim[1]) s[nt][2 + k] = -INFINITY;
-          }
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        top[0] = fmaxf(top[0], fmaxf(s[nt][0], s[nt][1]));
-        top[1] = fmaxf(top[1], fmaxf(s[nt][2], s[nt][3]));
-      }
-      float alpha[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        const float m_new = fmaxf(m[i], top[i]);
-        alpha[i] = m_new == m[i] ? 1.f : fast_exp2(m[i] - m_new);
-        m[i] = m_new;
-        l[i] *= alpha[i];
-      }
-      const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[nt][2 * i] = fast_exp2(s[nt][2 * i] - base[i]);
-          s[nt][2 * i + 1] = fast_exp2(s[nt][2 * i + 1] - base[i]);
-          l[i] += s[nt][2 * i] + s[nt][2 * i + 1];
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {  // 16 positions each
-        // o into units of these positions' v_scale (0: they add nothing)
-        float r = 1.f;
-        if ((held_now >> t) & 1) {
-          if (vs[t] != 0.f && vs[t] != v_unit) {
-            r = v_unit / vs[t];
-            v_unit = vs[t];
-          }
-        }
-        const float f0 = alpha[0] * r, f1 = alpha[1] * r;
-        alpha[0] = alpha[1] = 1.f;
-        if (!__all_sync(0xffffffffu, f0 == 1.f && f1 == 1.f)) {
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            o[i][0] *= f0;
-            o[i][1] *= f0;
-            o[i][2] *= f1;
-            o[i][3] *= f1;
-          }
-        }
-        const uint32_t p[4] = {pack_half(s[2 * t][0], s[2 * t][1]), pack_half(s[2 * t][2], s[2 * t][3]),
-                               pack_half(s[2 * t + 1][0], s[2 * t + 1][1]),
-                               pack_half(s[2 * t + 1][2], s[2 * t + 1][3])};
-        // the four positions whose p this thread holds
-        const int row[4] = {16 * t + Lay<D>::perm(2 * c), 16 * t + Lay<D>::perm(2 * c + 1),
-                            16 * t + 8 + Lay<D>::perm(2 * c), 16 * t + 8 + Lay<D>::perm(2 * c + 1)};
-        constexpr int kWords = kTiles / 4;  // 32-bit words per position
-        uint32_t w[4][kWords];
-#pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if constexpr (D == 128) {
-            const uint4 x = lds_v4(v_stage + Lay<D>::piece(row[k], Lay<D>::col(j) / 16));
-            w[k][0] = x.x;
-            w[k][1] = x.y;
-            w[k][2] = x.z;
-            w[k][3] = x.w;
-          } else {
-            const uint2 x = lds_v2(v_stage + Lay<D>::piece(row[k], j >> 1) + (j & 1) * 8);
-            w[k][0] = x.x;
-            w[k][1] = x.y;
-          }
+          const bool in = there && t0 + row[k] < all;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) w[k][e] = in ? w[k][e] : 0u;
         }
-        // A position that some row does not see stays out of the
-        // product: 0 * NaN of a stale or masked value would reach that
-        // row.  Zero values here, added below for the rows that see them.
-        if (edge) {
+      }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool in = t0 + row[k] < all && ((held_now >> t) & 1) && vs[t] != 0.f;
+      for (int e = 0; e < D / 32; ++e) {
 #pragma unroll
-            for (int e = 0; e < kWords; ++e) w[k][e] = in ? w[k][e] : 0u;
-          }
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t lo = __byte_perm(w[0][e], w[1][e], x ? 0x7362 : 0x5140);
+          const uint32_t hi = __byte_perm(w[2][e], w[3][e], x ? 0x7362 : 0x5140);
+          uint32_t a0, a1, a2, a3;
+          widen4(lo, a0, a1);
+          widen4(hi, a2, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(o[2 * e + x][n], a0, a1, a2, a3, p[mt][n][0], p[mt][n][1]);
         }
+      }
+      if (edge && there) {
+        // the drafts' own positions: at most s_q - 1, one by one
+        const int lo = max(max(all, 0), t0 + 16 * mt), hi = min(cur.len, t0 + 16 * mt + 16);
+        for (int x = lo; x < hi; ++x) {
+          const int in8 = (x - t0) & 7, h = ((x - t0) >> 3) & 1;
+          const int from_lane = Lay<D>::unperm(in8) * 4 + c;
+          uint32_t v[D / 32];
+          lds_v_row<D>(v_tile, x - t0, g, v);
 #pragma unroll
-        for (int e = 0; e < kWords; ++e) {
-          const uint32_t a01 = __byte_perm(w[0][e], w[1][e], 0x5140), a23 = __byte_perm(w[0][e], w[1][e], 0x7362);
-          const uint32_t b01 = __byte_perm(w[2][e], w[3][e], 0x5140), b23 = __byte_perm(w[2][e], w[3][e], 0x7362);
-          mma_f16(o[4 * e + 0], p, widen(a01 & 0xFFFFu), widen(b01 & 0xFFFFu));
-          mma_f16(o[4 * e + 1], p, widen(a01 >> 16), widen(b01 >> 16));
-          mma_f16(o[4 * e + 2], p, widen(a23 & 0xFFFFu), widen(b23 & 0xFFFFu));
-          mma_f16(o[4 * e + 3], p, widen(a23 >> 16), widen(b23 >> 16));
-        }
-        if (edge && a.s_q > 1 && ((held_now >> t) & 1) && vs[t] != 0.f) {
-          // the drafts' own positions: at most s_q - 1, row by row
-          const int lo = max(max(all, 0), t0 + 16 * t), hi = min(cur.len, t0 + 16 * t + 16);
-          for (int x = lo; x < hi; ++x) {
-            const int in8 = (x - t0) & 7, half = ((x - t0) >> 3) & 1;
-            const int col = Lay<D>::perm(in8);  // perm of Lay<64> is its own inverse
-            const int cc = D == 128 ? ((in8 & 3) << 1 | (in8 >> 2)) : col;  // the column that holds position x
-            const float x0 = half ? ((cc & 1) ? s[2 * t + 1][1] : s[2 * t + 1][0])
-                                  : ((cc & 1) ? s[2 * t][1] : s[2 * t][0]);
-            const float x1 = half ? ((cc & 1) ? s[2 * t + 1][3] : s[2 * t + 1][2])
-                                  : ((cc & 1) ? s[2 * t][3] : s[2 * t][2]);
-            const float p0 = __shfl_sync(0xffffffffu, x0, (lane & ~3) | (cc >> 1));
-            const float p1 = __shfl_sync(0xffffffffu, x1, (lane & ~3) | (cc >> 1));
-            const bool see0 = x < lim[0], see1 = x < lim[1];
-            // this thread's columns: tile i, columns 2 c and 2 c + 1 are dims col(2 c) + i, col(2 c + 1) + i
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
+            for (int k = 0; k < 2; ++k) {
+              const float px = __shfl_sync(0xffffffffu, h ? s[mt][n][2 + k] : s[mt][n][k], from_lane);
+              if (x < cur.end + q_of[n][k]) {
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int dim = Lay<D>::col(2 * c + k) + i;
-                uint32_t byte;
-                asm volatile("ld.shared.u8 %0, [%1];"
-                             : "=r"(byte)
-                             : "r"(v_stage + Lay<D>::piece(x - t0, dim >> 4) + (dim & 15)));
-                const uint32_t h2 = widen(byte);
-                const float val = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
-                if (see0) o[i][k] += p0 * val;
-                if (see1) o[i][2 + k] += p1 * val;
+                for (int i = 0; i < kSteps; ++i) {
+                  const uint32_t two = widen((v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+                  const float2 val = __half22float2(*reinterpret_cast<const __half2*>(&two));
+                  o[i][n][k] += px * val.x;
+                  o[i][n][2 + k] += px * val.y;
+                }
               }
             }
+        }
+      }
+    }
+    __syncwarp();
+    now = next;
+    load_next(slot);
+    next_slot();
+    --left;
+    const bool done = cur.u + 1 == cur.nu;  // the (sequence, head, group) ends here
+    if (done || left == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 4);
+          l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 8);
+          l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 16);
+        }
+      const bool whole = from == 0 && done;
+      const int piece = 2 * warp + (first ? 0 : 1);
+      float* keep = left == 0 ? reinterpret_cast<float*>(smem + warp * kSlots * kTile) : first_o(warp);
+      if (!whole && lane == 0) {
+        sh.id[piece] = (cur.b * a.h_kv + cur.kvh) * a.groups + cur.grp;
+        sh.from[piece] = from;
+        sh.to[piece] = cur.u + 1;
+        sh.nu[piece] = cur.nu;
+        sh.in_ring[piece] = left == 0;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int row = 8 * n + 2 * c + k, r = r0 + row;
+          const bool none = m[n][k] == -INFINITY;
+          const float f = whole ? (none ? 0.f : v_unit / l[n][k]) : v_unit;
+          float v[2 * kSteps];
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            v[2 * i] = o[i][n][k] * f;
+            v[2 * i + 1] = o[i][n][2 + k] * f;
           }
-        }
-      }
-      --left;
-      const int now_u = cur.u, now_nu = cur.nu, now_b = cur.b, now_kvh = cur.kvh, now_grp = cur.grp;
-      advance(cur);
-      const bool done = now_u + 1 == now_nu;  // the (sequence, head, group) ends here
-      __syncwarp();
-      if (to_load > 0) {
-        held_now = load_unit<D, true>(a, &tk, &tv, pages, ld.b, ld.kvh, ld.u, ld.len, k_stage, &full[st],
-                                      scale_now, false);
+          if (whole) {
+            if (r < rows) {
+              T* p = out_row<T>(a, cur.b, cur.kvh, r) + Lay<D>::col(g);
 #pragma unroll
-        for (int i = 0; i < kStages; ++i) {
-          held[i] = st == i ? held_now : held[i];
-          scales[i] = st == i ? scale_now : scales[i];
-        }
-        advance(ld);
-        --to_load;
-      }
-      if (done || left == 0) {
+              for (int e = 0; e < 2 * kSteps; e += 8)
+                *reinterpret_cast<uint4*>(p + e) = make_uint4(pack16<T>(v[e], v[e + 1]), pack16<T>(v[e + 2], v[e + 3]),
+                                                              pack16<T>(v[e + 4], v[e + 5]), pack16<T>(v[e + 6], v[e + 7]));
+              if (g == 0) *lse_at(a, cur.b, cur.kvh, r) = none ? -INFINITY : (m[n][k] + log2f(l[n][k])) * kLn2;
+            }
+          } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-          l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        }
-        const bool whole = from == 0 && done;
-        if (!whole && c == 0) {
-          sh.m[warp][slot][j] = m[0];
-          sh.m[warp][slot][j + 8] = m[1];
-          sh.l[warp][slot][j] = l[0];
-          sh.l[warp][slot][j + 8] = l[1];
-        }
-        if (!whole && lane == 0) {
-          sh.id[warp][slot] = (now_b * a.h_kv + now_kvh) * a.groups + now_grp;
-          sh.from[warp][slot] = from;
-          sh.to[warp][slot] = now_u + 1;
-          sh.nu[warp][slot] = now_nu;
-        }
-        float* keep = slot == 0 ? first_o + warp * kRows * D : ring_o;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = r0 + j + 8 * i;
-          const float f = whole ? (m[i] == -INFINITY ? 0.f : v_unit / l[i]) : v_unit;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float v[kTiles];
-#pragma unroll
-            for (int e = 0; e < kTiles; ++e) v[e] = o[e][2 * i + k] * f;
-            if (whole) {
-              if (r < rows) store_row16(out_row<T>(a, now_b, now_kvh, r) + Lay<D>::col(2 * c + k), v, kTiles);
-            } else {
-#pragma unroll
-              for (int e = 0; e < kTiles; e += 4)
-                *reinterpret_cast<float4*>(keep + (j + 8 * i) * D + Lay<D>::col(2 * c + k) + e) =
-                    make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 2 * kSteps; e += 4)
+              *reinterpret_cast<float4*>(keep + row * D + Lay<D>::col(g) + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            if (g == 0) {
+              sh.ml[piece][row] = m[n][k];
+              sh.ml[piece][kRows + row] = l[n][k];
             }
           }
-          if (whole && c == 0 && r < rows)
-            *lse_at(a, now_b, now_kvh, r) = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
         }
-        if (!whole) slot = 1;
-        fresh = true;
-      }
+      first = false;
+      fresh = true;
     }
-    if (++st == kStages) {
-      st = 0;
-      phase ^= 1;
-    }
+    advance(cur);
   }
-  if (!ok) {  // this warp's loads in flight land (or their waits run out) before its shared memory goes
-    const int flying = (int)min((long long)kStages, left - to_load);
-    for (int i = 0; i < flying; ++i) {
-      const int x = (st + i) % kStages;
-      const long long t = clock64();
-      while (!mbar_try_wait(smem_u32(&full[x]), phase ^ (x < st ? 1u : 0u), 1000u) && clock64() - t < kWaitLimitCycles) {
-      }
-    }
-  }
+  if (!ok) drain(full, kSlots, slot, phase, 2 * left - tiles);
   __syncthreads();
 
   // Pieces in order of the list: warp 0's first and last, warp 1's, ...
-  Partial<D>* mine = reinterpret_cast<Partial<D>*>(a.ws) + (int64_t)blockIdx.x * 2;
+  Partial<D, NT>* mine = reinterpret_cast<Partial<D, NT>*>(a.ws) + (int64_t)blockIdx.x * 2;
   if (tid < 2) mine[tid].id = -1;
   __syncthreads();
   if (sh.abort) return;
   for (int x = 0; x < 2 * kWarps;) {
-    const int id = sh.id[x >> 1][x & 1];
+    const int id = sh.id[x];
     if (id < 0) {
       ++x;
       continue;
     }
-    int e = x + 1, last = x;
-    while (e < 2 * kWarps && (sh.id[e >> 1][e & 1] == id || sh.id[e >> 1][e & 1] < 0)) {
-      if (sh.id[e >> 1][e & 1] == id) last = e;
-      ++e;
+    int e = x, n = 0, last = x;  // the pieces x .. last of this id; others between them are empty
+    for (; e < 2 * kWarps && (sh.id[e] == id || sh.id[e] < 0); ++e) {
+      if (sh.id[e] == id) {
+        if (tid == 0) sh.list_of[n] = e;
+        ++n;
+        last = e;
+      }
     }
-    const bool begins = sh.from[x >> 1][x & 1] == 0;
-    const bool ends = sh.to[last >> 1][last & 1] == sh.nu[last >> 1][last & 1];
-    Partial<D>* part = begins && ends ? nullptr : mine + (begins ? 1 : 0);
-    // the pieces x .. last that there are, as a dense list
-    int idx[2 * kWarps], n = 0;
-    for (int k = x; k <= last; ++k)
-      if (sh.id[k >> 1][k & 1] == id) idx[n++] = k;
-    __shared__ float ml[2 * kWarps][2 * kRows];
-    for (int k = tid; k < n * kRows; k += kThreads) {
-      const int p = idx[k / kRows];
-      ml[k / kRows][k % kRows] = sh.m[p >> 1][p & 1][k % kRows];
-      ml[k / kRows][kRows + k % kRows] = sh.l[p >> 1][p & 1][k % kRows];
-    }
+    const bool begins = sh.from[x] == 0, ends = sh.to[last] == sh.nu[last];
+    Partial<D, NT>* part = begins && ends ? nullptr : mine + (begins ? 1 : 0);
     __syncthreads();
-    join<T, D>(a, n, id, [&](int i) -> const float* { return ml[i]; },
-               [&](int i) -> const float* {
-                 const int p = idx[i];
-                 return (p & 1) ? reinterpret_cast<const float*>(smem + (p >> 1) * R::kBytes)
-                                : first_o + (p >> 1) * kRows * D;
-               },
-               part);
+    // the joined pieces' maxima and sums stand one after another from here on
+    float keep_ml[2];
+    for (int k = tid, i = 0; k < n * 2 * kRows; k += C::kThreads, ++i)
+      if (i < 2) keep_ml[i] = sh.ml[sh.list_of[k / (2 * kRows)]][k % (2 * kRows)];
+    __syncthreads();
+    for (int k = tid, i = 0; k < n * 2 * kRows; k += C::kThreads, ++i)
+      if (i < 2) sh.ml[x + k / (2 * kRows)][k % (2 * kRows)] = keep_ml[i];
+    __syncthreads();
+    join<T, D, NT, C::kThreads>(a, n, id, sh.ml + x,
+                                [&](int i) -> const float* {
+                                  const int p = sh.list_of[i];
+                                  return sh.in_ring[p] ? reinterpret_cast<const float*>(smem + (p >> 1) * kSlots * kTile)
+                                                       : first_o(p >> 1);
+                                },
+                                part);
     if (part && tid == 0) {
       part->id = id;
       part->begins = begins;
       part->ends = ends;
-      // the CTA that holds the last unit of this (sequence, head, group)
       part->last = 0;
       if (!ends) {
-        const long long here = piece_begin(total, first_part + (last >> 1) + 1, parts);  // list position after the piece
-        const long long end = here + (sh.nu[last >> 1][last & 1] - sh.to[last >> 1][last & 1]);
+        const long long here = piece_begin(total, first_part + (last >> 1) + 1, parts);  // the list position behind it
+        const long long end = here + (sh.nu[last] - sh.to[last]);
         part->last = piece_of(total, end - 1, parts) / kWarps;
       }
     }
@@ -882,85 +943,107 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 // it begins there.  The pieces lie in the CTAs up to `last` (a short list
 // leaves some of them without a unit).
 constexpr int kMaxCtas = 192;
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) gqa_join_kernel(const GqaArgs a) {
+constexpr int kJoinThreads = 256;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) gqa_join_kernel(const GqaArgs a) {
+  constexpr int kRows = 8 * NT;
   __shared__ float ml[kMaxCtas][2 * kRows];
+  __shared__ int there[kMaxCtas];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Partial<D>* all = reinterpret_cast<const Partial<D>*>(a.ws);
-  const Partial<D>* p = all + (int64_t)blockIdx.x * 2 + 1;
-  const int id = p->id;
+  const Partial<D, NT>* all = reinterpret_cast<const Partial<D, NT>*>(a.ws);
+  const Partial<D, NT>* p = all + (int64_t)blockIdx.x * 2 + 1;
+  const int id = p->id, n = p->last - (int)blockIdx.x + 1;
   if (id < 0) return;
-  const int n = p->last - (int)blockIdx.x + 1;
   auto piece = [&](int i) { return i == 0 ? p : all + (int64_t)(blockIdx.x + i) * 2; };
-  for (int k = threadIdx.x; k < n * kRows; k += kThreads) {
-    const Partial<D>* x = piece(k / kRows);
-    const bool there = x->id == id;
-    ml[k / kRows][k % kRows] = there ? x->m[k % kRows] : -INFINITY;
-    ml[k / kRows][kRows + k % kRows] = there ? x->l[k % kRows] : 0.f;
+  for (int k = threadIdx.x; k < n * kRows; k += kJoinThreads) {
+    const int i = k / kRows, row = k % kRows;
+    const Partial<D, NT>* x = piece(i);
+    const bool is = x->id == id;
+    const float xm = x->m[row], xl = x->l[row];
+    ml[i][row] = is ? xm : -INFINITY;
+    ml[i][kRows + row] = is ? xl : 0.f;
+    if (row == 0) there[i] = is;
   }
   __syncthreads();
-  join<T, D>(a, n, id, [&](int i) -> const float* { return ml[i]; },
-             // a piece that is not there has no values: any finite ones do, their factor is 0
-             [&](int i) -> const float* { return ml[i][0] == -INFINITY && piece(i)->id != id ? p->o : piece(i)->o; },
-             (Partial<D>*)nullptr);
+  join<T, D, NT, kJoinThreads>(a, n, id, ml,
+                               // one that is not there has no values: any of this id do, its factor is 0
+                               [&](int i) -> const float* { return there[i] ? piece(i)->o : p->o; },
+                               (Partial<D, NT>*)nullptr);
 }
 
 // ------------------------------------------------------------------ weights
 // One CTA takes a contiguous piece of the units of all (sequence, KV head)
-// pairs, its warps every eighth unit of it.  A unit's 32 weights are the sum
-// over all rows: thread (j, c) adds p of its rows, then the eight j are
-// joined by a halving exchange that leaves one position per lane.  Rows of
-// more than one group have their fragments of q in shared memory, up to
-// kHeldGroups of them; more take further passes over the piece.
-constexpr int kHeldGroups = 16;
-template <int D>
+// pairs, its warps every kWarps-th unit of it.  K's fragments are widened
+// once per unit and multiplied with the n-tiles of 8 rows one after another;
+// a thread adds p of its rows, then the four c are joined by a halving
+// exchange that leaves one position per lane.  One n-tile's q stays in the
+// registers of every warp; more stand in shared memory, up to kHeldTiles of
+// them, and further ones take further passes over the piece.
+constexpr int kHeldTiles = 32;
+template <int D, bool ONE>
+struct Wts {
+  static constexpr int kUnit = ONE ? 64 : 32;
+  static constexpr int kWarps = 12;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kTile = kUnit * D;
+  static constexpr int kSlots = 2;
+  static constexpr int kQBytes = ONE ? 0 : kHeldTiles * (D / 16) * 2 * 32 * 4;
+};
+template <int D, bool ONE>
 struct WeightsShared {
-  uint64_t full[kWarps][Ring<D, false>::kStages];
-  ListShared list;
-  float factor[kHeldGroups][kRows], lse[kHeldGroups][kRows];
+  uint64_t full[Wts<D, ONE>::kWarps][Wts<D, ONE>::kSlots];
+  ListShared<Wts<D, ONE>::kWarps> list;
+  float factor[ONE ? 1 : kHeldTiles][8], lse[ONE ? 1 : kHeldTiles][8];
   int abort;
 };
 template <int D, bool ONE>
 constexpr int weights_smem() {
-  return 1024 + kWarps * Ring<D, false>::kBytes + (ONE ? 0 : kHeldGroups * (D / 16) * 4 * 32 * 4) +
-         (int)sizeof(WeightsShared<D>);
+  using C = Wts<D, ONE>;
+  return 1024 + C::kWarps * C::kSlots * C::kTile + C::kQBytes + (int)sizeof(WeightsShared<D, ONE>);
+}
+
+// lse of row r in log2 units; +inf, which makes its p 0, for a row that is
+// not there or that saw nothing.
+__device__ __forceinline__ float lse_log2(const GqaArgs& a, int b, int kvh, int r, int rows) {
+  if (r >= rows) return INFINITY;
+  const float x = __ldg(a.lse_in + ((int64_t)b * a.h_q + kvh * a.g + r % a.g) * a.s_q + r / a.g) * kLog2e;
+  return x == -INFINITY ? INFINITY : x;
 }
 
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Wts<D, ONE>::kThreads, 1)
 gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
-  using R = Ring<D, false>;
-  constexpr int kStages = R::kStages;
-  constexpr int kQ = D / 16;
+  using C = Wts<D, ONE>;
+  constexpr int kWarps = C::kWarps, kSlots = C::kSlots, kTile = C::kTile, kSteps = D / 16;
+  constexpr int kUnit = C::kUnit, kRuns = kUnit / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint4* q_held = reinterpret_cast<uint4*>(smem + kWarps * R::kBytes);  // [group][k-step][lane]
-  WeightsShared<D>& sh =
-      *reinterpret_cast<WeightsShared<D>*>(smem + kWarps * R::kBytes + (ONE ? 0 : kHeldGroups * kQ * 32 * 16));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane >> 2, c = lane & 3;
-  const uint32_t ring = smem_u32(smem + warp * R::kBytes);
+  uint4* q_held = reinterpret_cast<uint4*>(smem + kWarps * kSlots * kTile);  // [n-tile][two k-steps][lane]
+  WeightsShared<D, ONE>& sh =
+      *reinterpret_cast<WeightsShared<D, ONE>*>(smem + kWarps * kSlots * kTile + C::kQBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(smem + warp * kSlots * kTile);
   uint64_t* full = sh.full[warp];
   if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], 1);
     fence_mbarrier_init();
   }
   if (tid == 0) sh.abort = 0;
   const int rows = a.g * a.s_q;
   const long long parts = gridDim.x;
-  find_places(a, a.h_kv, 1, sh.list, [&](int, long long total) { return piece_begin(total, blockIdx.x, parts); });
+  find_places<kWarps, kUnit>(a, a.h_kv, 1, sh.list,
+                      [&](int, long long total) { return piece_begin(total, blockIdx.x, parts); });
   const long long total = sh.list.total;
   const long long mine = piece_begin(total, blockIdx.x + 1, parts) - piece_begin(total, blockIdx.x, parts);
-  const int b0 = sh.list.b[0];
-  const long long u0 = mine > 0 ? sh.list.u[0] : 0;
 
   struct Cursor {
-    int b, kvh, u, nu, len;
-    long long left;
+    int b, kvh, u, nu, len, end;
   };
   auto enter = [&](Cursor& x) {
     if (x.b >= a.b) return;
     x.len = held_len(a, x.b);
-    x.nu = max(1, (x.len + kUnit - 1) / kUnit);
+    x.end = __ldg(a.ctx + x.b) - a.s_q + 1;
+    x.nu = units_of<kUnit>(x.len);
   };
   auto skip = [&](Cursor& x, int n) {  // n units on
     x.u += n;
@@ -975,214 +1058,210 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
   };
   Cursor start = {};
   if (mine > 0) {
-    start.b = b0;
+    start.b = sh.list.b[0];
     enter(start);
-    start.kvh = (int)(u0 / start.nu);
-    start.u = (int)(u0 - (long long)start.kvh * start.nu);
+    const long long u = sh.list.u[0];
+    start.kvh = (int)(u / start.nu);
+    start.u = (int)(u - (long long)start.kvh * start.nu);
   }
-  const long long my_units = mine > warp ? (mine - warp + kWarps - 1) / kWarps : 0;
-  Cursor first = start;  // this warp's first unit
-  if (my_units > 0) skip(first, warp);
-  first.left = my_units;
+  const int units = mine > warp ? (int)((mine - warp + kWarps - 1) / kWarps) : 0;  // this warp's
+  Cursor first = start;
+  if (units > 0) skip(first, warp);
 
+  int slot = 0;
   uint32_t phase = 0;
-  int st = 0;
   bool ok = true;
-  uint32_t q[kQ][4];
+  uint32_t q[kSteps][2];
   float factor[2], lse2[2];
-  for (int g0 = 0; g0 < a.groups; g0 += kHeldGroups) {
-    const int ng = min(kHeldGroups, a.groups - g0);
+  Info<kUnit> now, next;  // of the unit at the products' cursor, and of the one behind it
+  const int tiles = (rows + 7) / 8;
+  for (int n0 = 0; n0 < tiles; n0 += kHeldTiles) {
+    const int nt = min(kHeldTiles, tiles - n0), q_first = n0 * 8 / a.g;
     Cursor ld = first, cur = first;
-    Pages pages = {-1, -1, -1};
-    float scales[kStages];
-    int held[kStages];
+    int to_load = ok ? units : 0, left = to_load;
+    Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
+    auto load_next = [&](int to) {
+      if (to_load == 0) return;
+      fetch_pages<kUnit, false>(a, pages, ld.b, ld.kvh, ld.u, ld.len);
+      int ids[kRuns];
+      next.held = 0;
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) {
-      const int x = (st + s) % kStages;
-      float sc = 1.f;
-      int h = 0;
-      if (ld.left > 0 && ok) {
-        h = load_unit<D, false>(a, &tk, &tk, pages, ld.b, ld.kvh, ld.u, ld.len, ring + x * R::kStage, &full[x], sc,
-                                false);
-        --ld.left;
-        if (ld.left > 0) skip(ld, kWarps);
+      for (int i = 0; i < kRuns; ++i) {
+        const int from = (ld.u - pages.base) * kRuns + i;
+        ids[i] = __shfl_sync(0xffffffffu, pages.id, from);
+        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, from);
+        next.held |= (ids[i] >= 0 ? 1 : 0) << i;
       }
-#pragma unroll
-      for (int i = 0; i < kStages; ++i) {
-        held[i] = x == i ? h : held[i];
-        scales[i] = x == i ? sc : scales[i];
-      }
-    }
+      if (lane == 0) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + to * kTile, &full[to]);
+      if (--to_load > 0) skip(ld, kWarps);
+    };
+    load_next(slot);
+    now = next;
+    load_next((slot + 1) % kSlots);
     // the pairs of the piece, one after another
     Cursor pair = start;
     long long to_go = mine;
-    bool fresh = true;
     while (to_go > 0) {
       const long long in_pair = min(to_go, (long long)(pair.nu - pair.u));
       if constexpr (!ONE) {
         __syncthreads();  // the last pair's fragments are read
-        for (int gr = warp; gr < ng; gr += kWarps) {
-          uint32_t f[kQ][4];
+        for (int n = warp; n < nt; n += kWarps) {
+          uint32_t f[kSteps][2];
           float fac[2];
-          load_q<T, D>(a, pair.b, pair.kvh, (g0 + gr) * kRows, rows, f, fac);
+          load_q<T, D>(a, pair.b, pair.kvh, (n0 + n) * 8, rows, f, fac);
 #pragma unroll
-          for (int s = 0; s < kQ; ++s) q_held[(gr * kQ + s) * 32 + lane] = make_uint4(f[s][0], f[s][1], f[s][2], f[s][3]);
-          if (c == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int r = (g0 + gr) * kRows + j + 8 * i;
-              float e = INFINITY;  // a row that is not there, or saw nothing, adds exp2(-inf)
-              if (r < rows) {
-                e = __ldg(a.lse_in + ((int64_t)pair.b * a.h_q + pair.kvh * a.g + r % a.g) * a.s_q + r / a.g) * kLog2e;
-                if (e == -INFINITY) e = INFINITY;
-              }
-              sh.factor[gr][j + 8 * i] = fac[i];
-              sh.lse[gr][j + 8 * i] = e;
-            }
+          for (int s = 0; s < kSteps; s += 2)
+            q_held[(n * (kSteps / 2) + s / 2) * 32 + lane] = make_uint4(f[s][0], f[s][1], f[s + 1][0], f[s + 1][1]);
+          if (g == 0) {
+            sh.factor[n][2 * c] = fac[0];
+            sh.factor[n][2 * c + 1] = fac[1];
           }
+          if (lane < 8) sh.lse[n][lane] = lse_log2(a, pair.b, pair.kvh, (n0 + n) * 8 + lane, rows);
         }
         __syncthreads();
       }
-      fresh = true;
-      while (ok && cur.left > 0 && cur.b == pair.b && cur.kvh == pair.kvh) {
+      bool fresh = true;
+      while (ok && left > 0 && cur.b == pair.b && cur.kvh == pair.kvh) {
         if constexpr (ONE) {
           if (fresh) {
             load_q<T, D>(a, cur.b, cur.kvh, 0, rows, q, factor);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int r = j + 8 * i;
-              lse2[i] = INFINITY;
-              if (r < rows) {
-                lse2[i] = __ldg(a.lse_in + ((int64_t)cur.b * a.h_q + cur.kvh * a.g + r % a.g) * a.s_q + r / a.g) * kLog2e;
-                if (lse2[i] == -INFINITY) lse2[i] = INFINITY;
-              }
-            }
+            lse2[0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
+            lse2[1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
             fresh = false;
           }
         }
-        int held_now = held[0];
-        float scale_now = scales[0];
-#pragma unroll
-        for (int i = 1; i < kStages; ++i) {
-          held_now = st == i ? held[i] : held_now;
-          scale_now = st == i ? scales[i] : scale_now;
-        }
-        const float ks[2] = {__shfl_sync(0xffffffffu, scale_now, 0), __shfl_sync(0xffffffffu, scale_now, 1)};
         const int t0 = cur.u * kUnit;
-        const int end = __ldg(a.ctx + cur.b) - a.s_q + 1;
-        const bool edge = t0 + kUnit > min(cur.len, end) || held_now != 3;
-        // the position whose weight this lane will hold
-        const int t_mine = t0 + 8 * (j >> 1) + Lay<D>::perm(2 * c + (j & 1));
+        const bool edge = t0 + kUnit > min(cur.len, cur.end + q_first) || now.held != (1 << kRuns) - 1;
+        // the positions whose weights this lane will hold
+        const int t_mine = t0 + 8 * c + Lay<D>::perm(g);
         float* w = a.weights + (int64_t)cur.b * a.stride_w_b + (int64_t)cur.kvh * a.stride_w_h + t_mine;
-        const bool write = t_mine < cur.len && t_mine < a.width;
-        const float before = write && (a.accumulate || g0 > 0) ? *w : 0.f;
-        ok = mbar_wait(&full[st], phase, &sh.abort, &g_gqa_status);
-        if (!ok) break;
-        float sum[8];
+        float before[kUnit / 32];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] = 0.f;
-        for (int gr = 0; gr < ng; ++gr) {
-          if constexpr (!ONE) {
-#pragma unroll
-            for (int s = 0; s < kQ; ++s) {
-              const uint4 f = q_held[(gr * kQ + s) * 32 + lane];
-              q[s][0] = f.x;
-              q[s][1] = f.y;
-              q[s][2] = f.z;
-              q[s][3] = f.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              factor[i] = sh.factor[gr][j + 8 * i];
-              lse2[i] = sh.lse[gr][j + 8 * i];
-            }
-          }
-          float s[4][4];
-          score_unit<D>(ring + st * R::kStage, q, s);
-          const int lim0 = end + ((g0 + gr) * kRows + j) / a.g, lim1 = end + ((g0 + gr) * kRows + j + 8) / a.g;
-#pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float p0 = fast_exp2(s[nt][k] * (factor[0] * ks[nt >> 1]) - lse2[0]);
-              float p1 = fast_exp2(s[nt][2 + k] * (factor[1] * ks[nt >> 1]) - lse2[1]);
-              if (edge) {
-                const int t = t0 + nt * 8 + Lay<D>::perm(2 * c + k);
-                const bool there = (held_now >> (nt >> 1)) & 1;
-                p0 = there && t < lim0 ? p0 : 0.f;
-                p1 = there && t < lim1 ? p1 : 0.f;
-              }
-              sum[2 * nt + k] += p0 + p1;
-            }
-          }
+        for (int x = 0; x < kUnit / 32; ++x) {
+          const int t = t_mine + 32 * x;
+          before[x] = (a.accumulate || n0 > 0) && t < cur.len && t < a.width ? w[32 * x] : 0.f;
         }
-        // eight values over the eight j: each step sends half of them
+        if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+        uint32_t f[ONE ? 1 : kRuns][ONE ? 1 : D / 64][4][4];
+        float s[kRuns][4];
+        if constexpr (ONE) {
 #pragma unroll
-        for (int h = 4; h >= 1; h >>= 1) {
-          const bool up = lane & (h * 4);
+          for (int mt = 0; mt < kRuns; ++mt) {
+            s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
 #pragma unroll
-          for (int i = 0; i < h; ++i) {
-            const float send = up ? sum[i] : sum[i + h], keep = up ? sum[i + h] : sum[i];
-            sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, h * 4);
+            for (int h = 0; h < D / 64; ++h) {
+              k_frags<D>(ring + slot * kTile, mt, h, f[0][0]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_f16(s[mt], f[0][0][k][0], f[0][0][k][1], f[0][0][k][2], f[0][0][k][3], q[4 * h + k][0], q[4 * h + k][1]);
+            }
           }
+        } else {
+#pragma unroll
+          for (int mt = 0; mt < kRuns; ++mt)
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) k_frags<D>(ring + slot * kTile, mt, h, f[mt][h]);
         }
-        if (write) *w = before + sum[0];
         __syncwarp();
-        if (ld.left > 0) {
-          held_now = load_unit<D, false>(a, &tk, &tk, pages, ld.b, ld.kvh, ld.u, ld.len, ring + st * R::kStage,
-                                         &full[st], scale_now, false);
-#pragma unroll
-          for (int i = 0; i < kStages; ++i) {
-            held[i] = st == i ? held_now : held[i];
-            scales[i] = st == i ? scale_now : scales[i];
-          }
-          --ld.left;
-          if (ld.left > 0) skip(ld, kWarps);
-        }
-        --cur.left;
-        if (cur.left > 0) skip(cur, kWarps);
-        if (++st == kStages) {
-          st = 0;
+        const Info<kUnit> here = now;
+        now = next;
+        load_next(slot);
+        if (++slot == kSlots) {
+          slot = 0;
           phase ^= 1;
         }
+        float sum[2 * kRuns];  // positions 8 i + perm(g)
+#pragma unroll
+        for (int i = 0; i < 2 * kRuns; ++i) sum[i] = 0.f;
+        for (int n = 0; n < nt; ++n) {
+          if constexpr (!ONE) {
+#pragma unroll
+            for (int k = 0; k < kSteps; k += 2) {
+              const uint4 x = q_held[(n * (kSteps / 2) + k / 2) * 32 + lane];
+              q[k][0] = x.x;
+              q[k][1] = x.y;
+              q[k + 1][0] = x.z;
+              q[k + 1][1] = x.w;
+            }
+            const float2 x = *reinterpret_cast<const float2*>(&sh.factor[n][2 * c]);
+            const float2 y = *reinterpret_cast<const float2*>(&sh.lse[n][2 * c]);
+            factor[0] = x.x;
+            factor[1] = x.y;
+            lse2[0] = y.x;
+            lse2[1] = y.y;
+#pragma unroll
+            for (int mt = 0; mt < kRuns; ++mt) s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int mt = 0; mt < kRuns; ++mt)
+                  mma_f16(s[mt], f[mt][h][k][0], f[mt][h][k][1], f[mt][h][k][2], f[mt][h][k][3], q[4 * h + k][0],
+                          q[4 * h + k][1]);
+          }
+          if (!edge) {
+#pragma unroll
+            for (int i = 0; i < 2 * kRuns; ++i)
+              sum[i] += fast_exp2(fmaf(s[i >> 1][2 * (i & 1)], factor[0] * here.ks[i >> 1], -lse2[0])) +
+                        fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + 1], factor[1] * here.ks[i >> 1], -lse2[1]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2 * kRuns; ++i) {
+              const bool there = (here.held >> (i >> 1)) & 1;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float p = fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + k], factor[k] * here.ks[i >> 1], -lse2[k]));
+                const int lim = cur.end + ((n0 + n) * 8 + 2 * c + k) / a.g;
+                sum[i] += there && t0 + 8 * i + Lay<D>::perm(g) < lim ? p : 0.f;
+              }
+            }
+          }
+        }
+        // four values over the four c: each step sends half of them
+#pragma unroll
+        for (int x = 0; x < kUnit / 32; ++x) {
+#pragma unroll
+          for (int h = 2; h >= 1; h >>= 1) {
+            const bool up = lane & h;
+#pragma unroll
+            for (int i = 4 * x; i < 4 * x + h; ++i) {
+              const float send = up ? sum[i] : sum[i + h], keep = up ? sum[i + h] : sum[i];
+              sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, h);
+            }
+          }
+          const int t = t_mine + 32 * x;
+          if (t < cur.len && t < a.width) w[32 * x] = before[x] + sum[4 * x];
+        }
+        if (--left > 0) skip(cur, kWarps);
       }
       to_go -= in_pair;
       if (to_go > 0) skip(pair, (int)in_pair);
     }
-    if (!ok) {  // this warp's loads in flight land (or their waits run out) before its shared memory goes
-      const int flying = (int)min((long long)kStages, cur.left - ld.left);
-      for (int i = 0; i < flying; ++i) {
-        const int x = (st + i) % kStages;
-        const long long t = clock64();
-        while (!mbar_try_wait(smem_u32(&full[x]), phase ^ (x < st ? 1u : 0u), 1000u) &&
-               clock64() - t < kWaitLimitCycles) {
-        }
-      }
-      first.left = 0;
-    }
+    if (!ok && left > 0) drain(full, kSlots, slot, phase, left - to_load);
   }
   if (!a.accumulate) {  // zeros behind each context
     for (int x = blockIdx.x; x < a.b * a.h_kv; x += gridDim.x) {
       float* w = a.weights + (int64_t)(x / a.h_kv) * a.stride_w_b + (int64_t)(x % a.h_kv) * a.stride_w_h;
-      for (int t = held_len(a, x / a.h_kv) + tid; t < a.width; t += kThreads) w[t] = 0.f;
+      for (int t = held_len(a, x / a.h_kv) + tid; t < a.width; t += C::kThreads) w[t] = 0.f;
     }
   }
 }
 
 // ------------------------------------------------------------------ host
-// [num_blocks][h_kv][page][d] of one byte, boxes of up to 32 rows of a head.
+// [num_blocks][h_kv][page][d] of one byte, boxes of up to `unit` rows of a head.
 bool make_map(CUtensorMap* m, const void* base, int64_t stride_block, int64_t stride_row, int64_t stride_head,
-              const dsv4b_gqa_cache& c) {
+              int unit, const dsv4b_gqa_cache& c) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
   if (!enc) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)c.d, (cuuint64_t)c.page_block_size, (cuuint64_t)c.h_kv,
                               (cuuint64_t)c.num_blocks};
   const cuuint64_t strides[3] = {(cuuint64_t)stride_row, (cuuint64_t)stride_head, (cuuint64_t)stride_block};
-  const cuuint32_t box[4] = {(cuuint32_t)c.d, (cuuint32_t)(c.page_block_size < kUnit ? c.page_block_size : kUnit), 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)c.d, (cuuint32_t)(c.page_block_size < unit ? c.page_block_size : unit), 1, 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, c.d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 GqaArgs make_args(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q) {
@@ -1195,7 +1274,6 @@ GqaArgs make_args(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q) {
   a.h_q = q.h_q;
   a.h_kv = c.h_kv;
   a.g = q.h_q / c.h_kv;
-  a.groups = (a.g * q.s_q + kRows - 1) / kRows;
   a.scale_log2 = q.sm_scale * kLog2e;
   a.k_scale = c.k_scale;
   a.v_scale = c.v_scale;
@@ -1223,26 +1301,33 @@ cudaError_t allow_smem(K* kernel, int bytes, bool (&done)[64]) {
   return e;
 }
 
-template <typename T, int D>
-cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const GqaArgs& a, int grid,
-                          cudaStream_t stream) {
-  constexpr int smem = decode_smem<D>();
+template <typename T, int D, int NT>
+cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, GqaArgs a, int grid, cudaStream_t stream) {
+  using C = Dec<D, NT>;
+  constexpr int smem = decode_smem<D, NT>();
   static_assert(smem <= 227 * 1024, "decode kernel shared memory");
   static bool done[64] = {};
-  cudaError_t e = allow_smem(&gqa_decode_kernel<T, D>, smem, done);
+  cudaError_t e = allow_smem(&gqa_decode_kernel<T, D, NT>, smem, done);
   if (e != cudaSuccess) return e;
-  gqa_decode_kernel<T, D><<<grid, kThreads, smem, stream>>>(tk, tv, a);
+  a.groups = (a.g * a.s_q + C::kRows - 1) / C::kRows;
+  gqa_decode_kernel<T, D, NT><<<grid, C::kThreads, smem, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr;  // its launch overlaps the decode; it waits in the kernel
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gqa_join_kernel<T, D>, a);
+  return cudaLaunchKernelEx(&cfg, gqa_join_kernel<T, D, NT>, a);
+}
+
+template <typename T, int D>
+cudaError_t pick_decode(const CUtensorMap& tk, const CUtensorMap& tv, const GqaArgs& a, int grid, cudaStream_t stream) {
+  return a.g * a.s_q <= 8 ? launch_decode<T, D, 1>(tk, tv, a, grid, stream)
+                          : launch_decode<T, D, 2>(tk, tv, a, grid, stream);
 }
 
 template <typename T, int D, bool ONE>
@@ -1252,22 +1337,32 @@ cudaError_t launch_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cu
   static bool done[64] = {};
   cudaError_t e = allow_smem(&gqa_weights_kernel<T, D, ONE>, smem, done);
   if (e != cudaSuccess) return e;
-  gqa_weights_kernel<T, D, ONE><<<grid, kThreads, smem, stream>>>(tk, a);
+  gqa_weights_kernel<T, D, ONE><<<grid, Wts<D, ONE>::kThreads, smem, stream>>>(tk, a);
   return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t pick_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cudaStream_t stream) {
+  return a.g * a.s_q <= 8 ? launch_weights<T, D, true>(tk, a, grid, stream)
+                          : launch_weights<T, D, false>(tk, a, grid, stream);
 }
 
 }  // namespace
 
 size_t gqa_decode_ws_bytes(int sms, int d) {
-  return (size_t)grid_of(sms) * 2 * (d == 128 ? sizeof(Partial<128>) : sizeof(Partial<64>));
+  const int n = grid_of(sms);
+  const size_t one = d == 128 ? ws_bytes<128, 1>(n) : ws_bytes<64, 1>(n);
+  const size_t two = d == 128 ? ws_bytes<128, 2>(n) : ws_bytes<64, 2>(n);
+  return one > two ? one : two;
 }
 
 cudaError_t launch_gqa_decode(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q, void* out, int64_t stride_o_b,
                               int64_t stride_o_s, int64_t stride_o_h, float* lse, void* ws, int sms,
                               cudaStream_t stream, int* bad_arg) {
   CUtensorMap tk, tv;
-  if (!make_map(&tk, c.k, c.stride_k_block, c.stride_k_row, c.stride_k_head, c) ||
-      !make_map(&tv, c.v, c.stride_v_block, c.stride_v_row, c.stride_v_head, c)) {
+  constexpr int kUnit = Dec<128, 1>::kUnit;  // every variant's
+  if (!make_map(&tk, c.k, c.stride_k_block, c.stride_k_row, c.stride_k_head, kUnit, c) ||
+      !make_map(&tv, c.v, c.stride_v_block, c.stride_v_row, c.stride_v_head, kUnit, c)) {
     *bad_arg = 1;
     return cudaErrorInvalidValue;
   }
@@ -1280,21 +1375,22 @@ cudaError_t launch_gqa_decode(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q
   a.ws = static_cast<float*>(ws);
   const int grid = grid_of(sms);
   if (q.dtype == DSV4B_BF16)
-    return c.d == 128 ? launch_decode<__nv_bfloat16, 128>(tk, tv, a, grid, stream)
-                      : launch_decode<__nv_bfloat16, 64>(tk, tv, a, grid, stream);
-  return c.d == 128 ? launch_decode<__half, 128>(tk, tv, a, grid, stream)
-                    : launch_decode<__half, 64>(tk, tv, a, grid, stream);
+    return c.d == 128 ? pick_decode<__nv_bfloat16, 128>(tk, tv, a, grid, stream)
+                      : pick_decode<__nv_bfloat16, 64>(tk, tv, a, grid, stream);
+  return c.d == 128 ? pick_decode<__half, 128>(tk, tv, a, grid, stream)
+                    : pick_decode<__half, 64>(tk, tv, a, grid, stream);
 }
 
 cudaError_t launch_gqa_weights(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& q, const float* lse, float* weights,
                                int64_t stride_w_b, int64_t stride_w_h, int width, int accumulate, int sms,
                                cudaStream_t stream, int* bad_arg) {
+  GqaArgs a = make_args(c, q);
   CUtensorMap tk;
-  if (!make_map(&tk, c.k, c.stride_k_block, c.stride_k_row, c.stride_k_head, c)) {
+  const int unit = a.g * a.s_q <= 8 ? Wts<128, true>::kUnit : Wts<128, false>::kUnit;
+  if (!make_map(&tk, c.k, c.stride_k_block, c.stride_k_row, c.stride_k_head, unit, c)) {
     *bad_arg = 1;
     return cudaErrorInvalidValue;
   }
-  GqaArgs a = make_args(c, q);
   a.lse_in = lse;
   a.weights = weights;
   a.stride_w_b = stride_w_b;
@@ -1302,19 +1398,10 @@ cudaError_t launch_gqa_weights(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& 
   a.width = width;
   a.accumulate = accumulate;
   const int grid = grid_of(sms);
-  const bool one = a.groups == 1;  // one group's q stays in registers, without a barrier per pair
-  if (q.dtype == DSV4B_BF16) {
-    if (c.d == 128)
-      return one ? launch_weights<__nv_bfloat16, 128, true>(tk, a, grid, stream)
-                 : launch_weights<__nv_bfloat16, 128, false>(tk, a, grid, stream);
-    return one ? launch_weights<__nv_bfloat16, 64, true>(tk, a, grid, stream)
-               : launch_weights<__nv_bfloat16, 64, false>(tk, a, grid, stream);
-  }
-  if (c.d == 128)
-    return one ? launch_weights<__half, 128, true>(tk, a, grid, stream)
-               : launch_weights<__half, 128, false>(tk, a, grid, stream);
-  return one ? launch_weights<__half, 64, true>(tk, a, grid, stream)
-             : launch_weights<__half, 64, false>(tk, a, grid, stream);
+  if (q.dtype == DSV4B_BF16)
+    return c.d == 128 ? pick_weights<__nv_bfloat16, 128>(tk, a, grid, stream)
+                      : pick_weights<__nv_bfloat16, 64>(tk, a, grid, stream);
+  return c.d == 128 ? pick_weights<__half, 128>(tk, a, grid, stream) : pick_weights<__half, 64>(tk, a, grid, stream);
 }
 
 cudaError_t read_gqa_status(int* flags, cudaStream_t stream) {
