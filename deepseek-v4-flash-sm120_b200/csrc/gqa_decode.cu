@@ -189,10 +189,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// Four consecutive values of a 16-bit row.
+// Four 16-bit values.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p) {
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+__device__ __forceinline__ float4 four(uint2 w) {
   if constexpr (std::is_same_v<T, __half>) {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
@@ -208,19 +207,30 @@ __device__ __forceinline__ float4 load4(const T* p) {
 // it reads of K.  Rows from `rows` on are zero.  factor[k] is what the
 // products of row 2c + k are multiplied by: the row's power of two and the
 // softmax scale.
+template <int D>
+struct RawQ {
+  uint2 w[D / 16];
+};
 template <typename T, int D>
-__device__ __forceinline__ void load_q(const GqaArgs& a, int b, int kvh, int r0, int rows, uint32_t (&q)[D / 16][2],
-                                       float (&factor)[2]) {
+__device__ __forceinline__ void fetch_q(const GqaArgs& a, int b, int kvh, int r0, int rows, RawQ<D>& raw) {
   const int lane = threadIdx.x & 31, c = lane & 3, r = r0 + (lane >> 2);
   const bool live = r < rows;
   const T* p = static_cast<const T*>(a.q);
   if (live)
     p += (int64_t)b * a.stride_q_b + (int64_t)(r / a.g) * a.stride_q_s + (int64_t)(kvh * a.g + r % a.g) * a.stride_q_h;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+    raw.w[s] = live ? __ldg(reinterpret_cast<const uint2*>(p + (s >> 2) * 64 + c * 16 + (s & 3) * 4)) : make_uint2(0, 0);
+}
+template <typename T, int D>
+__device__ __forceinline__ void scale_q(const GqaArgs& a, const RawQ<D>& raw, uint32_t (&q)[D / 16][2],
+                                        float (&factor)[2]) {
+  const int c = threadIdx.x & 3;
   float4 f[D / 16];
   float top = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
-    f[s] = live ? load4(p + (s >> 2) * 64 + c * 16 + (s & 3) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    f[s] = four<T>(raw.w[s]);
     top = fmaxf(top, fmaxf(fmaxf(fabsf(f[s].x), fabsf(f[s].y)), fmaxf(fabsf(f[s].z), fabsf(f[s].w))));
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -236,6 +246,13 @@ __device__ __forceinline__ void load_q(const GqaArgs& a, int b, int kvh, int r0,
   }
   factor[0] = __shfl_sync(0xffffffffu, down, 8 * c);
   factor[1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+}
+template <typename T, int D>
+__device__ __forceinline__ void load_q(const GqaArgs& a, int b, int kvh, int r0, int rows, uint32_t (&q)[D / 16][2],
+                                       float (&factor)[2]) {
+  RawQ<D> raw;
+  fetch_q<T, D>(a, b, kvh, r0, rows, raw);
+  scale_q<T, D>(a, raw, q, factor);
 }
 
 // K's fragments of 16 positions of a tile for k-steps 4 h .. 4 h + 3.
@@ -253,6 +270,27 @@ __device__ __forceinline__ void k_frags(uint32_t tile, int mt, int h, uint32_t (
 }
 
 // ------------------------------------------------------------------ the list
+// `parts` equal pieces of a list (the first `more` of them one unit longer):
+// where piece i begins, and which piece holds position x.
+struct Split {
+  long long each;
+  int more;
+  __device__ __forceinline__ Split(long long total, int parts) {
+    if (total < (1ll << 31)) {  // a 64-bit division takes a microsecond of a cold start
+      each = (unsigned)total / (unsigned)parts;
+      more = (int)((unsigned)total - (unsigned)each * (unsigned)parts);
+    } else {
+      each = total / parts;
+      more = (int)(total - each * parts);
+    }
+  }
+  __device__ __forceinline__ long long begin(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int holder(long long x) const {
+    const long long longer = (each + 1) * more;
+    return x < longer ? (int)(x / (each + 1)) : more + (int)((x - longer) / each);
+  }
+};
+
 template <int W>
 struct ListShared {
   long long sum[W];
@@ -261,13 +299,14 @@ struct ListShared {
   long long u[W];
 };
 
-// Where n wanted positions of the list of all sequences' units (per_seq
-// times over for a sequence's heads and groups) lie: sh.b[k] the sequence
-// (-1: past the end), sh.u[k] the unit among all of the sequence's.  Every
-// thread sums a run of sequences, the sums are scanned, and the thread whose
-// run holds a wanted position walks to it.
-template <int W, int U, typename Want>
-__device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n, ListShared<W>& sh, Want want) {
+// Where n pieces, from part0 on, of `parts` equal ones of the list of all
+// sequences' units (per_seq times over for a sequence's heads and groups)
+// begin: sh.b[k] the sequence (-1: past the end), sh.u[k] the unit among all
+// of the sequence's.  Every thread sums a run of sequences, the sums are
+// scanned, and the thread whose run holds a beginning walks to it.
+template <int W, int U>
+__device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int part0, int n, int parts,
+                                            ListShared<W>& sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int run = (a.b + W * 32 - 1) / (W * 32);
   const int i0 = min(a.b, tid * run), i1 = min(a.b, i0 + run);
@@ -290,8 +329,9 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n
   }
   if (tid == 0) sh.total = total;
   if (sum > 0) {
+    const Split split(total, parts);
     for (int k = 0; k < n; ++k) {
-      const long long x = want(k, total);
+      const long long x = split.begin(part0 + k);
       if (x < pre || x >= pre + sum) continue;
       long long at = pre;
       for (int i = i0; i < i1; ++i) {
@@ -306,15 +346,6 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int n
     }
   }
   __syncthreads();
-}
-
-// Where piece i of `parts` equal pieces of a list begins, and which piece
-// holds position x.
-__device__ __forceinline__ long long piece_begin(long long total, long long i, long long parts) {
-  return total * i / parts;
-}
-__device__ __forceinline__ int piece_of(long long total, long long x, long long parts) {
-  return (int)(((x + 1) * parts - 1) / total);
 }
 
 // ------------------------------------------------------------------ loading
@@ -403,13 +434,12 @@ struct Dec {
   static constexpr int kSlots = NT == 1 && D == 128 ? 2 : 3;
 };
 
-// A piece of one (sequence, head, group of rows): id numbers these; begins
-// and ends: whether it holds the first and the last of its units; last: the
-// CTA that holds the last one.  o is not divided by l, both are relative to
+// A piece of one (sequence, head, group of rows): id numbers these; last:
+// the CTA that holds its last unit.  o is not divided by l, both are relative to
 // 2^m.
 template <int D, int NT>
 struct Partial {
-  int id, last, begins, ends;
+  int id, last, unused[2];
   float m[8 * NT], l[8 * NT];
   float o[8 * NT * D];
 };
@@ -432,7 +462,7 @@ struct DecodeShared {
   int id[2 * C::kWarps];  // -1: none
   int from[2 * C::kWarps], to[2 * C::kWarps], nu[2 * C::kWarps], in_ring[2 * C::kWarps];
   float ml[2 * C::kWarps][2 * C::kRows];  // m, l
-  int list_of[2 * C::kWarps];             // pieces of the one that is being joined
+  int list_of[2 * C::kWarps], run[2 * C::kWarps + 1], n_runs;
   int abort;
 };
 template <int D, int NT>
@@ -460,55 +490,52 @@ __device__ __forceinline__ float* lse_at(const GqaArgs& a, int b, int kvh, int r
   return a.lse + ((int64_t)b * a.h_q + kvh * a.g + r % a.g) * a.s_q + r / a.g;
 }
 
-// Joins n pieces of one (sequence, head, group), in order, by all threads:
-// piece i has maxima and sums ml[i] (m, then l) and values o_of(i) [rows][D].
-// Writes the result, or the joined piece to `part`.
-template <typename T, int D, int NT, int THREADS, typename O>
-__device__ __forceinline__ void join(const GqaArgs& a, int n, int id, const float (*ml)[16 * NT], O o_of,
-                                     Partial<D, NT>* part) {
+// Joins n pieces of one (sequence, head, group), in order, for the four
+// consecutive values from e on of its [rows][D]: piece i has maxima and sums
+// ml_of(i) (m, then l) and values o_of(i).  Writes the result, or the joined
+// piece to `part`.
+template <typename T, int D, int NT, typename ML, typename O>
+__device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML ml_of, O o_of, Partial<D, NT>* part) {
   constexpr int kRows = 8 * NT;
   const int grp = id % a.groups, kvh = id / a.groups % a.h_kv, b = id / a.groups / a.h_kv;
-  for (int e = threadIdx.x * 4; e < kRows * D; e += THREADS * 4) {
-    const int row = e / D, d0 = e % D;
-    const int r = grp * kRows + row;
-    if (r >= a.g * a.s_q) continue;
-    float m = -INFINITY;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, ml[i][row]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kDeep = 8;  // loads in flight
-    for (int i0 = 0; i0 < n; i0 += kDeep) {
-      float4 x[kDeep];
+  const int row = e / D, d0 = e % D;
+  const int r = grp * kRows + row;
+  if (r >= a.g * a.s_q) return;
+  float m = -INFINITY;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, ml_of(i)[row]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kDeep = 8;  // loads in flight
+  for (int i0 = 0; i0 < n; i0 += kDeep) {
+    float4 x[kDeep];
 #pragma unroll
-      for (int i = 0; i < kDeep; ++i)
-        x[i] = *reinterpret_cast<const float4*>(o_of(min(i0 + i, n - 1)) + e);
+    for (int i = 0; i < kDeep; ++i) x[i] = *reinterpret_cast<const float4*>(o_of(min(i0 + i, n - 1)) + e);
 #pragma unroll
-      for (int i = 0; i < kDeep; ++i) {
-        if (i0 + i < n) {
-          const float f = fast_exp2(ml[i0 + i][row] - base);  // 0 where nothing was seen
-          l += f * ml[i0 + i][kRows + row];
-          o.x += f * x[i].x;
-          o.y += f * x[i].y;
-          o.z += f * x[i].z;
-          o.w += f * x[i].w;
-        }
+    for (int i = 0; i < kDeep; ++i) {
+      if (i0 + i < n) {
+        const float f = fast_exp2(ml_of(i0 + i)[row] - base);  // 0 where nothing was seen
+        l += f * ml_of(i0 + i)[kRows + row];
+        o.x += f * x[i].x;
+        o.y += f * x[i].y;
+        o.z += f * x[i].z;
+        o.w += f * x[i].w;
       }
     }
-    if (part) {
-      if (d0 == 0) {
-        part->m[row] = m;
-        part->l[row] = l;
-      }
-      *reinterpret_cast<float4*>(part->o + e) = o;
-      continue;
-    }
-    const bool none = m == -INFINITY;
-    const float inv = none ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) =
-        make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
-    if (d0 == 0) *lse_at(a, b, kvh, r) = none ? -INFINITY : (m + log2f(l)) * kLn2;
   }
+  if (part) {
+    if (d0 == 0) {
+      part->m[row] = m;
+      part->l[row] = l;
+    }
+    *reinterpret_cast<float4*>(part->o + e) = o;
+    return;
+  }
+  const bool none = m == -INFINITY;
+  const float inv = none ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) =
+      make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
+  if (d0 == 0) *lse_at(a, b, kvh, r) = none ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 template <typename T, int D, int NT>
@@ -537,11 +564,10 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     sh.id[2 * warp] = sh.id[2 * warp + 1] = -1;
   }
   if (tid == 0) sh.abort = 0;
-  const long long parts = (long long)gridDim.x * kWarps, first_part = (long long)blockIdx.x * kWarps;
-  find_places<kWarps, kUnit>(a, a.h_kv * a.groups, kWarps, sh.list,
-                      [&](int k, long long total) { return piece_begin(total, first_part + k, parts); });
-  const long long total = sh.list.total;
-  int left = (int)(piece_begin(total, first_part + warp + 1, parts) - piece_begin(total, first_part + warp, parts));
+  const int parts = gridDim.x * kWarps, first_part = blockIdx.x * kWarps;
+  find_places<kWarps, kUnit>(a, a.h_kv * a.groups, first_part, kWarps, parts, sh.list);
+  const Split split(sh.list.total, parts);
+  int left = (int)split.each + (first_part + warp < split.more ? 1 : 0);
 
   // the two cursors: where loads and where products are
   struct Cursor {
@@ -566,10 +592,10 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     cur.b = sh.list.b[warp];
     enter(cur);
     const long long u = sh.list.u[warp];
-    const int pair = (int)(u / cur.nu);
+    const int pair = u < (1ll << 31) ? (int)((unsigned)u / (unsigned)cur.nu) : (int)(u / cur.nu);
     cur.u = (int)(u - (long long)pair * cur.nu);
     cur.kvh = pair / a.groups;
-    cur.grp = pair % a.groups;
+    cur.grp = pair - cur.kvh * a.groups;
   }
   Cursor ld = cur;
   int tiles = 2 * left;  // to be loaded
@@ -589,18 +615,28 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int i = 0; i < kRuns; ++i) {
         const int from = (ld.u - pages.base) * kRuns + i;
         ids[i] = __shfl_sync(0xffffffffu, pages.id, from);
-        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, from);
-        next.vs[i] = __shfl_sync(0xffffffffu, pages.vs, from);
         next.held |= (ids[i] >= 0 ? 1 : 0) << i;
       }
       if (lane == 0 && !withhold) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + slot * kTile, &full[slot]);
       withhold = false;
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {  // after the load: these may still be on their way
+        const int from = (ld.u - pages.base) * kRuns + i;
+        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, from);
+        next.vs[i] = __shfl_sync(0xffffffffu, pages.vs, from);
+      }
     } else {
       if (lane == 0) load_tile<D, kUnit>(a, &tv, ids, ld.kvh, ld.u, ring + slot * kTile, &full[slot]);
       advance(ld);
     }
     ld_v = !ld_v;
   };
+  const int rows = a.g * a.s_q;
+  RawQ<D> raw[NT];
+  if (left > 0) {  // the first rows of q, ahead of the tiles that would be in their way
+#pragma unroll
+    for (int n = 0; n < NT; ++n) fetch_q<T, D>(a, cur.b, cur.kvh, cur.grp * kRows + 8 * n, rows, raw[n]);
+  }
   load_next(0);
   now = next;
 #pragma unroll
@@ -612,7 +648,11 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   float m[NT][2], l[NT][2], v_unit = 1.f;
   int from = 0, q_first = 0, q_of[NT][2];  // the first row's query, and those of rows 2c, 2c + 1
   bool fresh = true, ok = true, first = true;
-  const int rows = a.g * a.s_q;
+  if (left > 0) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) scale_q<T, D>(a, raw[n], q[n], factor[n]);
+  }
+  bool q_ready = true;
   int slot = 0;
   uint32_t phase = 0;
   auto next_slot = [&]() {
@@ -625,8 +665,11 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   while (left > 0) {
     const int r0 = cur.grp * kRows;
     if (fresh) {
+      if (!q_ready) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) load_q<T, D>(a, cur.b, cur.kvh, r0 + 8 * n, rows, q[n], factor[n]);
+        for (int n = 0; n < NT; ++n) load_q<T, D>(a, cur.b, cur.kvh, r0 + 8 * n, rows, q[n], factor[n]);
+      }
+      q_ready = false;
       q_first = r0 / a.g;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -886,56 +929,47 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (!ok) drain(full, kSlots, slot, phase, 2 * left - tiles);
   __syncthreads();
 
-  // Pieces in order of the list: warp 0's first and last, warp 1's, ...
+  // The CTA's pieces in order of the list (warp 0's first and last, warp 1's,
+  // ...): sh.list_of; runs of one id are joined.
+  static_assert(2 * kWarps <= 32, "one lane per piece");
+  if (warp == 0) {
+    const int id = lane < 2 * kWarps ? sh.id[lane] : -1;
+    const unsigned there = __ballot_sync(0xffffffffu, id >= 0), before = there & ((1u << lane) - 1u);
+    const int id_before = __shfl_sync(0xffffffffu, id, before ? 31 - __clz(before) : 0);
+    const bool begins = id >= 0 && (!before || id_before != id);
+    const unsigned runs = __ballot_sync(0xffffffffu, begins);
+    if (id >= 0) sh.list_of[__popc(before)] = lane;
+    if (begins) sh.run[__popc(runs & ((1u << lane) - 1u))] = __popc(before);
+    if (lane == 0) {
+      sh.n_runs = __popc(runs);
+      sh.run[__popc(runs)] = __popc(there);
+    }
+  }
   Partial<D, NT>* mine = reinterpret_cast<Partial<D, NT>*>(a.ws) + (int64_t)blockIdx.x * 2;
   if (tid < 2) mine[tid].id = -1;
   __syncthreads();
   if (sh.abort) return;
-  for (int x = 0; x < 2 * kWarps;) {
-    const int id = sh.id[x];
-    if (id < 0) {
-      ++x;
-      continue;
-    }
-    int e = x, n = 0, last = x;  // the pieces x .. last of this id; others between them are empty
-    for (; e < 2 * kWarps && (sh.id[e] == id || sh.id[e] < 0); ++e) {
-      if (sh.id[e] == id) {
-        if (tid == 0) sh.list_of[n] = e;
-        ++n;
-        last = e;
-      }
-    }
-    const bool begins = sh.from[x] == 0, ends = sh.to[last] == sh.nu[last];
+  for (int x = tid; x < sh.n_runs * (kRows * D / 4); x += C::kThreads) {
+    const int run = x / (kRows * D / 4), e = x % (kRows * D / 4) * 4;
+    const int p0 = sh.run[run], n = sh.run[run + 1] - p0;
+    const int head = sh.list_of[p0], last = sh.list_of[p0 + n - 1], id = sh.id[head];
+    const bool begins = sh.from[head] == 0, ends = sh.to[last] == sh.nu[last];
     Partial<D, NT>* part = begins && ends ? nullptr : mine + (begins ? 1 : 0);
-    __syncthreads();
-    // the joined pieces' maxima and sums stand one after another from here on
-    float keep_ml[2];
-    for (int k = tid, i = 0; k < n * 2 * kRows; k += C::kThreads, ++i)
-      if (i < 2) keep_ml[i] = sh.ml[sh.list_of[k / (2 * kRows)]][k % (2 * kRows)];
-    __syncthreads();
-    for (int k = tid, i = 0; k < n * 2 * kRows; k += C::kThreads, ++i)
-      if (i < 2) sh.ml[x + k / (2 * kRows)][k % (2 * kRows)] = keep_ml[i];
-    __syncthreads();
-    join<T, D, NT, C::kThreads>(a, n, id, sh.ml + x,
-                                [&](int i) -> const float* {
-                                  const int p = sh.list_of[i];
-                                  return sh.in_ring[p] ? reinterpret_cast<const float*>(smem + (p >> 1) * kSlots * kTile)
-                                                       : first_o(p >> 1);
-                                },
-                                part);
-    if (part && tid == 0) {
+    join<T, D, NT>(a, e, n, id, [&](int i) -> const float* { return sh.ml[sh.list_of[p0 + i]]; },
+                   [&](int i) -> const float* {
+                     const int p = sh.list_of[p0 + i];
+                     return sh.in_ring[p] ? reinterpret_cast<const float*>(smem + (p >> 1) * kSlots * kTile)
+                                          : first_o(p >> 1);
+                   },
+                   part);
+    if (part && e == 0) {
       part->id = id;
-      part->begins = begins;
-      part->ends = ends;
       part->last = 0;
       if (!ends) {
-        const long long here = piece_begin(total, first_part + (last >> 1) + 1, parts);  // the list position behind it
-        const long long end = here + (sh.nu[last] - sh.to[last]);
-        part->last = piece_of(total, end - 1, parts) / kWarps;
+        const long long here = split.begin(first_part + (last >> 1) + 1);  // the list position behind it
+        part->last = split.holder(here + (sh.nu[last] - sh.to[last]) - 1) / kWarps;
       }
     }
-    __syncthreads();
-    x = e;
   }
 }
 
@@ -965,10 +999,10 @@ __global__ void __launch_bounds__(kJoinThreads) gqa_join_kernel(const GqaArgs a)
     if (row == 0) there[i] = is;
   }
   __syncthreads();
-  join<T, D, NT, kJoinThreads>(a, n, id, ml,
-                               // one that is not there has no values: any of this id do, its factor is 0
-                               [&](int i) -> const float* { return there[i] ? piece(i)->o : p->o; },
-                               (Partial<D, NT>*)nullptr);
+  for (int e = threadIdx.x * 4; e < kRows * D; e += kJoinThreads * 4)
+    join<T, D, NT>(a, e, n, id, [&](int i) -> const float* { return ml[i]; },
+                   // one that is not there has no values: any of this id do, its factor is 0
+                   [&](int i) -> const float* { return there[i] ? piece(i)->o : p->o; }, (Partial<D, NT>*)nullptr);
 }
 
 // ------------------------------------------------------------------ weights
@@ -1030,11 +1064,9 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
   }
   if (tid == 0) sh.abort = 0;
   const int rows = a.g * a.s_q;
-  const long long parts = gridDim.x;
-  find_places<kWarps, kUnit>(a, a.h_kv, 1, sh.list,
-                      [&](int, long long total) { return piece_begin(total, blockIdx.x, parts); });
-  const long long total = sh.list.total;
-  const long long mine = piece_begin(total, blockIdx.x + 1, parts) - piece_begin(total, blockIdx.x, parts);
+  find_places<kWarps, kUnit>(a, a.h_kv, blockIdx.x, 1, gridDim.x, sh.list);
+  const Split split(sh.list.total, gridDim.x);
+  const long long mine = split.each + ((int)blockIdx.x < split.more ? 1 : 0);
 
   struct Cursor {
     int b, kvh, u, nu, len, end;
@@ -1089,10 +1121,12 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
       for (int i = 0; i < kRuns; ++i) {
         const int from = (ld.u - pages.base) * kRuns + i;
         ids[i] = __shfl_sync(0xffffffffu, pages.id, from);
-        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, from);
         next.held |= (ids[i] >= 0 ? 1 : 0) << i;
       }
       if (lane == 0) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + to * kTile, &full[to]);
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)  // after the load: these may still be on their way
+        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, (ld.u - pages.base) * kRuns + i);
       if (--to_load > 0) skip(ld, kWarps);
     };
     load_next(slot);
