@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "dsv4b.h"
 #include "dsv4b_kernels.h"
@@ -53,10 +54,23 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
+// The larger of two 16-bit integers, in both halves.
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.s16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Two fp32 times r, at once (each an ordinary product).
+__device__ __forceinline__ float2 scaled(float2 f, float r) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(f.x), "+f"(f.y)
+      : "f"(r));
+  return f;
+}
 // Four e4m3 of a word times r, rounded again.
 __device__ __forceinline__ uint32_t rescale_word(uint32_t w, float r) {
-  const float2 a = from_e4m3x2(w & 0xFFFFu), b = from_e4m3x2(w >> 16);
-  return to_e4m3x2(a.x * r, a.y * r) | (to_e4m3x2(b.x * r, b.y * r) << 16);
+  const float2 a = scaled(from_e4m3x2(w & 0xFFFFu), r), b = scaled(from_e4m3x2(w >> 16), r);
+  return to_e4m3x2(a.x, a.y) | (to_e4m3x2(b.x, b.y) << 16);
 }
 
 // ------------------------------------------------------------------ append
@@ -70,7 +84,7 @@ struct AppendArgs {
   const int32_t* ctx;
   const int32_t* table;
   int64_t stride_table;
-  int table_width, b, h_kv, num_blocks, page, n;
+  int table_width, b, h_kv, num_blocks, page, page_shift, n;
 };
 
 // Index of the sequence that owns work item w, by a whole block: item bases
@@ -109,12 +123,12 @@ __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
   __shared__ float s_red[8];
   auto cu = [&](int i) { return min(max(__ldg(a.cu + i), 0), a.n); };
   const int w = blockIdx.x;
-  const int seq = owner_of(w, a.b, [&](int i) { return cu(i) / a.page + 2 * i; });
+  const int seq = owner_of(w, a.b, [&](int i) { return (cu(i) >> a.page_shift) + 2 * i; });
   const int t0 = cu(seq), n_i = max(0, cu(seq + 1) - t0);
   const int ctx = max(__ldg(a.ctx + seq), 0);
   const int start = ctx - n_i;  // position of the first new token (< 0: the tokens before 0 are skipped)
-  const int item = w - (t0 / a.page + 2 * seq);  // < 0: offsets that do not ascend
-  const int pi = max(start, 0) / a.page + item;
+  const int item = w - ((t0 >> a.page_shift) + 2 * seq);  // < 0: offsets that do not ascend
+  const int pi = (max(start, 0) >> a.page_shift) + item;
   const int64_t pos0 = (int64_t)pi * a.page;
   if (n_i == 0 || item < 0 || pos0 >= ctx || pi >= a.table_width) return;
   const int blk = __ldg(a.table + (int64_t)seq * a.stride_table + pi);
@@ -138,7 +152,6 @@ __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
   const float s_old = old && live ? *scale : 0.f;
 
   uint4 x[kVec];
-  float amax = 0.f;
   auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -146,19 +159,35 @@ __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
       x[i] = r < rows ? __ldg(src + r * step) : make_uint4(0, 0, 0, 0);
     }
   };
+  // The largest magnitude: of the values' bits without signs, whose order is
+  // the values', two at a time.  Infinities and NaN, which do not count, are
+  // left out by a second look where there are any.
+  constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+  uint32_t top = 0;
   for (int base = 0; base < rows; base += kRowsHeld) {
     load(base);
+    uint32_t t = 0;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = to_f32x2<T>(q[j]);
-        const float u = fabsf(f.x), v = fabsf(f.y);
-        amax = fmaxf(amax, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+      for (int j = 0; j < 4; ++j) t = max_halves(t, q[j] & 0x7FFF7FFFu);
+    }
+    if (max(t & 0xFFFFu, t >> 16) >= kInf) {
+      t = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = q[j] & 0x7FFFu, hi = (q[j] >> 16) & 0x7FFFu;
+          t = max(t, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+        }
       }
     }
+    top = max(top, max(t & 0xFFFFu, t >> 16));
   }
+  float amax = to_f32x2<T>(top).x;
 #pragma unroll
   for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if constexpr (TEAM > 1) {
@@ -201,8 +230,7 @@ __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
         for (int j = 0; j < 4; ++j) {
           float2 f = to_f32x2<T>(q[j]);
           if (exact) {
-            f.x *= inv;
-            f.y *= inv;
+            f = scaled(f, inv);
           } else {
             f.x /= s;
             f.y /= s;
@@ -260,102 +288,140 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return bits ^ ((bits >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-constexpr int kSelThreads = 512;
-constexpr int kSelPer = 4;         // positions per thread and step of the last pass
-constexpr int kBins = 256;
-constexpr int kHists = 8;          // copies of the histogram, against conflicts on equal weights
+constexpr int kSelThreads = 1024;
+constexpr int kChunk = 4 * kSelThreads;  // positions of a step, four to a thread
+constexpr int kHeld = 8;                 // steps whose keys a thread keeps: 32,768 positions
+constexpr int kBins = 2048;              // digits of 11, 11 and 10 bits
+constexpr int kHists = 4;                // copies of the histogram, against conflicts on near weights
 
-// One CTA per (sequence, KV head): the weight of the n-th heaviest position
-// by four passes of an 8-bit radix histogram, then one ordered pass that
-// writes the kept positions (a running count of those above it and of those
-// equal to it; of the latter only the first ones are kept).  Reads the
-// weights five times, from L2 after the first; the sizes of a cache (tens of
-// thousands of positions) keep a CTA at some microseconds.
+// One CTA per (sequence, KV head): the key of the last position that is kept
+// by three passes of a radix histogram from the top digit down, then one
+// ordered pass that writes the kept positions (a running count of those
+// above that key and of those equal to it; of the latter only the first ones
+// are kept).  The weights are read once into registers (32 a thread; longer
+// sequences are read again, from L2, in every pass).  The histogram's
+// conflicts bound it: a digit of sign, exponent and two bits spreads weights
+// of one magnitude over some bins, and exact zeros (positions that nothing
+// looked at) are counted by vote.
 __global__ void __launch_bounds__(kSelThreads) gqa_evict_select_kernel(const EvictArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   __shared__ uint32_t hist[kHists][kBins];
   __shared__ uint32_t s_scan[kSelThreads / 32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
-  const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+  const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = evict_len(a, seq);
   const int new_len = min(len, a.budget);
   const float* w = a.weights + (int64_t)seq * a.stride_w_b + (int64_t)head * a.stride_w_h;
   float* nw = a.new_weights + (int64_t)seq * a.stride_nw_b + (int64_t)head * a.stride_nw_h;
   int32_t* kept = a.kept + ((int64_t)seq * a.h_kv + head) * a.budget;
   if (head == 0 && tid == 0) a.new_lens[seq] = new_len;
-  for (int i = new_len + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
-  for (int i = new_len + tid; i < a.new_width; i += kSelThreads) nw[i] = 0.f;
   const int recent = len > a.budget ? a.recent : len;  // positions that are kept without a look
   const int older = len - recent;
+  const int pick = new_len - recent;  // of the older ones
+  // four positions from i on, as keys; those that are not older ones are 0,
+  // which no weight's key is
+  const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  auto keys_at = [&](int i, uint32_t (&k)[4]) {
+    float x[4];
+    if (vec && i + 4 <= older) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(w + i));
+      x[0] = v.x;
+      x[1] = v.y;
+      x[2] = v.z;
+      x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = i + j < older ? __ldg(w + i + j) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j] = i + j < older ? weight_key(x[j]) : 0u;
+  };
+  const bool held = older <= kHeld * kChunk;
+  uint32_t mine[kHeld][4];
+  if (pick > 0 && held) {
+#pragma unroll
+    for (int s = 0; s < kHeld; ++s) keys_at(s * kChunk + 4 * tid, mine[s]);
+  }
+  for (int i = new_len + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
+  for (int i = new_len + tid; i < a.new_width; i += kSelThreads) nw[i] = 0.f;
   for (int i = tid; i < recent; i += kSelThreads) {
     kept[new_len - recent + i] = older + i;
     nw[new_len - recent + i] = __ldg(w + older + i);
   }
-  const int pick = new_len - recent;  // of the older ones
   if (pick == 0) return;
+  // f(step, keys) over all steps
+  auto each = [&](auto f) {
+    if (held) {
+#pragma unroll
+      for (int s = 0; s < kHeld; ++s)
+        if (s * kChunk < older) f(s, mine[s]);
+    } else {
+      for (int s = 0; s * kChunk < older; ++s) {
+        uint32_t k[4];
+        keys_at(s * kChunk + 4 * tid, k);
+        f(s, k);
+      }
+    }
+  };
 
+  constexpr uint32_t kZero = 0x80000000u;  // weight_key(0)
   uint32_t prefix = 0;
   int need = pick;  // the need-th largest key is looked for among those that share `prefix`
-  for (int shift = 24; shift >= 0; shift -= 8) {
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     for (int i = tid; i < kHists * kBins; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    uint32_t* h = hist[(tid >> 2) % kHists];
-    for (int i = tid; i < older; i += kSelThreads) {
-      const uint32_t key = weight_key(__ldg(w + i));
-      if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&h[(key >> shift) & (kBins - 1)], 1u);
-    }
+    uint32_t* h = hist[(tid >> 1) % kHists];
+    uint32_t zeros = 0;
+    each([&](int, const uint32_t(&k)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = k[j] != 0 && (pass == 0 || (k[j] >> (shift + bits)) == prefix);
+        if (in && k[j] == kZero) ++zeros;
+        if (in && k[j] != kZero) atomicAdd(&h[(k[j] >> shift) & ((1u << bits) - 1)], 1u);
+      }
+    });
+    zeros = __reduce_add_sync(0xffffffffu, zeros);
+    if (lane == 0 && zeros) atomicAdd(&hist[0][(kZero >> shift) & ((1u << bits) - 1)], zeros);
     __syncthreads();
-    if (tid < 32) {
-      // lane l takes the 8 bins below 256 - 8 l, the largest keys first
-      uint32_t c[8], sum = 0;
+    // thread t has the two bins below 2048 - 2 t, the largest keys first
+    uint32_t c[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        c[j] = 0;
-        for (int k = 0; k < kHists; ++k) c[j] += hist[k][kBins - 1 - (tid * 8 + j)];
-        sum += c[j];
-      }
-      uint32_t before = sum;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
-        if (tid >= o) before += v;
-      }
-      before -= sum;
-      if ((int)before < need && need <= (int)(before + sum)) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if ((int)before < need && need <= (int)(before + c[j])) {
-            s_prefix = (prefix << 8) | (uint32_t)(kBins - 1 - (tid * 8 + j));
-            s_need = need - (int)before;
-          }
-          before += c[j];
-        }
+      for (int k = 0; k < kHists; ++k) c[j] += hist[k][kBins - 1 - (2 * tid + j)];
+    uint32_t incl = c[0] + c[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    const uint32_t others = __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0u);
+    uint32_t before = others + incl - c[0] - c[1];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if ((int)before < need && need <= (int)(before + c[j])) {
+        s_prefix = (prefix << bits) | (uint32_t)(kBins - 1 - (2 * tid + j));
+        s_need = need - (int)before;
       }
+      before += c[j];
     }
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
   }
-  // prefix is the threshold; `need` of the positions equal to it are kept
+  // prefix is the last kept key; `need` of the positions equal to it are kept
   uint32_t above = 0, equal = 0;  // counts before this step
-  const int lane = tid & 31, warp = tid >> 5;
-  for (int base = 0; base < older; base += kSelThreads * kSelPer) {
-    float x[kSelPer];
-    uint32_t flags = 0, mine = 0;
+  each([&](int s, const uint32_t(&k)[4]) {
+    uint32_t n = 0;  // (above << 16) | equal: a step has 4,096 positions
 #pragma unroll
-    for (int j = 0; j < kSelPer; ++j) {
-      const int i = base + tid * kSelPer + j;
-      x[j] = i < older ? __ldg(w + i) : 0.f;
-      const uint32_t key = weight_key(x[j]);
-      if (i < older && key > prefix) {
-        flags |= 1u << j;
-        mine += 1u << 16;
-      } else if (i < older && key == prefix) {
-        flags |= 16u << j;
-        mine += 1u;
-      }
-    }
-    uint32_t incl = mine;  // (above << 16) | equal: a step has 2048 positions
+    for (int j = 0; j < 4; ++j) n += k[j] > prefix ? 1u << 16 : k[j] == prefix ? 1u : 0u;
+    uint32_t incl = n;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
@@ -363,28 +429,25 @@ __global__ void __launch_bounds__(kSelThreads) gqa_evict_select_kernel(const Evi
     __syncthreads();
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    uint32_t pre = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kSelThreads / 32; ++i) {
-      if (i < warp) pre += s_scan[i];
-      total += s_scan[i];
-    }
-    pre += incl - mine;
+    const uint32_t sums = s_scan[lane];
+    const uint32_t pre = __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0u) + incl - n;
+    const uint32_t total = __reduce_add_sync(0xffffffffu, sums);
     uint32_t g = above + (pre >> 16), e = equal + (pre & 0xFFFFu);
 #pragma unroll
-    for (int j = 0; j < kSelPer; ++j) {
-      const bool is_above = (flags >> j) & 1u, is_equal = (flags >> (4 + j)) & 1u;
+    for (int j = 0; j < 4; ++j) {
+      const bool is_above = k[j] > prefix, is_equal = k[j] == prefix;
       if (is_above || (is_equal && e < (uint32_t)need)) {
         const uint32_t at = g + min(e, (uint32_t)need);
-        kept[at] = base + tid * kSelPer + j;
-        nw[at] = x[j];
+        const int pos = s * kChunk + 4 * tid + j;
+        kept[at] = pos;
+        nw[at] = __ldg(w + pos);  // the weight itself: a key does not tell -0 from 0, nor NaN from NaN
       }
       g += is_above;
       e += is_equal;
     }
     above += total >> 16;
     equal += total & 0xFFFFu;
-  }
+  });
 }
 
 // One CTA per (new block, KV head, sequence): the sources of its rows, the
@@ -394,7 +457,7 @@ constexpr int kGatherThreads = 128;
 template <int D>
 __global__ void __launch_bounds__(kGatherThreads) gqa_evict_gather_kernel(const EvictArgs a) {
   constexpr int kVec = D / 16;
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 8;  // K and V of 64 rows of 128: all loads in flight at once
   extern __shared__ uint8_t smem_raw[];
   int64_t* s_off = reinterpret_cast<int64_t*>(smem_raw);        // [2][page] source bytes, -1: nothing there
   float* s_scale = reinterpret_cast<float*>(s_off + 2 * a.page);  // [2][page]
@@ -437,34 +500,34 @@ __global__ void __launch_bounds__(kGatherThreads) gqa_evict_gather_kernel(const 
     for (int i = 0; i < kGatherThreads / 32; ++i) top[kv] = fmaxf(top[kv], s_red[kv][i]);
     if (tid == 0) a.scale[kv][(int64_t)dest * a.h_kv + head] = top[kv];
   }
+  // K's rows, then V's
+  for (int e0 = tid; e0 < 2 * rows * kVec; e0 += kGatherThreads * kUnroll) {
+    uint4 q[kUnroll];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint8_t* to = a.cache[kv] + (int64_t)dest * a.stride_block[kv] + (int64_t)head * a.stride_head[kv];
-    for (int e0 = tid; e0 < rows * kVec; e0 += kGatherThreads * kUnroll) {
-      uint4 q[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int e = e0 + u * kGatherThreads;
-        q[u] = make_uint4(0, 0, 0, 0);
-        if (e < rows * kVec) {
-          const int64_t off = s_off[kv * a.page + e / kVec];
-          if (off >= 0) q[u] = *(reinterpret_cast<const uint4*>(a.cache[kv] + off) + e % kVec);
-        }
+    for (int u = 0; u < kUnroll; ++u) {
+      const int e = e0 + u * kGatherThreads;
+      q[u] = make_uint4(0, 0, 0, 0);
+      if (e < 2 * rows * kVec) {
+        const int kv = e >= rows * kVec, r = e / kVec - kv * rows;
+        const int64_t off = s_off[kv * a.page + r];
+        if (off >= 0) q[u] = *(reinterpret_cast<const uint4*>(a.cache[kv] + off) + e % kVec);
       }
+    }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int e = e0 + u * kGatherThreads;
-        if (e < rows * kVec) {
-          const float s = s_scale[kv * a.page + e / kVec];
-          if (s != top[kv]) {
-            const float ratio = s / top[kv];  // 0 <= s < top
-            q[u].x = rescale_word(q[u].x, ratio);
-            q[u].y = rescale_word(q[u].y, ratio);
-            q[u].z = rescale_word(q[u].z, ratio);
-            q[u].w = rescale_word(q[u].w, ratio);
-          }
-          *(reinterpret_cast<uint4*>(to + (int64_t)(e / kVec) * a.stride_row[kv]) + e % kVec) = q[u];
+    for (int u = 0; u < kUnroll; ++u) {
+      const int e = e0 + u * kGatherThreads;
+      if (e < 2 * rows * kVec) {
+        const int kv = e >= rows * kVec, r = e / kVec - kv * rows;
+        const float s = s_scale[kv * a.page + r];
+        if (s != top[kv]) {
+          const float ratio = s / top[kv];  // 0 <= s < top
+          q[u].x = rescale_word(q[u].x, ratio);
+          q[u].y = rescale_word(q[u].y, ratio);
+          q[u].z = rescale_word(q[u].z, ratio);
+          q[u].w = rescale_word(q[u].w, ratio);
         }
+        uint8_t* to = a.cache[kv] + (int64_t)dest * a.stride_block[kv] + (int64_t)head * a.stride_head[kv];
+        *(reinterpret_cast<uint4*>(to + (int64_t)r * a.stride_row[kv]) + e % kVec) = q[u];
       }
     }
   }
@@ -501,6 +564,7 @@ cudaError_t launch_gqa_append(const dsv4b_gqa_cache& c, int dtype, const void* k
   a.h_kv = c.h_kv;
   a.num_blocks = c.num_blocks;
   a.page = c.page_block_size;
+  while ((1 << a.page_shift) < a.page) ++a.page_shift;
   a.n = n;
   if (dtype == DSV4B_BF16)
     return c.d == 128 ? launch_append<__nv_bfloat16, 128>(a, stream) : launch_append<__nv_bfloat16, 64>(a, stream);

@@ -1006,13 +1006,14 @@ __global__ void __launch_bounds__(kJoinThreads) gqa_join_kernel(const GqaArgs a)
 }
 
 // ------------------------------------------------------------------ weights
-// One CTA takes a contiguous piece of the units of all (sequence, KV head)
-// pairs, its warps every kWarps-th unit of it.  K's fragments are widened
-// once per unit and multiplied with the n-tiles of 8 rows one after another;
-// a thread adds p of its rows, then the four c are joined by a halving
-// exchange that leaves one position per lane.  One n-tile's q stays in the
-// registers of every warp; more stand in shared memory, up to kHeldTiles of
-// them, and further ones take further passes over the piece.
+// Up to 8 rows (one n-tile): every warp of the grid takes a contiguous piece
+// of the units of all (sequence, KV head) pairs and keeps the rows' q in
+// registers.  More: every CTA takes a piece, in it a warp a contiguous part
+// of each pair, and q stands in shared memory, up to kHeldTiles n-tiles of it
+// (further ones take further passes over the piece); K's fragments are
+// widened once per unit and multiplied with two n-tiles at a time.  A thread
+// adds p of its rows, then the four c are joined by a halving exchange that
+// leaves one position per lane.
 constexpr int kHeldTiles = 32;
 template <int D, bool ONE>
 struct Wts {
@@ -1064,85 +1065,125 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
   }
   if (tid == 0) sh.abort = 0;
   const int rows = a.g * a.s_q;
-  find_places<kWarps, kUnit>(a, a.h_kv, blockIdx.x, 1, gridDim.x, sh.list);
-  const Split split(sh.list.total, gridDim.x);
-  const long long mine = split.each + ((int)blockIdx.x < split.more ? 1 : 0);
+  // the piece of the list: the warp's own, or the CTA's
+  const int parts = ONE ? gridDim.x * kWarps : gridDim.x, part = ONE ? blockIdx.x * kWarps + warp : blockIdx.x;
+  find_places<kWarps, kUnit>(a, a.h_kv, ONE ? blockIdx.x * kWarps : blockIdx.x, ONE ? kWarps : 1, parts, sh.list);
+  const Split split(sh.list.total, parts);
 
+  // A walk over the piece's pairs, and in each over this warp's units.
   struct Cursor {
-    int b, kvh, u, nu, len, end;
+    int b, kvh, nu, len, end;
+    int from;             // the piece's first unit of this pair
+    long long left;       // the piece's units from there on
+    int u, to;            // this warp's next unit of the pair, and the end of its units
+    __device__ __forceinline__ bool in_pair() const { return u < to; }
   };
-  auto enter = [&](Cursor& x) {
-    if (x.b >= a.b) return;
+  auto enter = [&](Cursor& x) {  // b, kvh, from and left are set
     x.len = held_len(a, x.b);
     x.end = __ldg(a.ctx + x.b) - a.s_q + 1;
     x.nu = units_of<kUnit>(x.len);
+    const int n = (int)min(x.left, (long long)(x.nu - x.from));
+    x.u = ONE ? x.from : x.from + (int)((long long)n * warp / kWarps);
+    x.to = ONE ? x.from + n : x.from + (int)((long long)n * (warp + 1) / kWarps);
   };
-  auto skip = [&](Cursor& x, int n) {  // n units on
-    x.u += n;
-    while (x.u >= x.nu && x.b < a.b) {
-      x.u -= x.nu;
-      if (++x.kvh == a.h_kv) {
-        x.kvh = 0;
-        ++x.b;
-        enter(x);
-      }
+  auto next_pair = [&](Cursor& x) {  // false: the piece ends
+    x.left -= min(x.left, (long long)(x.nu - x.from));
+    if (x.left == 0) return false;
+    x.from = 0;
+    if (++x.kvh == a.h_kv) {
+      x.kvh = 0;
+      ++x.b;
     }
+    enter(x);
+    return true;
   };
-  Cursor start = {};
-  if (mine > 0) {
-    start.b = sh.list.b[0];
-    enter(start);
-    const long long u = sh.list.u[0];
-    start.kvh = (int)(u / start.nu);
-    start.u = (int)(u - (long long)start.kvh * start.nu);
+  Cursor first = {};
+  first.left = split.each + (part < split.more ? 1 : 0);
+  if (first.left > 0) {
+    const int i = ONE ? warp : 0;
+    first.b = sh.list.b[i];
+    first.nu = units_of<kUnit>(held_len(a, first.b));
+    const long long u = sh.list.u[i];
+    first.kvh = u < (1ll << 31) ? (int)((unsigned)u / (unsigned)first.nu) : (int)(u / first.nu);
+    first.from = (int)(u - (long long)first.kvh * first.nu);
+    enter(first);
   }
-  const int units = mine > warp ? (int)((mine - warp + kWarps - 1) / kWarps) : 0;  // this warp's
-  Cursor first = start;
-  if (units > 0) skip(first, warp);
 
+  constexpr int kN = ONE ? 1 : 2;  // n-tiles at a time
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
-  uint32_t q[kSteps][2];
-  float factor[2], lse2[2];
+  uint32_t q[kN][kSteps][2];
+  float factor[kN][2], lse2[kN][2];
   Info<kUnit> now, next;  // of the unit at the products' cursor, and of the one behind it
-  const int tiles = (rows + 7) / 8;
+  const int tiles = (rows + 8 * kN - 1) / (8 * kN) * kN;
   for (int n0 = 0; n0 < tiles; n0 += kHeldTiles) {
     const int nt = min(kHeldTiles, tiles - n0), q_first = n0 * 8 / a.g;
     Cursor ld = first, cur = first;
-    int to_load = ok ? units : 0, left = to_load;
+    bool more = first.left > 0 && ok;
+    int loaded = 0;  // and not yet used
     Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
     auto load_next = [&](int to) {
-      if (to_load == 0) return;
+      while (more && !ld.in_pair()) more = next_pair(ld);
+      if (!more) return;
       fetch_pages<kUnit, false>(a, pages, ld.b, ld.kvh, ld.u, ld.len);
       int ids[kRuns];
       next.held = 0;
 #pragma unroll
       for (int i = 0; i < kRuns; ++i) {
-        const int from = (ld.u - pages.base) * kRuns + i;
-        ids[i] = __shfl_sync(0xffffffffu, pages.id, from);
+        ids[i] = __shfl_sync(0xffffffffu, pages.id, (ld.u - pages.base) * kRuns + i);
         next.held |= (ids[i] >= 0 ? 1 : 0) << i;
       }
       if (lane == 0) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + to * kTile, &full[to]);
 #pragma unroll
       for (int i = 0; i < kRuns; ++i)  // after the load: these may still be on their way
         next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, (ld.u - pages.base) * kRuns + i);
-      if (--to_load > 0) skip(ld, kWarps);
+      ++ld.u;
+      ++loaded;
     };
+    RawQ<D> raw;
+    if constexpr (ONE) {  // the first rows of q, ahead of the tiles that would be in their way
+      if (first.left > 0) fetch_q<T, D>(a, cur.b, cur.kvh, 0, rows, raw);
+    }
     load_next(slot);
     now = next;
     load_next((slot + 1) % kSlots);
-    // the pairs of the piece, one after another
-    Cursor pair = start;
-    long long to_go = mine;
-    while (to_go > 0) {
-      const long long in_pair = min(to_go, (long long)(pair.nu - pair.u));
-      if constexpr (!ONE) {
+    if (!a.accumulate && n0 == 0) {  // zeros behind each context, while the first tiles come
+      constexpr int kSpan = 512;  // of a row, one warp's
+      const int spans = (a.width + kSpan - 1) / kSpan;
+      const long long items = (long long)a.b * a.h_kv * spans;
+      for (long long x = blockIdx.x * kWarps + warp; x < items; x += gridDim.x * kWarps) {
+        const int row = items < (1ll << 31) ? (int)((unsigned)x / (unsigned)spans) : (int)(x / spans);
+        const int from = (int)(x - (long long)row * spans) * kSpan, to = min(from + kSpan, a.width);
+        const int len = held_len(a, row / a.h_kv);
+        if (len >= to) continue;
+        float* w = a.weights + (int64_t)(row / a.h_kv) * a.stride_w_b + (int64_t)(row % a.h_kv) * a.stride_w_h;
+        if (len <= from && to - from == kSpan && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+#pragma unroll
+          for (int t = 0; t < kSpan; t += 128) *reinterpret_cast<float4*>(w + from + t + 4 * lane) = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          for (int t = max(from, len) + lane; t < to; t += 32) w[t] = 0.f;
+        }
+      }
+    }
+    bool go = first.left > 0;
+    bool q_ready = false;
+    if constexpr (ONE) {
+      if (go) scale_q<T, D>(a, raw, q[0], factor[0]);
+      q_ready = true;
+    }
+    while (go) {  // the pairs of the piece, one after another
+      if constexpr (ONE) {
+        if (!q_ready) load_q<T, D>(a, cur.b, cur.kvh, 0, rows, q[0], factor[0]);
+        q_ready = false;
+        lse2[0][0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
+        lse2[0][1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
+      } else {
         __syncthreads();  // the last pair's fragments are read
         for (int n = warp; n < nt; n += kWarps) {
           uint32_t f[kSteps][2];
           float fac[2];
-          load_q<T, D>(a, pair.b, pair.kvh, (n0 + n) * 8, rows, f, fac);
+          load_q<T, D>(a, cur.b, cur.kvh, (n0 + n) * 8, rows, f, fac);
 #pragma unroll
           for (int s = 0; s < kSteps; s += 2)
             q_held[(n * (kSteps / 2) + s / 2) * 32 + lane] = make_uint4(f[s][0], f[s][1], f[s + 1][0], f[s + 1][1]);
@@ -1150,20 +1191,11 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
             sh.factor[n][2 * c] = fac[0];
             sh.factor[n][2 * c + 1] = fac[1];
           }
-          if (lane < 8) sh.lse[n][lane] = lse_log2(a, pair.b, pair.kvh, (n0 + n) * 8 + lane, rows);
+          if (lane < 8) sh.lse[n][lane] = lse_log2(a, cur.b, cur.kvh, (n0 + n) * 8 + lane, rows);
         }
         __syncthreads();
       }
-      bool fresh = true;
-      while (ok && left > 0 && cur.b == pair.b && cur.kvh == pair.kvh) {
-        if constexpr (ONE) {
-          if (fresh) {
-            load_q<T, D>(a, cur.b, cur.kvh, 0, rows, q, factor);
-            lse2[0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
-            lse2[1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
-            fresh = false;
-          }
-        }
+      for (; ok && cur.in_pair(); ++cur.u) {
         const int t0 = cur.u * kUnit;
         const bool edge = t0 + kUnit > min(cur.len, cur.end + q_first) || now.held != (1 << kRuns) - 1;
         // the positions whose weights this lane will hold
@@ -1177,17 +1209,18 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
         }
         if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
         uint32_t f[ONE ? 1 : kRuns][ONE ? 1 : D / 64][4][4];
-        float s[kRuns][4];
+        float s[kN][kRuns][4];
         if constexpr (ONE) {
 #pragma unroll
           for (int mt = 0; mt < kRuns; ++mt) {
-            s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+            s[0][mt][0] = s[0][mt][1] = s[0][mt][2] = s[0][mt][3] = 0.f;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h) {
               k_frags<D>(ring + slot * kTile, mt, h, f[0][0]);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mma_f16(s[mt], f[0][0][k][0], f[0][0][k][1], f[0][0][k][2], f[0][0][k][3], q[4 * h + k][0], q[4 * h + k][1]);
+                mma_f16(s[0][mt], f[0][0][k][0], f[0][0][k][1], f[0][0][k][2], f[0][0][k][3], q[0][4 * h + k][0],
+                        q[0][4 * h + k][1]);
             }
           }
         } else {
@@ -1197,6 +1230,7 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
             for (int h = 0; h < D / 64; ++h) k_frags<D>(ring + slot * kTile, mt, h, f[mt][h]);
         }
         __syncwarp();
+        --loaded;
         const Info<kUnit> here = now;
         now = next;
         load_next(slot);
@@ -1207,47 +1241,55 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
         float sum[2 * kRuns];  // positions 8 i + perm(g)
 #pragma unroll
         for (int i = 0; i < 2 * kRuns; ++i) sum[i] = 0.f;
-        for (int n = 0; n < nt; ++n) {
+        for (int n = 0; n < nt; n += kN) {
           if constexpr (!ONE) {
 #pragma unroll
-            for (int k = 0; k < kSteps; k += 2) {
-              const uint4 x = q_held[(n * (kSteps / 2) + k / 2) * 32 + lane];
-              q[k][0] = x.x;
-              q[k][1] = x.y;
-              q[k + 1][0] = x.z;
-              q[k + 1][1] = x.w;
-            }
-            const float2 x = *reinterpret_cast<const float2*>(&sh.factor[n][2 * c]);
-            const float2 y = *reinterpret_cast<const float2*>(&sh.lse[n][2 * c]);
-            factor[0] = x.x;
-            factor[1] = x.y;
-            lse2[0] = y.x;
-            lse2[1] = y.y;
+            for (int x = 0; x < kN; ++x) {
 #pragma unroll
-            for (int mt = 0; mt < kRuns; ++mt) s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+              for (int k = 0; k < kSteps; k += 2) {
+                const uint4 v = q_held[((n + x) * (kSteps / 2) + k / 2) * 32 + lane];
+                q[x][k][0] = v.x;
+                q[x][k][1] = v.y;
+                q[x][k + 1][0] = v.z;
+                q[x][k + 1][1] = v.w;
+              }
+              const float2 v = *reinterpret_cast<const float2*>(&sh.factor[n + x][2 * c]);
+              const float2 y = *reinterpret_cast<const float2*>(&sh.lse[n + x][2 * c]);
+              factor[x][0] = v.x;
+              factor[x][1] = v.y;
+              lse2[x][0] = y.x;
+              lse2[x][1] = y.y;
+#pragma unroll
+              for (int mt = 0; mt < kRuns; ++mt) s[x][mt][0] = s[x][mt][1] = s[x][mt][2] = s[x][mt][3] = 0.f;
+            }
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int mt = 0; mt < kRuns; ++mt)
-                  mma_f16(s[mt], f[mt][h][k][0], f[mt][h][k][1], f[mt][h][k][2], f[mt][h][k][3], q[4 * h + k][0],
-                          q[4 * h + k][1]);
+                for (int x = 0; x < kN; ++x)
+#pragma unroll
+                  for (int mt = 0; mt < kRuns; ++mt)
+                    mma_f16(s[x][mt], f[mt][h][k][0], f[mt][h][k][1], f[mt][h][k][2], f[mt][h][k][3], q[x][4 * h + k][0],
+                            q[x][4 * h + k][1]);
           }
-          if (!edge) {
 #pragma unroll
-            for (int i = 0; i < 2 * kRuns; ++i)
-              sum[i] += fast_exp2(fmaf(s[i >> 1][2 * (i & 1)], factor[0] * here.ks[i >> 1], -lse2[0])) +
-                        fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + 1], factor[1] * here.ks[i >> 1], -lse2[1]));
-          } else {
+          for (int x = 0; x < kN; ++x) {
+            if (!edge) {
 #pragma unroll
-            for (int i = 0; i < 2 * kRuns; ++i) {
-              const bool there = (here.held >> (i >> 1)) & 1;
+              for (int i = 0; i < 2 * kRuns; ++i)
+                sum[i] += fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1)], factor[x][0] * here.ks[i >> 1], -lse2[x][0])) +
+                          fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1) + 1], factor[x][1] * here.ks[i >> 1], -lse2[x][1]));
+            } else {
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float p = fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + k], factor[k] * here.ks[i >> 1], -lse2[k]));
-                const int lim = cur.end + ((n0 + n) * 8 + 2 * c + k) / a.g;
-                sum[i] += there && t0 + 8 * i + Lay<D>::perm(g) < lim ? p : 0.f;
+                const int lim = cur.end + ((n0 + n + x) * 8 + 2 * c + k) / a.g;
+#pragma unroll
+                for (int i = 0; i < 2 * kRuns; ++i) {
+                  const bool there = (here.held >> (i >> 1)) & 1;
+                  const float p = fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1) + k], factor[x][k] * here.ks[i >> 1], -lse2[x][k]));
+                  sum[i] += there && t0 + 8 * i + Lay<D>::perm(g) < lim ? p : 0.f;
+                }
               }
             }
           }
@@ -1267,18 +1309,10 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
           const int t = t_mine + 32 * x;
           if (t < cur.len && t < a.width) w[32 * x] = before[x] + sum[4 * x];
         }
-        if (--left > 0) skip(cur, kWarps);
       }
-      to_go -= in_pair;
-      if (to_go > 0) skip(pair, (int)in_pair);
+      go = next_pair(cur);
     }
-    if (!ok && left > 0) drain(full, kSlots, slot, phase, left - to_load);
-  }
-  if (!a.accumulate) {  // zeros behind each context
-    for (int x = blockIdx.x; x < a.b * a.h_kv; x += gridDim.x) {
-      float* w = a.weights + (int64_t)(x / a.h_kv) * a.stride_w_b + (int64_t)(x % a.h_kv) * a.stride_w_h;
-      for (int t = held_len(a, x / a.h_kv) + tid; t < a.width; t += C::kThreads) w[t] = 0.f;
-    }
+    if (!ok) drain(full, kSlots, slot, phase, loaded);
   }
 }
 
