@@ -67,10 +67,32 @@ __device__ __forceinline__ float2 scaled(float2 f, float r) {
       : "f"(r));
   return f;
 }
-// Four e4m3 of a word times r, rounded again.
+// Sixteen e4m3 times r <= 1, rounded again.  A power of two from 2^-15 on
+// keeps e4m3's values (multiples of 2^-9 up to 448) exact in fp16, so the
+// product is rounded once there too; other factors go through fp32.
+__device__ __forceinline__ uint32_t rescale_word_half(uint32_t w, __half2 r) {
+  uint32_t lo, hi;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+  const __half2 a = __hmul2(*reinterpret_cast<__half2*>(&lo), r), b = __hmul2(*reinterpret_cast<__half2*>(&hi), r);
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f16x2 l, %1;\n\tcvt.rn.satfinite.e4m3x2.f16x2 h, %2;\n\tmov.b32 %0, {l, h};\n\t}"
+      : "=r"(d)
+      : "r"(*reinterpret_cast<const uint32_t*>(&a)), "r"(*reinterpret_cast<const uint32_t*>(&b)));
+  return d;
+}
 __device__ __forceinline__ uint32_t rescale_word(uint32_t w, float r) {
   const float2 a = scaled(from_e4m3x2(w & 0xFFFFu), r), b = scaled(from_e4m3x2(w >> 16), r);
   return to_e4m3x2(a.x, a.y) | (to_e4m3x2(b.x, b.y) << 16);
+}
+__device__ __forceinline__ uint4 rescale(uint4 q, float r) {
+  if (is_power_of_two(r) && r >= 3.0517578125e-5f) {
+    const __half2 h = __float2half2_rn(r);
+    return make_uint4(rescale_word_half(q.x, h), rescale_word_half(q.y, h), rescale_word_half(q.z, h),
+                      rescale_word_half(q.w, h));
+  }
+  return make_uint4(rescale_word(q.x, r), rescale_word(q.y, r), rescale_word(q.z, r), rescale_word(q.w, r));
 }
 
 // ------------------------------------------------------------------ append
@@ -101,13 +123,15 @@ __device__ __forceinline__ int owner_of(int w, int b, F f) {
   return owner;
 }
 
-// A task is one (sequence, block of the cache, head, k or v): its new rows
-// are read once into registers (kVec 16-byte vectors per thread), their
-// largest magnitude gives the scale, and the quantised rows are written.
-// TEAM warps share a task.  Bound by its 3 bytes per element; a task of one
-// token (a decode step) is one warp's, a page of a prompt is a whole team's
-// so that its loads are all in flight together.  A block of more rows than
-// a team holds is read twice (the second time from L2).
+// A task is one (sequence, block of the cache, head): its new rows of k and
+// v are read once into registers (kVec 16-byte vectors of each per thread),
+// their largest magnitudes give the two scales, and the quantised rows are
+// written.  TEAM warps share a task.  Bound by its 3 bytes per element; a
+// task of one token (a decode step) is one warp's, a block of a prompt is a
+// whole team's so that its loads are all in flight together, and k and v
+// share what finding the task costs (about 300 instructions, as many as
+// quantising eight vectors).  A block of more rows than a team holds is read
+// twice (the second time from L2).
 //
 // Which blocks a sequence touches is not known on the host.  Sequence i
 // with n_i new tokens touches at most n_i / P + 2 blocks, so the items
@@ -115,12 +139,13 @@ __device__ __forceinline__ int owner_of(int w, int b, F f) {
 // CTA finds its own without a scan.
 template <typename T, int D, int TEAM>
 __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
-  constexpr int kVec = 8;
+  constexpr int kVec = TEAM == 1 ? 2 : 8;
   constexpr int kLanes = TEAM * 32;
   constexpr int kVecPerRow = D / 8;                   // 16-byte vectors per row
   constexpr int kRowsPerPass = kLanes / kVecPerRow;   // rows that a team covers per vector
   constexpr int kRowsHeld = kRowsPerPass * kVec;
-  __shared__ float s_red[8];
+  constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+  __shared__ float s_red[2][8];
   auto cu = [&](int i) { return min(max(__ldg(a.cu + i), 0), a.n); };
   const int w = blockIdx.x;
   const int seq = owner_of(w, a.b, [&](int i) { return (cu(i) >> a.page_shift) + 2 * i; });
@@ -135,111 +160,142 @@ __global__ void __launch_bounds__(256) gqa_append_kernel(const AppendArgs a) {
   if (blk < 0 || blk >= a.num_blocks) return;
 
   const int team = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  const int task = blockIdx.y * (256 / kLanes) + team;
-  const bool live = task < 2 * a.h_kv;  // teams past the last task only take part in the barriers
-  const int kv = live ? task / a.h_kv : 0, head = live ? task % a.h_kv : 0;
+  const int head = blockIdx.y * (256 / kLanes) + team;
+  const bool live = head < a.h_kv;  // teams past the last head only take part in the barriers
   const int first = max(start, (int)pos0), last = min((int64_t)ctx, pos0 + a.page);
   const int rows = live ? last - first : 0;
   const int r0 = first - (int)pos0;  // row in the block of the first new token
-  const int old = start > pos0 ? start - (int)pos0 : 0;
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[kv]) +
-                                                    (int64_t)(t0 + first - start) * a.stride_t[kv] +
-                                                    (int64_t)head * a.stride_h[kv]) + lane % kVecPerRow;
-  const int64_t step = a.stride_t[kv] / 8;  // in 16-byte vectors
-  const int row = lane / kVecPerRow;
-  uint8_t* page = a.cache[kv] + (int64_t)blk * a.stride_block[kv] + (int64_t)head * a.stride_head[kv];
-  float* scale = a.scale[kv] + (int64_t)blk * a.h_kv + head;
-  const float s_old = old && live ? *scale : 0.f;
-
-  uint4 x[kVec];
-  auto load = [&](int base) {
+  const int old = start > pos0 ? r0 : 0;
+  const int row = lane / kVecPerRow, col = lane % kVecPerRow;
+  const int64_t token = t0 + first - start + row;
+  const uint4* src[2];
+  int64_t step[2];  // kRowsPerPass rows, in 16-byte vectors
+  uint8_t* page[2];
+  float* scale[2];
+  float s_old[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int r = base + i * kRowsPerPass + row;
-      x[i] = r < rows ? __ldg(src + r * step) : make_uint4(0, 0, 0, 0);
+  for (int kv = 0; kv < 2; ++kv) {
+    src[kv] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[kv]) + token * a.stride_t[kv] +
+                                             (int64_t)head * a.stride_h[kv]) + col;
+    step[kv] = a.stride_t[kv] / 8 * kRowsPerPass;
+    page[kv] = a.cache[kv] + (int64_t)blk * a.stride_block[kv] + (int64_t)head * a.stride_head[kv];
+    scale[kv] = a.scale[kv] + (int64_t)blk * a.h_kv + head;
+    if (old && live) s_old[kv] = *scale[kv];
+  }
+
+  uint4 x[2][kVec];
+  auto load = [&](int base) {  // base: a multiple of kRowsHeld
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint4* p = src[kv] + (int64_t)(base / kRowsPerPass) * step[kv];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i, p += step[kv])
+        x[kv][i] = base + i * kRowsPerPass + row < rows ? __ldg(p) : make_uint4(0, 0, 0, 0);
     }
   };
-  // The largest magnitude: of the values' bits without signs, whose order is
-  // the values', two at a time.  Infinities and NaN, which do not count, are
-  // left out by a second look where there are any.
-  constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
-  uint32_t top = 0;
+  // The largest magnitudes: of the values' bits without signs, whose order
+  // is the values', two at a time.  Infinities and NaN, which do not count,
+  // are left out by a second look where there are any.
+  uint32_t top[2] = {0, 0};
   for (int base = 0; base < rows; base += kRowsHeld) {
     load(base);
-    uint32_t t = 0;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[i]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t = max_halves(t, q[j] & 0x7FFF7FFFu);
-    }
-    if (max(t & 0xFFFFu, t >> 16) >= kInf) {
-      t = 0;
+    for (int kv = 0; kv < 2; ++kv) {
+      uint32_t t = 0;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[i]);
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[kv][i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = q[j] & 0x7FFFu, hi = (q[j] >> 16) & 0x7FFFu;
-          t = max(t, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+        for (int j = 0; j < 4; ++j) t = max_halves(t, q[j] & 0x7FFF7FFFu);
+      }
+      if (max(t & 0xFFFFu, t >> 16) >= kInf) {
+        t = 0;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[kv][i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = q[j] & 0x7FFFu, hi = (q[j] >> 16) & 0x7FFFu;
+            t = max(t, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+          }
         }
       }
+      top[kv] = max(top[kv], max(t & 0xFFFFu, t >> 16));
     }
-    top = max(top, max(t & 0xFFFFu, t >> 16));
   }
-  float amax = to_f32x2<T>(top).x;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int kv = 0; kv < 2; ++kv) top[kv] = __reduce_max_sync(0xffffffffu, top[kv]);
+  float amax[2] = {to_f32x2<T>(top[0]).x, to_f32x2<T>(top[1]).x};
   if constexpr (TEAM > 1) {
-    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = amax;
+    if ((threadIdx.x & 31) == 0) {
+      s_red[0][threadIdx.x >> 5] = amax[0];
+      s_red[1][threadIdx.x >> 5] = amax[1];
+    }
     __syncthreads();  // also: every thread has read s_old before the scale is written
 #pragma unroll
-    for (int i = 0; i < TEAM; ++i) amax = fmaxf(amax, s_red[team * TEAM + i]);
+    for (int i = 0; i < TEAM; ++i) {
+      amax[0] = fmaxf(amax[0], s_red[0][team * TEAM + i]);
+      amax[1] = fmaxf(amax[1], s_red[1][team * TEAM + i]);
+    }
   } else {
     __syncwarp();
   }
   if (!live) return;
-  float s = __uint_as_float((uint32_t)(scale_exponent(amax) + 127) << 23);
-  if (old) s = fmaxf(s, s_old);
-  if (lane == 0) *scale = s;
-  if (old && s != s_old) {
-    const float ratio = s_old / s;
-    for (int e = lane; e < old * (D / 16); e += kLanes) {
-      uint4* p = reinterpret_cast<uint4*>(page + (int64_t)(e / (D / 16)) * a.stride_row[kv]) + e % (D / 16);
-      uint4 q = *p;
-      q.x = rescale_word(q.x, ratio);
-      q.y = rescale_word(q.y, ratio);
-      q.z = rescale_word(q.z, ratio);
-      q.w = rescale_word(q.w, ratio);
-      *p = q;
+  float s[2], inv[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    s[kv] = __uint_as_float((uint32_t)(scale_exponent(amax[kv]) + 127) << 23);
+    if (old) s[kv] = fmaxf(s[kv], s_old[kv]);
+    inv[kv] = 1.f / s[kv];
+    if (lane == 0) *scale[kv] = s[kv];
+    if (old && s[kv] != s_old[kv]) {
+      const float ratio = s_old[kv] / s[kv];
+      for (int e = lane; e < old * (D / 16); e += kLanes) {
+        uint4* p = reinterpret_cast<uint4*>(page[kv] + (int64_t)(e / (D / 16)) * a.stride_row[kv]) + e % (D / 16);
+        *p = rescale(*p, ratio);
+      }
     }
   }
-  // A power of two divides exactly by its reciprocal; any other scale (a
-  // block that the caller filled by a rule of their own) takes the division.
-  const bool exact = is_power_of_two(s);
-  const float inv = 1.f / s;
   for (int base = 0; base < rows; base += kRowsHeld) {
     if (rows > kRowsHeld) load(base);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int r = base + i * kRowsPerPass + row;
-      if (r < rows) {
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[i]);
-        uint32_t b[4];
+    for (int kv = 0; kv < 2; ++kv) {
+      if (!is_power_of_two(s[kv])) continue;
+      uint8_t* p = page[kv] + (int64_t)(r0 + base + row) * a.stride_row[kv] + col * 8;
+      const int64_t next = a.stride_row[kv] * kRowsPerPass;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 f = to_f32x2<T>(q[j]);
-          if (exact) {
-            f = scaled(f, inv);
-          } else {
-            f.x /= s;
-            f.y /= s;
+      for (int i = 0; i < kVec; ++i, p += next) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(&x[kv][i]);
+        if (base + i * kRowsPerPass + row < rows) {
+          uint32_t b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // a power of two divides exactly by its reciprocal
+            const float2 f = scaled(to_f32x2<T>(q[j]), inv[kv]);
+            b[j] = to_e4m3x2(f.x, f.y);
           }
-          b[j] = to_e4m3x2(f.x, f.y);
+          *reinterpret_cast<uint2*>(p) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
         }
-        *reinterpret_cast<uint2*>(page + (int64_t)(r0 + r) * a.stride_row[kv] + (lane % kVecPerRow) * 8) =
-            make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
       }
+    }
+  }
+  // Another scale (a block that the caller filled by a rule of their own)
+  // takes the division, which unrolled above would crowd out the rest.
+#pragma unroll 1
+  for (int kv = 0; kv < 2; ++kv) {
+    const float sc = kv ? s[1] : s[0];
+    if (is_power_of_two(sc)) continue;
+#pragma unroll 1
+    for (int r = row; r < rows; r += kRowsPerPass) {
+      const uint4 v = __ldg((kv ? src[1] : src[0]) + (int64_t)(r / kRowsPerPass) * (kv ? step[1] : step[0]));
+      const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = to_f32x2<T>(q[j]);
+        b[j] = to_e4m3x2(f.x / sc, f.y / sc);
+      }
+      *reinterpret_cast<uint2*>((kv ? page[1] : page[0]) + (int64_t)(r0 + r) * (kv ? a.stride_row[1] : a.stride_row[0]) +
+                                col * 8) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
     }
   }
 }
@@ -250,15 +306,15 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t stream) {
   // From about 8 tokens a sequence on, a block's rows fill a team of four
   // warps' registers; below it they are mostly one warp's.
   if (a.n > 8 * (int64_t)a.b)
-    gqa_append_kernel<T, D, 4><<<dim3(items, (2 * a.h_kv + 1) / 2), 256, 0, stream>>>(a);
+    gqa_append_kernel<T, D, 4><<<dim3(items, (a.h_kv + 1) / 2), 256, 0, stream>>>(a);
   else
-    gqa_append_kernel<T, D, 1><<<dim3(items, (2 * a.h_kv + 7) / 8), 256, 0, stream>>>(a);
+    gqa_append_kernel<T, D, 1><<<dim3(items, (a.h_kv + 7) / 8), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ eviction
 struct EvictArgs {
-  int budget, recent, width, new_width, page, table_width, new_table_width, num_blocks, h_kv, b;
+  int budget, recent, width, new_width, page, page_shift, table_width, new_table_width, num_blocks, h_kv, b;
   const float* weights;
   int64_t stride_w_b, stride_w_h;
   float* new_weights;
@@ -281,68 +337,51 @@ __device__ __forceinline__ int evict_len(const EvictArgs& a, int seq) {
 }
 
 // Bits whose unsigned order is the order of the weights: NaN above all
-// numbers, +0 and -0 alike.
+// numbers, +0 and -0 alike.  Adding zero makes -0 +0 and any NaN the one
+// with all bits but the sign set.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0xFFFFFFFFu;
-  const uint32_t bits = __float_as_uint(w + 0.f);  // -0 + 0 = +0
-  return bits ^ ((bits >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  const uint32_t bits = __float_as_uint(__fadd_rn(w, 0.f));
+  return bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u);
 }
 
 constexpr int kSelThreads = 1024;
 constexpr int kChunk = 4 * kSelThreads;  // positions of a step, four to a thread
-constexpr int kHeld = 8;                 // steps whose keys a thread keeps: 32,768 positions
 constexpr int kBins = 2048;              // digits of 11, 11 and 10 bits
 constexpr int kHists = 4;                // copies of the histogram, against conflicts on near weights
+constexpr int kList = 3400;              // keys of one digit that are listed (static shared memory ends at 48 KB)
 
 // One CTA per (sequence, KV head): the key of the last position that is kept
-// by three passes of a radix histogram from the top digit down, then one
-// ordered pass that writes the kept positions (a running count of those
-// above that key and of those equal to it; of the latter only the first ones
-// are kept).  The weights are read once into registers (32 a thread; longer
-// sequences are read again, from L2, in every pass).  The histogram's
-// conflicts bound it: a digit of sign, exponent and two bits spreads weights
-// of one magnitude over some bins, and exact zeros (positions that nothing
-// looked at) are counted by vote.
-__global__ void __launch_bounds__(kSelThreads) gqa_evict_select_kernel(const EvictArgs a) {
+// by a radix histogram from the top digit down, then one ordered pass that
+// writes the kept positions (a running count of those above that key and of
+// those equal to it; of the latter only the first ones are kept).  Where few
+// keys share the top digit (a digit of sign, exponent and two bits spreads
+// weights of one magnitude over some bins), they are listed and the other
+// digits look at the list only, so the weights are read three times (from L2
+// after the first).  Exact zeros, of positions that nothing looked at, are
+// counted by vote instead of by conflicting atomics.  Bound by instructions
+// (65 % of the issue slots), and by the longest sequence.  32 sequences of
+// up to 32,768, 8 heads: 31 us; an earlier form with the keys held in
+// registers and one CTA per SM 37, with 512 threads 45, with a cluster of
+// four CTAs per sequence that sum their histograms over distributed shared
+// memory 66 (its fixed cost, paid four times, outweighs the split).
+__global__ void __launch_bounds__(kSelThreads, 2) gqa_evict_select_kernel(const EvictArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
-  __shared__ uint32_t hist[kHists][kBins];
+  __shared__ alignas(16) uint32_t hist[kHists][kBins];
+  __shared__ uint32_t list[kList];
   __shared__ uint32_t s_scan[kSelThreads / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ uint32_t s_prefix, s_found;
+  __shared__ int s_need, s_count;
+  const int head = blockIdx.x, seq = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = evict_len(a, seq);
   const int new_len = min(len, a.budget);
   const float* w = a.weights + (int64_t)seq * a.stride_w_b + (int64_t)head * a.stride_w_h;
   float* nw = a.new_weights + (int64_t)seq * a.stride_nw_b + (int64_t)head * a.stride_nw_h;
   int32_t* kept = a.kept + ((int64_t)seq * a.h_kv + head) * a.budget;
-  if (head == 0 && tid == 0) a.new_lens[seq] = new_len;
   const int recent = len > a.budget ? a.recent : len;  // positions that are kept without a look
   const int older = len - recent;
   const int pick = new_len - recent;  // of the older ones
-  // four positions from i on, as keys; those that are not older ones are 0,
-  // which no weight's key is
-  const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
-  auto keys_at = [&](int i, uint32_t (&k)[4]) {
-    float x[4];
-    if (vec && i + 4 <= older) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(w + i));
-      x[0] = v.x;
-      x[1] = v.y;
-      x[2] = v.z;
-      x[3] = v.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = i + j < older ? __ldg(w + i + j) : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k[j] = i + j < older ? weight_key(x[j]) : 0u;
-  };
-  const bool held = older <= kHeld * kChunk;
-  uint32_t mine[kHeld][4];
-  if (pick > 0 && held) {
-#pragma unroll
-    for (int s = 0; s < kHeld; ++s) keys_at(s * kChunk + 4 * tid, mine[s]);
-  }
+  if (head == 0 && tid == 0) a.new_lens[seq] = new_len;
   for (int i = new_len + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
   for (int i = new_len + tid; i < a.new_width; i += kSelThreads) nw[i] = 0.f;
   for (int i = tid; i < recent; i += kSelThreads) {
@@ -350,49 +389,50 @@ __global__ void __launch_bounds__(kSelThreads) gqa_evict_select_kernel(const Evi
     nw[new_len - recent + i] = __ldg(w + older + i);
   }
   if (pick == 0) return;
-  // f(step, keys) over all steps
-  auto each = [&](auto f) {
-    if (held) {
-#pragma unroll
-      for (int s = 0; s < kHeld; ++s)
-        if (s * kChunk < older) f(s, mine[s]);
+  // f(i, keys, weights) for each four positions from i on; those that are not
+  // older ones have the key 0, which no weight's is
+  const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  auto four = [&](int i, auto f) {
+    if (vec && i + 4 <= older) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(w + i));
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      const uint32_t k[4] = {weight_key(x.x), weight_key(x.y), weight_key(x.z), weight_key(x.w)};
+      f(k, v);
     } else {
-      for (int s = 0; s * kChunk < older; ++s) {
-        uint32_t k[4];
-        keys_at(s * kChunk + 4 * tid, k);
-        f(s, k);
+      float v[4];
+      uint32_t k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = i + j < older ? __ldg(w + i + j) : 0.f;
+        k[j] = i + j < older ? weight_key(v[j]) : 0u;
       }
+      f(k, v);
     }
   };
 
   constexpr uint32_t kZero = 0x80000000u;  // weight_key(0)
+  bool listed = false;
   uint32_t prefix = 0;
-  int need = pick;  // the need-th largest key is looked for among those that share `prefix`
-#pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kHists * kBins; i += kSelThreads) (&hist[0][0])[i] = 0;
+  int need = pick, same = 0;  // the need-th largest key is looked for among those that share `prefix`, `same` of them
+  // One digit: count(histogram) adds the keys with the prefix to the copies
+  // and returns how many zeros there are among them, which it leaves out.
+  auto digit = [&](int shift, int bits, auto count) {
+    for (int i = 4 * tid; i < kHists * kBins; i += 4 * kSelThreads)
+      *reinterpret_cast<uint4*>(&hist[0][0] + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    uint32_t* h = hist[(tid >> 1) % kHists];
-    uint32_t zeros = 0;
-    each([&](int, const uint32_t(&k)[4]) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = k[j] != 0 && (pass == 0 || (k[j] >> (shift + bits)) == prefix);
-        if (in && k[j] == kZero) ++zeros;
-        if (in && k[j] != kZero) atomicAdd(&h[(k[j] >> shift) & ((1u << bits) - 1)], 1u);
-      }
-    });
-    zeros = __reduce_add_sync(0xffffffffu, zeros);
+    const uint32_t zeros = __reduce_add_sync(0xffffffffu, count(hist[(tid >> 1) % kHists]));
     if (lane == 0 && zeros) atomicAdd(&hist[0][(kZero >> shift) & ((1u << bits) - 1)], zeros);
     __syncthreads();
     // thread t has the two bins below 2048 - 2 t, the largest keys first
+    const int bin0 = kBins - 2 * (tid + 1);
     uint32_t c[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int k = 0; k < kHists; ++k) c[j] += hist[k][kBins - 1 - (2 * tid + j)];
-    uint32_t incl = c[0] + c[1];
+    for (int k = 0; k < kHists; ++k) {
+      const uint2 v = *reinterpret_cast<const uint2*>(&hist[k][bin0]);
+      c[0] += v.y;
+      c[1] += v.x;
+    }
+    uint32_t incl = c[0] + c[1], before = 0u - incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -400,67 +440,149 @@ __global__ void __launch_bounds__(kSelThreads) gqa_evict_select_kernel(const Evi
     }
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    const uint32_t others = __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0u);
-    uint32_t before = others + incl - c[0] - c[1];
+    before += incl + __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0u);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if ((int)before < need && need <= (int)(before + c[j])) {
-        s_prefix = (prefix << bits) | (uint32_t)(kBins - 1 - (2 * tid + j));
+        s_prefix = (prefix << bits) | (uint32_t)(bin0 + 1 - j);
         s_need = need - (int)before;
+        s_count = (int)c[j];
       }
       before += c[j];
     }
+    if (tid == 0 && !listed) s_found = 0;
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
-  }
-  // prefix is the last kept key; `need` of the positions equal to it are kept
-  uint32_t above = 0, equal = 0;  // counts before this step
-  each([&](int s, const uint32_t(&k)[4]) {
-    uint32_t n = 0;  // (above << 16) | equal: a step has 4,096 positions
+    same = s_count;
+  };
+  digit(21, 11, [&](uint32_t* h) {
+    uint32_t zeros = 0;
+#pragma unroll 2
+    for (int i = 4 * tid; i < older; i += kChunk)
+      four(i, [&](const uint32_t(&k)[4], const float(&)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) n += k[j] > prefix ? 1u << 16 : k[j] == prefix ? 1u : 0u;
+        for (int j = 0; j < 4; ++j) {
+          if (k[j] == kZero) ++zeros;
+          else if (k[j] != 0) atomicAdd(&h[k[j] >> 21], 1u);
+        }
+      });
+    return zeros;
+  });
+  if (same <= kList) {
+    listed = true;
+#pragma unroll 2
+    for (int i = 4 * tid; i < older; i += kChunk)
+      four(i, [&](const uint32_t(&k)[4], const float(&)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if ((k[j] >> 21) == prefix) list[atomicAdd(&s_found, 1u)] = k[j];
+      });
+  }
+#pragma unroll 1
+  for (int shift = 10; shift >= 0; shift -= 10) {
+    const int bits = shift ? 11 : 10;
+    digit(shift, bits, [&](uint32_t* h) {
+      uint32_t zeros = 0;
+      auto one = [&](uint32_t k) {
+        if ((k >> shift >> bits) != prefix || k == 0) return;
+        if (k == kZero) ++zeros;
+        else atomicAdd(&h[(k >> shift) & ((1u << bits) - 1)], 1u);
+      };
+      if (listed) {
+        for (int i = tid; i < (int)s_found; i += kSelThreads) one(list[i]);
+      } else {
+#pragma unroll 1
+        for (int i = 4 * tid; i < older; i += kChunk)
+          four(i, [&](const uint32_t(&k)[4], const float(&)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) one(k[j]);
+          });
+      }
+      return zeros;
+    });
+  }
+
+  // prefix is the last kept key; `need` of the `same` positions equal to it
+  // are kept: mostly all of them, otherwise the first.  Counts of those kept
+  // for certain (the low half of a step's sum) and of those equal (the high).
+  const bool ties = need < same, top = ties && prefix == 0xFFFFFFFFu;  // top: nothing lies above the last key
+  const uint32_t sure = ties && !top ? prefix + 1 : prefix;
+  uint32_t above = 0, equal = 0;  // counts before this step
+#pragma unroll 1
+  for (int base = 0; base < older; base += kChunk) {
+    const int i = base + 4 * tid;
+    uint32_t k[4];
+    float v[4];
+    four(i, [&](const uint32_t(&kk)[4], const float(&vv)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        k[j] = kk[j];
+        v[j] = vv[j];
+      }
+    });
+    uint32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += k[j] >= sure && !top ? 1u : 0u;
+    if (ties) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n += k[j] == prefix ? 1u << 16 : 0u;
+    }
     uint32_t incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
     }
-    __syncthreads();
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
     const uint32_t sums = s_scan[lane];
     const uint32_t pre = __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0u) + incl - n;
     const uint32_t total = __reduce_add_sync(0xffffffffu, sums);
-    uint32_t g = above + (pre >> 16), e = equal + (pre & 0xFFFFu);
+    __syncthreads();  // s_scan is read
+    uint32_t g = above + (pre & 0xFFFFu), e = equal + (pre >> 16);
+    if (!ties) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool is_above = k[j] > prefix, is_equal = k[j] == prefix;
-      if (is_above || (is_equal && e < (uint32_t)need)) {
-        const uint32_t at = g + min(e, (uint32_t)need);
-        const int pos = s * kChunk + 4 * tid + j;
-        kept[at] = pos;
-        nw[at] = __ldg(w + pos);  // the weight itself: a key does not tell -0 from 0, nor NaN from NaN
+      for (int j = 0; j < 4; ++j) {
+        if (k[j] >= sure) {
+          kept[g] = i + j;
+          nw[g] = v[j];
+          ++g;
+        }
       }
-      g += is_above;
-      e += is_equal;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool is_above = k[j] >= sure && !top, is_equal = k[j] == prefix;
+        if (is_above || (is_equal && e < (uint32_t)need)) {
+          const uint32_t at = g + min(e, (uint32_t)need);
+          kept[at] = i + j;
+          nw[at] = v[j];
+        }
+        g += is_above;
+        e += is_equal;
+      }
     }
-    above += total >> 16;
-    equal += total & 0xFFFFu;
-  });
+    above += total & 0xFFFFu;
+    equal += total >> 16;
+  }
 }
 
-// One CTA per (new block, KV head, sequence): the sources of its rows, the
-// largest of their scales, then the rows of K and V, 16 bytes per thread
-// and load.  Bound by the kept bytes, read and written once.
+// One CTA per (new block, KV head, sequence): the sources of its rows, then
+// the rows of K and V, 16 bytes per thread and load, and, while those are on
+// their way, the largest of the sources' scales.  Bound by the kept bytes,
+// read (rows at random places) and written once.
 constexpr int kGatherThreads = 128;
+struct Source {
+  int64_t off;  // bytes, -1: nothing there
+  float scale;
+  int unused;
+};
 template <int D>
-__global__ void __launch_bounds__(kGatherThreads) gqa_evict_gather_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(kGatherThreads, 8) gqa_evict_gather_kernel(const EvictArgs a) {
   constexpr int kVec = D / 16;
-  constexpr int kUnroll = 8;  // K and V of 64 rows of 128: all loads in flight at once
-  extern __shared__ uint8_t smem_raw[];
-  int64_t* s_off = reinterpret_cast<int64_t*>(smem_raw);        // [2][page] source bytes, -1: nothing there
-  float* s_scale = reinterpret_cast<float*>(s_off + 2 * a.page);  // [2][page]
+  constexpr int kUnroll = 4;  // of K and of V: all of 64 rows of 128 in flight at once
+  extern __shared__ Source s_src[];  // [2][page]
   __shared__ float s_red[2][kGatherThreads / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the kept positions
   const int nb = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;
@@ -472,23 +594,51 @@ __global__ void __launch_bounds__(kGatherThreads) gqa_evict_gather_kernel(const 
   if (dest < 0 || dest >= a.num_blocks) return;
   const int rows = min(a.page, new_len - j0);
   const int32_t* kept = a.kept + ((int64_t)seq * a.h_kv + head) * a.budget + j0;
-  float top[2] = {0.f, 0.f};
+  float top[2] = {0.f, 0.f}, mine[2] = {0.f, 0.f};  // mine: of row tid, not looked at before the loads below
   for (int r = tid; r < rows; r += kGatherThreads) {
     const int t = kept[r];
-    const int blk = t >= 0 && t < len ? __ldg(a.table + (int64_t)seq * a.stride_table + t / a.page) : -1;
+    const int blk = t >= 0 && t < len ? __ldg(a.table + (int64_t)seq * a.stride_table + (t >> a.page_shift)) : -1;
     const bool ok = blk >= 0 && blk < a.num_blocks;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      const float s = ok ? a.scale[kv][(int64_t)blk * a.h_kv + head] : 0.f;
-      s_off[kv * a.page + r] = ok ? (int64_t)blk * a.stride_block[kv] + (int64_t)(t % a.page) * a.stride_row[kv] +
-                                        (int64_t)head * a.stride_head[kv]
-                                  : -1;
-      s_scale[kv * a.page + r] = s;
-      top[kv] = fmaxf(top[kv], s);
+      const float scale = ok ? a.scale[kv][(int64_t)blk * a.h_kv + head] : 0.f;
+      s_src[kv * a.page + r].off = ok ? (int64_t)blk * a.stride_block[kv] + (int64_t)(t & (a.page - 1)) * a.stride_row[kv] +
+                                            (int64_t)head * a.stride_head[kv]
+                                      : -1;
+      if (r < kGatherThreads) {
+        mine[kv] = scale;
+      } else {
+        s_src[kv * a.page + r].scale = scale;
+        top[kv] = fmaxf(top[kv], scale);
+      }
     }
   }
+  __syncthreads();
+  const int n = rows * kVec;
+  uint8_t* to[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+    to[kv] = a.cache[kv] + (int64_t)dest * a.stride_block[kv] + (int64_t)head * a.stride_head[kv] + tid % kVec * 16;
+  static_assert(kGatherThreads % kVec == 0, "a thread keeps its 16 bytes of a row");
+  uint4 q[2][kUnroll];
+  auto load = [&](int e0) {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int e = e0 + u * kGatherThreads;
+        q[kv][u] = make_uint4(0, 0, 0, 0);
+        if (e < n) {
+          const int64_t off = s_src[kv * a.page + e / kVec].off;
+          if (off >= 0) q[kv][u] = *reinterpret_cast<const uint4*>(a.cache[kv] + off + tid % kVec * 16);
+        }
+      }
+  };
+  load(tid);
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
+    if (tid < rows) s_src[kv * a.page + tid].scale = mine[kv];
+    top[kv] = fmaxf(top[kv], mine[kv]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top[kv] = fmaxf(top[kv], __shfl_xor_sync(0xffffffffu, top[kv], o));
     if ((tid & 31) == 0) s_red[kv][tid >> 5] = top[kv];
@@ -500,36 +650,19 @@ __global__ void __launch_bounds__(kGatherThreads) gqa_evict_gather_kernel(const 
     for (int i = 0; i < kGatherThreads / 32; ++i) top[kv] = fmaxf(top[kv], s_red[kv][i]);
     if (tid == 0) a.scale[kv][(int64_t)dest * a.h_kv + head] = top[kv];
   }
-  // K's rows, then V's
-  for (int e0 = tid; e0 < 2 * rows * kVec; e0 += kGatherThreads * kUnroll) {
-    uint4 q[kUnroll];
+  for (int e0 = tid; e0 < n; e0 += kGatherThreads * kUnroll) {
+    if (e0 != tid) load(e0);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int e = e0 + u * kGatherThreads;
-      q[u] = make_uint4(0, 0, 0, 0);
-      if (e < 2 * rows * kVec) {
-        const int kv = e >= rows * kVec, r = e / kVec - kv * rows;
-        const int64_t off = s_off[kv * a.page + r];
-        if (off >= 0) q[u] = *(reinterpret_cast<const uint4*>(a.cache[kv] + off) + e % kVec);
-      }
-    }
+    for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int e = e0 + u * kGatherThreads;
-      if (e < 2 * rows * kVec) {
-        const int kv = e >= rows * kVec, r = e / kVec - kv * rows;
-        const float s = s_scale[kv * a.page + r];
-        if (s != top[kv]) {
-          const float ratio = s / top[kv];  // 0 <= s < top
-          q[u].x = rescale_word(q[u].x, ratio);
-          q[u].y = rescale_word(q[u].y, ratio);
-          q[u].z = rescale_word(q[u].z, ratio);
-          q[u].w = rescale_word(q[u].w, ratio);
+      for (int u = 0; u < kUnroll; ++u) {
+        const int e = e0 + u * kGatherThreads;
+        if (e < n) {
+          const float scale = s_src[kv * a.page + e / kVec].scale;
+          if (scale != top[kv]) q[kv][u] = rescale(q[kv][u], scale / top[kv]);  // 0 <= scale < top
+          *reinterpret_cast<uint4*>(to[kv] + (int64_t)(e / kVec) * a.stride_row[kv]) = q[kv][u];
         }
-        uint8_t* to = a.cache[kv] + (int64_t)dest * a.stride_block[kv] + (int64_t)head * a.stride_head[kv];
-        *(reinterpret_cast<uint4*>(to + (int64_t)r * a.stride_row[kv]) + e % kVec) = q[u];
       }
-    }
   }
 }
 
@@ -578,6 +711,7 @@ cudaError_t launch_gqa_evict(const dsv4b_gqa_cache& c, const dsv4b_gqa_evict_par
   a.width = e.width;
   a.new_width = e.new_width;
   a.page = c.page_block_size;
+  while ((1 << a.page_shift) < a.page) ++a.page_shift;
   a.table_width = c.table_width;
   a.new_table_width = e.new_table_width;
   a.num_blocks = c.num_blocks;
@@ -613,7 +747,7 @@ cudaError_t launch_gqa_evict(const dsv4b_gqa_cache& c, const dsv4b_gqa_evict_par
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks < e.new_table_width ? blocks : e.new_table_width, c.h_kv, c.b);
   cfg.blockDim = dim3(kGatherThreads);
-  cfg.dynamicSmemBytes = (size_t)c.page_block_size * 24;  // <= 24 KB
+  cfg.dynamicSmemBytes = (size_t)c.page_block_size * 2 * sizeof(Source);  // <= 32 KB
   cfg.stream = stream;
   cudaLaunchAttribute attr;  // starts while the selection ends; waits for it in the kernel
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
