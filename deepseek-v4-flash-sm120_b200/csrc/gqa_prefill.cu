@@ -9,9 +9,9 @@
 // core at d = 128, and 128^2 exponentials, 1,024 cycles of an SM's 16 a
 // cycle).
 //
-// One CTA has 256 queries of one head, as two tiles of 128, and walks the
-// keys they see.  While the tensor core multiplies for one tile, four warps
-// do the softmax of the other:
+// An item is 256 queries of one head, as two tiles of 128, and the keys they
+// see.  While the tensor core multiplies for one tile, four warps do the
+// softmax of the other:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, a thread per row: S comes from
 //                   TMEM, P goes back there over S (16 bits, the A operand
 //                   of O += P v).  O is rescaled only when a row's maximum
@@ -20,10 +20,17 @@
 //                   quotient), which after the first tiles is rare;
 //   warp 8          issues the MMAs: S_0 S_1, then per key tile O_0 S_0' O_1
 //                   S_1', so that each softmax has the other tile's MMAs to
-//                   hide behind;
-//   warp 9          loads Q once and the K, V ring by TMA (SWIZZLE_128B);
+//                   hide behind (starting O when half of P is there was
+//                   slower: the warp waits for the other half meanwhile);
+//   warp 9          finds the items and loads Q and the K and V rings by TMA
+//                   (SWIZZLE_128B), up to an item ahead of the rest;
 //   warps 10, 11    V's guards, below.
 // TMEM: S_0 [0, 128), S_1 [128, 256), O_0 and O_1 from 256 on.
+//
+// A CTA stays on its SM and takes its next item from the CTAs that have not
+// started yet (cluster launch control), so that the next item's loads and
+// first S run under this one's last softmax and output.  A CTA for each item
+// spent 6 us of it on its start and end.
 //
 // Masked keys have P = 0, but 0 * NaN is NaN: a row of V behind the
 // sequence's end belongs to another sequence or to nobody, and one behind a
@@ -32,9 +39,11 @@
 // that is not finite, before the MMA reads them, and notes the rows of the
 // latter: a query that does see one has the value added at the end.
 //
-// The list of CTAs needs no lengths on the host: sequence i has the tiles
+// The list of items needs no lengths on the host: sequence i has the tiles
 // from cu_i / 256 + i on, at least as many as it can fill.  The last tiles
-// of a sequence, which see most keys, come first.
+// of a sequence, which see most keys, come first.  Heads are taken in groups
+// whose K and V stay in L2 (kGroupBytes): 128 heads of 5,000 keys at once
+// read theirs from HBM for every tile.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -62,13 +71,15 @@ constexpr int kSoftmaxRegs = 216, kOtherRegs = 64;  // of 168 at launch: 2 * 216
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kGuardWarp = 10, kGuardWarps = 2;
 constexpr int kChunk = kM * 128;     // 128 rows x 64 16-bit columns, swizzled
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxEdge = 4;          // key tiles that some row of a CTA does not see whole
+constexpr int kMaxEdge = 4;          // key tiles that some row of an item does not see whole
+constexpr int kEdgeRing = 2 * kMaxEdge;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;      // log2 of how far a maximum may be outgrown
+constexpr int64_t kGroupBytes = 40 << 20;  // K and V of the heads that run at a time: a third of L2
 
 struct PrefillArgs {
-  int b, h_q, g, causal, total_q, total_k, tiles;
+  int b, h_q, g, causal, total_q, total_k, tiles, group_heads;
   float scale_log2;
   const void* v;
   int64_t stride_v_t, stride_v_h;
@@ -79,34 +90,76 @@ struct PrefillArgs {
   float* lse;
 };
 
-// Ring depths that fit 227 KB beside Q.
+// Ring depths that fit 227 KB beside Q: K in chunks of 64 columns, each
+// released by itself, V in whole tiles (its chunks stay side by side).
 template <int DQK, int DV>
 struct Cfg {
-  static constexpr int kQ = 2 * (DQK / 64) * kChunk;
-  static constexpr int kK = (DQK / 64) * kChunk;
+  static constexpr int kChunksQ = DQK / 64;
+  static constexpr int kQ = 2 * kChunksQ * kChunk;
   static constexpr int kV = (DV / 64) * kChunk;
-  static constexpr int kStagesK = DQK == 64 ? 4 : 2;
-  static constexpr int kStagesV = DQK == 64 ? 4 : DQK == 128 ? 2 : 1;
+  static constexpr int kSlotsK = DQK == 192 ? 4 : 6;
+  static constexpr int kStagesV = DQK == 64 ? 6 : 2;
+};
+
+// What a CTA works on.
+struct Item {
+  int q0, rows;       // first query (row of q) and how many, 1 .. 256; 0: no more items
+  int k0, n_k;        // the sequence's keys
+  int see;            // keys that the first query sees if causal (may be < 0)
+  int head;
+  __device__ __forceinline__ int limit(int r, int causal) const { return causal ? min(n_k, see + r) : n_k; }
+  // key tiles of query tile i
+  __device__ __forceinline__ int tiles(int i, int causal) const {
+    const int last = min(rows, (i + 1) * kM) - 1;
+    return last >= i * kM ? (max(0, limit(last, causal)) + kM - 1) / kM : 0;
+  }
+  // the first key tile that some row does not see whole
+  __device__ __forceinline__ int edge(int causal) const { return max(0, limit(0, causal)) / kM; }
 };
 
 struct Shared {
-  uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], go[kMaxEdge], guard[kMaxEdge];
+  uint64_t q_full[2], q_empty[2], k_full[6], k_empty[6], v_full[6], v_empty[6], go[kEdgeRing], guard[kEdgeRing];
   uint64_t s_full[2], p_full[2], o_full[2], done;
-  uint32_t bad[kMaxEdge][4];  // rows of V with a value that is not finite
+  uint64_t item_full[2], item_empty[2], next_full;
+  alignas(16) uint32_t next[4];  // cluster launch control's answer
+  Item item[2];
+  uint32_t bad[2][kMaxEdge][4];  // of an item: rows of V with a value that is not finite
   uint32_t tmem;
   int abort;
 };
+constexpr int kItemReaders = 8 + 1 + 2;  // softmax, MMA and guard warps
 
 template <int DQK, int DV>
 constexpr int smem_bytes() {
   using C = Cfg<DQK, DV>;
-  return 1024 + C::kQ + C::kStagesK * C::kK + C::kStagesV * C::kV + (int)sizeof(Shared);
+  return 1024 + C::kQ + C::kSlotsK * kChunk + C::kStagesV * C::kV + (int)sizeof(Shared);
 }
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
   return r != 0;
+}
+
+// Cluster launch control: asks for a CTA of this grid that has not started
+// (16 bytes of answer, counted on `bar`), and reads the answer: the CTA's
+// number, or -1 when there are none left (then it must not be asked again).
+__device__ __forceinline__ void ask_next(uint32_t answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   answer),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int read_next(uint32_t answer) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\tld.shared.b128 a, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\tmov.s32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=r"(r)
+      : "r"(answer)
+      : "memory");
+  return r;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem], 16-bit operands, fp32 sums.
@@ -152,6 +205,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// 32 bytes to a 32-byte aligned address.
+__device__ __forceinline__ void store_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -175,79 +235,44 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return __vcmpeq2(w & e, e);
 }
 
-// What a CTA works on, the same in every thread.
-struct Work {
-  int q0, rows;       // first query (row of q) and how many, 1 .. 256
-  int k0, n_k;        // the sequence's keys
-  int see;            // keys that the first query sees if causal (may be < 0)
-  int head;
-  __device__ __forceinline__ int limit(int r, int causal) const { return causal ? min(n_k, see + r) : n_k; }
-};
-
 template <typename T, int DQK, int DV>
 __global__ void __launch_bounds__(kThreads, 1)
 gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const PrefillArgs a) {
   using C = Cfg<DQK, DV>;
-  constexpr int kStagesK = C::kStagesK, kStagesV = C::kStagesV;
+  constexpr int kSlotsK = C::kSlotsK, kStagesV = C::kStagesV, kChunksQ = C::kChunksQ;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t q_s = smem_u32(smem), k_s = q_s + C::kQ, v_s = k_s + kStagesK * C::kK;
-  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kQ + kStagesK * C::kK + kStagesV * C::kV);
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + C::kQ, v_s = k_s + kSlotsK * kChunk;
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kQ + kSlotsK * kChunk + kStagesV * C::kV);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  Work w;
-  {
-    const int tile = a.tiles - 1 - (int)(blockIdx.x / a.h_q);
-    auto cq = [&](int i) { return min(max(__ldg(a.cu_q + i), 0), a.total_q); };
-    int seq = 0;  // the number of i in [1, b) with cu_i / 256 + i <= tile
-    for (int i0 = 1; i0 < a.b; i0 += kThreads) {
-      const int i = i0 + tid;
-      const int c = __syncthreads_count(i < a.b && cq(i) / kQueries + i <= tile);
-      seq += c;
-      if (c < kThreads) break;
-    }
-    const int lo = cq(seq), n_q = max(0, cq(seq + 1) - lo);
-    const int t0 = (tile - (lo / kQueries + seq)) * kQueries;
-    if (t0 < 0 || t0 >= n_q) return;  // (t0 < 0: offsets that do not ascend)
-    w.head = (int)(blockIdx.x % a.h_q);
-    w.q0 = lo + t0;
-    w.rows = min(kQueries, n_q - t0);
-    w.k0 = min(max(__ldg(a.cu_k + seq), 0), a.total_k);
-    w.n_k = max(0, min(__ldg(a.cu_k + seq + 1), a.total_k) - w.k0);
-    w.see = t0 + w.n_k - n_q + 1;
-  }
-  const int kvh = w.head / a.g;
-  // key tiles of each query tile, and the first that some row does not see whole
-  int n[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int last = min(w.rows, (i + 1) * kM) - 1;
-    n[i] = last >= i * kM ? (max(0, w.limit(last, a.causal)) + kM - 1) / kM : 0;
-  }
-  const int nt = max(n[0], n[1]);
-  const int edge = max(0, w.limit(0, a.causal)) / kM;
+  const int causal = a.causal;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.q_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], kM);
       mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.item_full[i], 1);
+      mbar_init(&sh.item_empty[i], kItemReaders);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 6; ++i) {
       mbar_init(&sh.k_full[i], 1);
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < kEdgeRing; ++i) {
       mbar_init(&sh.go[i], 1);
       mbar_init(&sh.guard[i], kGuardWarps);
     }
     mbar_init(&sh.done, 1);
+    mbar_init(&sh.next_full, 1);
     sh.abort = 0;
     fence_mbarrier_init();
   }
-  if (tid < 16) (&sh.bad[0][0])[tid] = 0;
   if (warp == kMmaWarp) {
     tmem_alloc(&sh.tmem, kTmemCols);
     tmem_relinquish();
@@ -258,45 +283,115 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   const uint32_t tmem = sh.tmem;
   volatile int* abort = &sh.abort;
   int* status = &g_gqa_prefill_status;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort, status); };
+  // The w-th item, in every role but the load warp's: rows == 0 at the end
+  // (or when a wait gave up).  Released when nothing of it is needed any more.
+  auto take = [&](int w) {
+    Item it = {};
+    if (wait(&sh.item_full[w & 1], (w >> 1) & 1)) it = sh.item[w & 1];
+    return it;
+  };
+  auto release = [&](int w) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[w & 1]);
+  };
 
   if (warp >= kMmaWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kLoadWarp) {
-    // ---------------------------------------------------------------- loads
-    if (lane == 0 && nt > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      // -------------------------------------------------------------- loads
       const bool withhold = g_gqa_prefill_test_stall != 0;
+      int nk = 0, nv = 0, nq[2] = {0, 0}, ge = 0, asks = 0;  // chunks of K, tiles of V, Q tiles, edge tiles, asks so far
+      bool ok = true;
+      auto load_k = [&](const Item& it, int kvh, int j) {
+        for (int c = 0; c < kChunksQ && ok; ++c, ++nk) {
+          const int st = nk % kSlotsK;
+          if (nk >= kSlotsK && !(ok = wait(&sh.k_empty[st], (nk / kSlotsK - 1) & 1))) return;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&sh.k_full[st], kChunk);
+            tma_load_3d(k_s + st * kChunk, &tk, c * 64, kvh, it.k0 + j * kM, &sh.k_full[st]);
+          }
+        }
+      };
+      int id = blockIdx.x;
+      for (int w = 0; ok; ) {
+        // the item's sequence: the last i with cu_i / 256 + i <= tile, 32 at a time
+        Item it = {};
+        if (id >= 0) {
+          const int group = id / (a.tiles * a.group_heads), in_group = id - group * (a.tiles * a.group_heads);
+          const int heads = min(a.group_heads, a.h_q - group * a.group_heads);
+          const int tile = a.tiles - 1 - in_group / heads;
+          auto cq = [&](int i) { return min(max(__ldg(a.cu_q + i), 0), a.total_q); };
+          int lo = 0, n = a.b;  // it is one of lo .. lo + n - 1
+          while (n > 1) {
+            const int step = (n + 31) / 32;
+            const int i = lo + lane * step;
+            const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && (lane == 0 || cq(i) / kQueries + i <= tile));
+            const int k = __popc(below) - 1;
+            lo += k * step;
+            n = min(step, n - k * step);
+          }
+          const int q_lo = cq(lo), n_q = max(0, cq(lo + 1) - q_lo);
+          const int t0 = (tile - (q_lo / kQueries + lo)) * kQueries;
+          if (t0 >= 0 && t0 < n_q) {  // (t0 < 0: offsets that do not ascend)
+            it.head = group * a.group_heads + in_group % heads;
+            it.q0 = q_lo + t0;
+            it.rows = min(kQueries, n_q - t0);
+            it.k0 = min(max(__ldg(a.cu_k + lo), 0), a.total_k);
+            it.n_k = max(0, min(__ldg(a.cu_k + lo + 1), a.total_k) - it.k0);
+            it.see = t0 + it.n_k - n_q + 1;
+          }
+        }
+        if (id >= 0 && lane == 0) {  // the next one's number, while this one is loaded
+          fence_proxy_async_smem();  // the last answer is read
+          mbar_arrive_expect_tx(&sh.next_full, 16);
+          ask_next(smem_u32(sh.next), &sh.next_full);
+        }
+        const bool asked = id >= 0;
+        if (it.rows > 0 || !asked) {  // an item, or the end
+          if (w >= 2 && !(ok = wait(&sh.item_empty[w & 1], ((w >> 1) - 1) & 1))) break;
+          if (lane < 16) (&sh.bad[w & 1][0][0])[lane] = 0;
+          __syncwarp();
+          if (lane == 0) {
+            sh.item[w & 1] = it;
+            mbar_arrive(&sh.item_full[w & 1]);
+          }
+          __syncwarp();
+          ++w;
+          if (!asked) break;
+          const int n0 = it.tiles(0, causal), n1 = it.tiles(1, causal), nt = max(n0, n1), edge = it.edge(causal);
+          const int kvh = it.head / a.g;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (n[i] == 0) continue;
-        if (withhold && i == 0) continue;
-        mbar_arrive_expect_tx(&sh.q_full[i], C::kQ / 2);
-        for (int c = 0; c < DQK / 64; ++c)
-          tma_load_3d(q_s + i * (C::kQ / 2) + c * kChunk, &tq, c * 64, w.head, w.q0 + i * kM, &sh.q_full[i]);
-      }
-      int nk = 0, nv = 0;  // tiles issued
-      auto load_k = [&]() {
-        const int st = nk % kStagesK;
-        if (nk >= kStagesK && !mbar_wait(&sh.k_empty[st], (nk / kStagesK - 1) & 1, abort, status)) return false;
-        mbar_arrive_expect_tx(&sh.k_full[st], C::kK);
-        for (int c = 0; c < DQK / 64; ++c)
-          tma_load_3d(k_s + st * C::kK + c * kChunk, &tk, c * 64, kvh, w.k0 + nk * kM, &sh.k_full[st]);
-        ++nk;
-        return true;
-      };
-      auto load_v = [&]() {
-        const int st = nv % kStagesV;
-        if (nv >= kStagesV && !mbar_wait(&sh.v_empty[st], (nv / kStagesV - 1) & 1, abort, status)) return false;
-        mbar_arrive_expect_tx(&sh.v_full[st], C::kV);
-        for (int c = 0; c < DV / 64; ++c)
-          tma_load_3d(v_s + st * C::kV + c * kChunk, &tv, c * 64, kvh, w.k0 + nv * kM, &sh.v_full[st]);
-        if (nv >= edge) mbar_arrive(&sh.go[nv - edge]);
-        ++nv;
-        return true;
-      };
-      bool ok = load_k();
-      while (ok && nv < nt) {  // in the order of use: K_0 K_1 V_0 K_2 V_1 ...
-        if (nk < nt) ok = load_k();
-        if (ok) ok = load_v();
+          for (int i = 0; i < 2; ++i) {
+            if ((i ? n1 : n0) == 0) continue;
+            if (nq[i] > 0 && !(ok = wait(&sh.q_empty[i], (nq[i] - 1) & 1))) break;
+            if (lane == 0 && !(withhold && i == 0)) {
+              mbar_arrive_expect_tx(&sh.q_full[i], C::kQ / 2);
+              for (int c = 0; c < kChunksQ; ++c)
+                tma_load_3d(q_s + i * (C::kQ / 2) + c * kChunk, &tq, c * 64, it.head, it.q0 + i * kM, &sh.q_full[i]);
+            }
+            ++nq[i];
+          }
+          if (nt > 0 && ok) load_k(it, kvh, 0);
+          for (int j = 0; j < nt && ok; ++j) {  // in the order of use: K_0 V_0 K_1 V_1 ...
+            const int st = nv % kStagesV;
+            if (nv >= kStagesV && !(ok = wait(&sh.v_empty[st], (nv / kStagesV - 1) & 1))) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&sh.v_full[st], C::kV);
+              for (int c = 0; c < DV / 64; ++c)
+                tma_load_3d(v_s + st * C::kV + c * kChunk, &tv, c * 64, kvh, it.k0 + j * kM, &sh.v_full[st]);
+              if (j >= edge) mbar_arrive(&sh.go[ge % kEdgeRing]);
+            }
+            if (j >= edge) ++ge;
+            ++nv;
+            if (j + 1 < nt) load_k(it, kvh, j + 1);
+          }
+          if (!ok) break;
+        }
+        if (!(ok = wait(&sh.next_full, asks & 1))) break;
+        ++asks;
+        id = read_next(smem_u32(sh.next));
+        __syncwarp();
       }
       if (*abort) {  // what is in flight lands (or its wait runs out) before the CTA's shared memory goes
         auto land = [&](uint64_t* bar, uint32_t parity) {
@@ -304,123 +399,170 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           while (!mbar_try_wait(smem_u32(bar), parity, 1000u) && clock64() - t < kWaitLimitCycles) {
           }
         };
-        for (int x = max(0, nk - kStagesK); x < nk; ++x) land(&sh.k_full[x % kStagesK], (x / kStagesK) & 1);
+        for (int x = max(0, nk - kSlotsK); x < nk; ++x) land(&sh.k_full[x % kSlotsK], (x / kSlotsK) & 1);
         for (int x = max(0, nv - kStagesV); x < nv; ++x) land(&sh.v_full[x % kStagesV], (x / kStagesV) & 1);
         for (int i = 0; i < 2; ++i)
-          if (n[i] && !(withhold && i == 0)) land(&sh.q_full[i], 0);
+          if (nq[i] && !(withhold && i == 0)) land(&sh.q_full[i], (nq[i] - 1) & 1);
+        land(&sh.next_full, asks & 1);
       }
-    }
-  } else if (warp >= kGuardWarp) {
-    // ---------------------------------------------------------------- guard
-    for (int j = edge; j < nt; ++j) {
-      const int sv = j % kStagesV;
-      // `go`: the tile's load is on its way, so its stage's phase is this one
-      // (a parity alone does not tell it from the one before the last)
-      if (!mbar_wait(&sh.go[j - edge], 0, abort, status)) break;
-      if (!mbar_wait(&sh.v_full[sv], (j / kStagesV) & 1, abort, status)) break;
-      const int end = w.n_k - j * kM;                                      // rows from here on are no keys of ours
-      const int from = max(0, w.limit(0, a.causal) - j * kM);              // rows before it are seen by all
-      // A guard takes every second eight rows; eight loads at once (one by one
-      // this took 3 us of every edge tile).
-      uint8_t* tile = smem + C::kQ + kStagesK * C::kK + sv * C::kV + (lane & 7) * 16;
-      constexpr int kDeep = 8;
-      for (int c = 0; c < DV / 64; ++c) {
-        for (int r0 = (from & ~7) + (warp - kGuardWarp) * 4 + (lane >> 3); r0 < kM; r0 += kDeep * 8) {
-          uint4 x[kDeep];
-          uint32_t any = 0;
+    } else if (warp >= kGuardWarp) {
+      // -------------------------------------------------------------- guards
+      int nv = 0, ge = 0;
+      bool ok = true;
+      for (int w = 0; ok; ++w) {
+        const Item it = take(w);
+        if (it.rows == 0) break;
+        const int nt = max(it.tiles(0, causal), it.tiles(1, causal)), edge = it.edge(causal);
+        for (int j = edge; j < nt; ++j, ++ge) {
+          const int x = nv + j, sv = x % kStagesV;
+          // `go`: the tile's load is on its way, so its stage's phase is this one
+          // (a parity alone does not tell it from the one before the last)
+          if (!(ok = wait(&sh.go[ge % kEdgeRing], (ge / kEdgeRing) & 1))) break;
+          if (!(ok = wait(&sh.v_full[sv], (x / kStagesV) & 1))) break;
+          const int end = it.n_k - j * kM;                           // rows from here on are no keys of ours
+          const int from = max(0, it.limit(0, causal) - j * kM);     // rows before it are seen by all
+          // A guard takes every second four rows; four loads at once (one by
+          // one this took 3 us of every edge tile).
+          uint8_t* tile = smem + C::kQ + kSlotsK * kChunk + sv * C::kV + (lane & 7) * 16;
+          constexpr int kDeep = 4;
+          for (int c = 0; c < DV / 64; ++c) {
+            for (int r0 = (from & ~7) + (warp - kGuardWarp) * 4 + (lane >> 3); r0 < kM; r0 += kDeep * 8) {
+              uint4 v[kDeep];
+              uint32_t any = 0;
 #pragma unroll
-          for (int i = 0; i < kDeep; ++i) {
-            const int r = r0 + i * 8;
-            x[i] = r < end && r < kM ? *reinterpret_cast<const uint4*>(tile + c * kChunk + r * 128) : make_uint4(0, 0, 0, 0);
-          }
+              for (int i = 0; i < kDeep; ++i) {
+                const int r = r0 + i * 8;
+                v[i] = r < end && r < kM ? *reinterpret_cast<const uint4*>(tile + c * kChunk + r * 128) : make_uint4(0, 0, 0, 0);
+              }
 #pragma unroll
-          for (int i = 0; i < kDeep; ++i)
-            any |= maybe_not_finite<T>(x[i].x) | maybe_not_finite<T>(x[i].y) | maybe_not_finite<T>(x[i].z) |
-                   maybe_not_finite<T>(x[i].w);
-          if (any & 0x80008000u) {
+              for (int i = 0; i < kDeep; ++i)
+                any |= maybe_not_finite<T>(v[i].x) | maybe_not_finite<T>(v[i].y) | maybe_not_finite<T>(v[i].z) |
+                       maybe_not_finite<T>(v[i].w);
+              if (any & 0x80008000u) {
 #pragma unroll
-            for (int i = 0; i < kDeep; ++i) {
-              const int r = r0 + i * 8;
-              const uint4 m = make_uint4(not_finite<T>(x[i].x), not_finite<T>(x[i].y), not_finite<T>(x[i].z), not_finite<T>(x[i].w));
-              if (r >= from && (m.x | m.y | m.z | m.w)) {
-                *reinterpret_cast<uint4*>(tile + c * kChunk + r * 128) =
-                    make_uint4(x[i].x & ~m.x, x[i].y & ~m.y, x[i].z & ~m.z, x[i].w & ~m.w);
-                atomicOr(&sh.bad[j - edge][r >> 5], 1u << (r & 31));
+                for (int i = 0; i < kDeep; ++i) {
+                  const int r = r0 + i * 8;
+                  const uint4 m = make_uint4(not_finite<T>(v[i].x), not_finite<T>(v[i].y), not_finite<T>(v[i].z),
+                                             not_finite<T>(v[i].w));
+                  if (r >= from && (m.x | m.y | m.z | m.w)) {
+                    *reinterpret_cast<uint4*>(tile + c * kChunk + r * 128) =
+                        make_uint4(v[i].x & ~m.x, v[i].y & ~m.y, v[i].z & ~m.z, v[i].w & ~m.w);
+                    atomicOr(&sh.bad[w & 1][j - edge][r >> 5], 1u << (r & 31));
+                  }
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < kDeep; ++i) {
+                const int r = r0 + i * 8;
+                if (r >= end && r < kM) *reinterpret_cast<uint4*>(tile + c * kChunk + r * 128) = make_uint4(0, 0, 0, 0);
               }
             }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.guard[ge % kEdgeRing]);
+        }
+        nv += nt;
+        release(w);
+      }
+    } else {
+      // -------------------------------------------------------------- MMAs
+      constexpr uint32_t idesc_s = idesc_of<T>(kM, false), idesc_o = idesc_of<T>(DV, true);
+      int nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ge = 0;
+      bool ok = true;
+      // Descriptors are made where they are used: hoisted out of the loops, they
+      // would fill the registers many times over.
+      auto here = [](uint32_t x) {
+        asm volatile("" : "+r"(x));
+        return x;
+      };
+      // The K chunks from nk on have landed.  (Even a wait that is over takes
+      // 120 cycles: none but P's stands between a softmax and its MMAs.)
+      auto keys = [&]() {
 #pragma unroll
-          for (int i = 0; i < kDeep; ++i) {
-            const int r = r0 + i * 8;
-            if (r >= end && r < kM) *reinterpret_cast<uint4*>(tile + c * kChunk + r * 128) = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < kChunksQ && ok; ++c) ok = wait(&sh.k_full[(nk + c) % kSlotsK], ((nk + c) / kSlotsK) & 1);
+      };
+      // S_i = Q_i K^T from the K chunks from nk on; `last`: they are released
+      auto scores = [&](int i, bool last) {
+#pragma unroll
+        for (int c = 0; c < kChunksQ; ++c) {
+          const int st = (nk + c) % kSlotsK;
+          const uint32_t q_at = here(q_s + i * (C::kQ / 2) + c * kChunk), k_at = here(k_s + st * kChunk);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16_ss(tmem + i * kM, sdesc_sw128(q_at + kk * 32, 16, 1024), sdesc_sw128(k_at + kk * 32, 16, 1024),
+                           idesc_s, (c | kk) != 0);
+            if (last) umma_commit(&sh.k_empty[st]);
+            if (c == kChunksQ - 1) umma_commit(&sh.s_full[i]);
           }
+          __syncwarp();
+        }
+      };
+      auto values = [&](int i, int sv, bool first) {  // O_i += P_i V
+        const uint32_t v_at = here(v_s + sv * C::kV);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kM / 16; ++kk)
+            umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8, sdesc_sw128(v_at + kk * 2048, kChunk, 1024), idesc_o,
+                    !(first && kk == 0));
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
+      };
+      for (int w = 0; ok; ++w) {
+        const Item it = take(w);
+        if (it.rows == 0) break;
+        const int n[2] = {it.tiles(0, causal), it.tiles(1, causal)}, nt = max(n[0], n[1]), edge = it.edge(causal);
+        release(w);
+        if (nt == 0) continue;
+        keys();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!ok || n[i] == 0) continue;
+          if (!(ok = wait(&sh.q_full[i], nq[i] & 1))) continue;
+          ++nq[i];
+          scores(i, i == 1 || n[1] == 0);
+          if (n[i] == 1) commit(&sh.q_empty[i]);
+        }
+        nk += kChunksQ;
+        for (int j = 0; j < nt && ok; ++j) {
+          const int sv = nv % kStagesV;
+          ok = wait(&sh.v_full[sv], (nv / kStagesV) & 1);
+          if (ok && j >= edge) {
+            ok = wait(&sh.guard[ge % kEdgeRing], (ge / kEdgeRing) & 1);
+            ++ge;
+          }
+          if (ok && j + 1 < nt) keys();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!ok || j >= n[i]) continue;
+            if (!(ok = wait(&sh.p_full[i], np[i] & 1))) continue;
+            ++np[i];
+            tc_fence_after();
+            values(i, sv, j == 0);
+            if (j + 1 < n[i]) {
+              scores(i, i == 1 || j + 1 >= n[1]);
+              if (j + 2 == n[i]) commit(&sh.q_empty[i]);
+            } else {
+              commit(&sh.o_full[i]);
+            }
+          }
+          if (!ok) break;
+          commit(&sh.v_empty[sv]);
+          ++nv;
+          if (j + 1 < nt) nk += kChunksQ;
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.guard[j - edge]);
-    }
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMAs
-    constexpr uint32_t idesc_s = idesc_of<T>(kM, false), idesc_o = idesc_of<T>(DV, true);
-    auto scores = [&](int i, int sk) {  // S_i = Q_i K^T
-      if (elect_one()) {
-#pragma unroll
-        for (int c = 0; c < DQK / 64; ++c)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_bf16_ss(tmem + i * kM, sdesc_sw128(q_s + i * (C::kQ / 2) + c * kChunk + kk * 32, 16, 1024),
-                         sdesc_sw128(k_s + sk * C::kK + c * kChunk + kk * 32, 16, 1024), idesc_s, (c | kk) != 0);
-        umma_commit(&sh.s_full[i]);
-      }
-      __syncwarp();
-    };
-    auto values = [&](int i, int sv, bool first) {  // O_i += P_i V
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < kM / 16; ++kk)
-          umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8,
-                  sdesc_sw128(v_s + sv * C::kV + kk * 2048, kChunk, 1024), idesc_o, !(first && kk == 0));
-      }
-      __syncwarp();
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
-    bool ok = true;
-    for (int i = 0; i < 2 && ok; ++i)
-      if (n[i]) ok = mbar_wait(&sh.q_full[i], 0, abort, status);
-    if (nt > 0 && ok && (ok = mbar_wait(&sh.k_full[0], 0, abort, status))) {
-      for (int i = 0; i < 2; ++i)
-        if (n[i]) scores(i, 0);
-      commit(&sh.k_empty[0]);
-      for (int j = 0; j < nt && ok; ++j) {
-        const int sv = j % kStagesV, sk = (j + 1) % kStagesK;
-        ok = mbar_wait(&sh.v_full[sv], (j / kStagesV) & 1, abort, status);
-        if (ok && j >= edge) ok = mbar_wait(&sh.guard[j - edge], 0, abort, status);
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= n[i]) continue;
-          if (!(ok = mbar_wait(&sh.p_full[i], j & 1, abort, status))) break;
-          tc_fence_after();
-          values(i, sv, j == 0);
-          if (j + 1 < n[i]) {
-            if (!(ok = mbar_wait(&sh.k_full[sk], ((j + 1) / kStagesK) & 1, abort, status))) break;
-            scores(i, sk);
-          } else {
-            commit(&sh.o_full[i]);
-          }
-        }
-        commit(&sh.v_empty[sv]);
-        if (j + 1 < nt) commit(&sh.k_empty[sk]);
+      // every MMA has completed before TMEM is freed
+      commit(&sh.done);
+      const long long t = clock64();
+      while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
       }
     }
-    // every MMA has completed before TMEM is freed
-    commit(&sh.done);
-    const long long t = clock64();
-    while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
-    }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------------------------------------------------------- softmax
@@ -428,84 +570,112 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int r = i * kM + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem + lanes + i * kM, o_t = tmem + lanes + 256 + i * DV;
-    const int lim = w.limit(r, a.causal), lim0 = w.limit(i * kM, a.causal);
-    const int mine = n[i];
     const float c = a.scale_log2;
-    float m = -INFINITY, l = 0.f;
+    int ns = 0, no = 0, ge = 0;  // S tiles, items with any, edge tiles so far
     bool ok = true;
-    for (int j = 0; j < mine; ++j) {
-      if (!(ok = mbar_wait(&sh.s_full[i], j & 1, abort, status))) break;
-      tc_fence_after();
-      float s[kM];
+    for (int w = 0; ok; ++w) {
+      const Item it = take(w);
+      if (it.rows == 0) break;
+      const int mine = it.tiles(i, causal), nt = max(it.tiles(0, causal), it.tiles(1, causal)), edge = it.edge(causal);
+      const int lim = it.limit(r, causal), lim0 = it.limit(i * kM, causal);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < mine; ++j, ++ns) {
+        if (!(ok = wait(&sh.s_full[i], ns & 1))) break;
+        tc_fence_after();
+        float s[kM];
 #pragma unroll
-      for (int x = 0; x < kM; x += 32) tmem_ld32(s_t + x, *reinterpret_cast<float(*)[32]>(&s[x]));
-      tc_wait_ld();
-      if (j * kM + kM > lim0) {
-        const int left = lim - j * kM;
+        for (int x = 0; x < kM; x += 32) tmem_ld32(s_t + x, *reinterpret_cast<float(*)[32]>(&s[x]));
+        tc_wait_ld();
+        // 32 columns at a time: those that some row of the warp does not see are
+        // masked, and from `seen` on no row of it sees any
+        int seen = kM;
+        if (j * kM + kM > lim0) {
+          const int left = lim - j * kM, least = __shfl_sync(0xffffffffu, left, 0);
+          seen = __shfl_sync(0xffffffffu, left, 31);
 #pragma unroll
-        for (int x = 0; x < kM; ++x) s[x] = x < left ? s[x] : -INFINITY;
-      }
-      float t[4] = {s[0], s[1], s[2], s[3]};
+          for (int x = 0; x < kM; x += 32) {
+            if (x + 32 > least) {
 #pragma unroll
-      for (int x = 4; x + 8 <= kM; x += 8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = max3(t[e], s[x + 2 * e], s[x + 2 * e + 1]);
-      }
-      t[0] = max3(t[0], s[kM - 4], s[kM - 3]);
-      t[1] = max3(t[1], s[kM - 2], s[kM - 1]);
-      const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
-      const bool grew = (top - m) * c > kRescale;  // from -inf: always
-      if (__any_sync(0xffffffffu, grew)) {
-        const float f = grew ? fast_exp2((m - top) * c) : 1.f;
-        if (grew) m = top;
-        l *= f;
-        if (j > 0) {  // the MMAs of the tile before are complete: this tile's S came after them
-#pragma unroll
-          for (int x = 0; x < DV; x += 32) {
-            float o[32];
-            tmem_ld32(o_t + x, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_st32(o_t + x, o);
+              for (int e = 0; e < 32; ++e) s[x + e] = x + e < left ? s[x + e] : -INFINITY;
+            }
           }
         }
-      }
-      const float mc = m == -INFINITY ? 0.f : -m * c;
-      const uint64_t cc = pair(c, c), mm = pair(mc, mc);
-      uint64_t l2[2] = {0, 0};  // two pairs of zeros
+        float t[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int x = 0; x < kM; x += 32) {
-        float p[16];
+        for (int x = 4; x + 8 <= kM; x += 8) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 u = unpair(fma2(pair(s[x + 2 * e], s[x + 2 * e + 1]), cc, mm));
-          u.x = fast_exp2(u.x);
-          u.y = fast_exp2(u.y);
-          l2[e & 1] = add2(l2[e & 1], pair(u.x, u.y));
-          p[e] = __uint_as_float(pack16<T>(u.x, u.y));
+          for (int e = 0; e < 4; ++e) t[e] = max3(t[e], s[x + 2 * e], s[x + 2 * e + 1]);
         }
-        tmem_st16(s_t + x / 2, p);
+        t[0] = max3(t[0], s[kM - 4], s[kM - 3]);
+        t[1] = max3(t[1], s[kM - 2], s[kM - 1]);
+        const float top = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+        const bool grew = (top - m) * c > kRescale;  // from -inf: always
+        if (__any_sync(0xffffffffu, grew)) {
+          const float f = grew ? fast_exp2((m - top) * c) : 1.f;
+          if (grew) m = top;
+          l *= f;
+          if (j > 0) {  // the MMAs of the tile before are complete: this tile's S came after them
+#pragma unroll
+            for (int x = 0; x < DV; x += 16) {  // (beside S's 128 registers)
+              float o[16];
+              tmem_ld16(o_t + x, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= f;
+              tmem_st16(o_t + x, o);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : -m * c;
+        const uint64_t cc = pair(c, c), mm = pair(mc, mc);
+        uint64_t l2[2] = {0, 0};  // two pairs of zeros
+#pragma unroll
+        for (int x = 0; x < kM; x += 32) {
+          float p[16];
+          if (x >= seen) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = 0.f;
+            tmem_st16(s_t + x / 2, p);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 u = unpair(fma2(pair(s[x + 2 * e], s[x + 2 * e + 1]), cc, mm));
+            u.x = fast_exp2(u.x);
+            u.y = fast_exp2(u.y);
+            l2[e & 1] = add2(l2[e & 1], pair(u.x, u.y));
+            p[e] = __uint_as_float(pack16<T>(u.x, u.y));
+          }
+          tmem_st16(s_t + x / 2, p);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_full[i]);
+        const float2 sum = unpair(add2(l2[0], l2[1]));
+        l += sum.x + sum.y;
       }
-      const float2 sum = unpair(add2(l2[0], l2[1]));
-      l += sum.x + sum.y;
-      tc_wait_st();
-      tc_fence_before();
-      mbar_arrive(&sh.p_full[i]);
-    }
-    if (mine > 0 && ok) ok = mbar_wait(&sh.o_full[i], 0, abort, status);
-    // rows of V that were kept out of the products, for those who see them
-    bool bad = false;
-    for (int j = edge; j < mine && ok; ++j) {
-      ok = mbar_wait(&sh.guard[j - edge], 0, abort, status);
-      bad |= (sh.bad[j - edge][0] | sh.bad[j - edge][1] | sh.bad[j - edge][2] | sh.bad[j - edge][3]) != 0;
-    }
-    tc_fence_after();
-    const bool live = r < w.rows;
-    const bool none = lim <= 0;
-    if (ok) {
+      if (!ok) break;
+      if (mine > 0) {
+        if (!(ok = wait(&sh.o_full[i], no & 1))) break;
+        ++no;
+      }
+      // rows of V that were kept out of the products, for those who see them
+      bool bad = false;
+      for (int j = edge; j < mine && ok; ++j) {
+        const int x = ge + j - edge;
+        ok = wait(&sh.guard[x % kEdgeRing], (x / kEdgeRing) & 1);
+        const uint32_t* b = sh.bad[w & 1][j - edge];
+        bad |= (b[0] | b[1] | b[2] | b[3]) != 0;
+      }
+      if (!ok) break;
+      ge += max(0, nt - edge);
+      tc_fence_after();
+      const bool live = r < it.rows;
+      const bool none = lim <= 0;
       const float inv = 1.f / l;
-      T* out = static_cast<T*>(a.out) + (int64_t)(w.q0 + r) * a.stride_o_t + (int64_t)w.head * a.stride_o_h;
+      // whole 32-byte sectors where every row starts on one
+      const bool wide = ((reinterpret_cast<uintptr_t>(a.out) & 31) | ((a.stride_o_t | a.stride_o_h) & 15)) == 0;
+      T* out = static_cast<T*>(a.out) + (int64_t)(it.q0 + r) * a.stride_o_t + (int64_t)it.head * a.stride_o_h;
 #pragma unroll
       for (int x = 0; x < DV; x += 32) {
         float o[32];
@@ -518,11 +688,11 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         if (bad) {
           for (int j = edge; j < mine; ++j)
             for (int k = 0; k < 4; ++k)
-              for (uint32_t bits = sh.bad[j - edge][k]; bits; bits &= bits - 1) {
+              for (uint32_t bits = sh.bad[w & 1][j - edge][k]; bits; bits &= bits - 1) {
                 const int t = j * kM + k * 32 + __ffs(bits) - 1;
                 if (t >= lim) continue;
-                const T* v = static_cast<const T*>(a.v) + (int64_t)(w.k0 + t) * a.stride_v_t +
-                             (int64_t)kvh * a.stride_v_h + x;
+                const T* v = static_cast<const T*>(a.v) + (int64_t)(it.k0 + t) * a.stride_v_t +
+                             (int64_t)(it.head / a.g) * a.stride_v_h + x;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   const float f = static_cast<float>(v[e]);
@@ -532,13 +702,22 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         }
         if (live) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            *reinterpret_cast<uint4*>(out + x + e) = make_uint4(pack16<T>(o[e], o[e + 1]), pack16<T>(o[e + 2], o[e + 3]),
-                                                               pack16<T>(o[e + 4], o[e + 5]), pack16<T>(o[e + 6], o[e + 7]));
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = pack16<T>(o[e + 2 * k], o[e + 2 * k + 1]);
+            if (wide) {
+              store_32(out + x + e, v);
+            } else {
+              *reinterpret_cast<uint4*>(out + x + e) = make_uint4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<uint4*>(out + x + e + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+            }
           }
         }
       }
-      if (live) a.lse[(int64_t)(w.q0 + r) * a.h_q + w.head] = none ? -INFINITY : (m * c + log2f(l)) * kLn2;
+      if (live) a.lse[(int64_t)(it.q0 + r) * a.h_q + it.head] = none ? -INFINITY : (m * c + log2f(l)) * kLn2;
+      tc_fence_before();  // O is read before the arrival that lets the next item's MMAs write it
+      release(w);
     }
   }
   tc_fence_before();
@@ -585,6 +764,9 @@ cudaError_t launch(const dsv4b_gqa_prefill_params& p, cudaStream_t stream, int* 
   a.total_q = (int)p.total_q;
   a.total_k = (int)p.total_k;
   a.tiles = (int)p.total_q / kQueries + p.b;
+  const int64_t head_bytes = p.total_k * (DQK + DV) * 2;
+  const int64_t kv_heads = head_bytes > 0 ? kGroupBytes / head_bytes : p.h_kv;
+  a.group_heads = a.g * (int)(kv_heads < 1 ? 1 : kv_heads > p.h_kv ? p.h_kv : kv_heads);
   a.scale_log2 = p.sm_scale * kLog2e;
   a.v = p.v;
   a.stride_v_t = p.stride_v_t;
