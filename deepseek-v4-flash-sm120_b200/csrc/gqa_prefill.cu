@@ -90,14 +90,17 @@ struct PrefillArgs {
   float* lse;
 };
 
-// Ring depths that fit 227 KB beside Q: K in chunks of 64 columns, each
-// released by itself, V in whole tiles (its chunks stay side by side).
+// Ring depths that fit 227 KB beside Q: V in whole tiles (its chunks stay
+// side by side), K too, but where only one and a third of its tiles fit (192
+// columns): in chunks of 64 columns, each released by itself.
 template <int DQK, int DV>
 struct Cfg {
   static constexpr int kChunksQ = DQK / 64;
   static constexpr int kQ = 2 * kChunksQ * kChunk;
   static constexpr int kV = (DV / 64) * kChunk;
-  static constexpr int kSlotsK = DQK == 192 ? 4 : 6;
+  static constexpr int kPartsK = DQK == 192 ? 3 : 1;           // of a K tile
+  static constexpr int kChunksK = kChunksQ / kPartsK;          // chunks of a part
+  static constexpr int kSlotsK = DQK == 192 ? 4 : 6 / kChunksQ;  // parts in the ring
   static constexpr int kStagesV = DQK == 64 ? 6 : 2;
 };
 
@@ -132,7 +135,7 @@ constexpr int kItemReaders = 8 + 1 + 2;  // softmax, MMA and guard warps
 template <int DQK, int DV>
 constexpr int smem_bytes() {
   using C = Cfg<DQK, DV>;
-  return 1024 + C::kQ + C::kSlotsK * kChunk + C::kStagesV * C::kV + (int)sizeof(Shared);
+  return 1024 + C::kQ + C::kSlotsK * C::kChunksK * kChunk + C::kStagesV * C::kV + (int)sizeof(Shared);
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -162,13 +165,26 @@ __device__ __forceinline__ int read_next(uint32_t answer) {
   return r;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem], 16-bit operands, fp32 sums.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem], 16-bit operands, fp32 sums; descriptors as
+// their low words and a common high one.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t high, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(high), "r"(idesc), "r"(accumulate));
+}
+// The same with A from TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t high, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(high), "r"(idesc), "r"(accumulate));
 }
 
 template <typename T>
@@ -241,10 +257,11 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
                    const __grid_constant__ CUtensorMap tv, const PrefillArgs a) {
   using C = Cfg<DQK, DV>;
   constexpr int kSlotsK = C::kSlotsK, kStagesV = C::kStagesV, kChunksQ = C::kChunksQ;
+  constexpr int kPartsK = C::kPartsK, kPart = C::kChunksK * kChunk;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t q_s = smem_u32(smem), k_s = q_s + C::kQ, v_s = k_s + kSlotsK * kChunk;
-  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kQ + kSlotsK * kChunk + kStagesV * C::kV);
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + C::kQ, v_s = k_s + kSlotsK * kPart;
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::kQ + kSlotsK * kPart + kStagesV * C::kV);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int causal = a.causal;
 
@@ -301,15 +318,16 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     if (warp == kLoadWarp) {
       // -------------------------------------------------------------- loads
       const bool withhold = g_gqa_prefill_test_stall != 0;
-      int nk = 0, nv = 0, nq[2] = {0, 0}, ge = 0, asks = 0;  // chunks of K, tiles of V, Q tiles, edge tiles, asks so far
+      int nk = 0, nv = 0, nq[2] = {0, 0}, ge = 0, asks = 0;  // parts of K, tiles of V, Q tiles, edge tiles, asks so far
       bool ok = true;
       auto load_k = [&](const Item& it, int kvh, int j) {
-        for (int c = 0; c < kChunksQ && ok; ++c, ++nk) {
+        for (int x = 0; x < kPartsK && ok; ++x, ++nk) {
           const int st = nk % kSlotsK;
           if (nk >= kSlotsK && !(ok = wait(&sh.k_empty[st], (nk / kSlotsK - 1) & 1))) return;
           if (lane == 0) {
-            mbar_arrive_expect_tx(&sh.k_full[st], kChunk);
-            tma_load_3d(k_s + st * kChunk, &tk, c * 64, kvh, it.k0 + j * kM, &sh.k_full[st]);
+            mbar_arrive_expect_tx(&sh.k_full[st], kPart);
+            for (int c = 0; c < C::kChunksK; ++c)
+              tma_load_3d(k_s + st * kPart + c * kChunk, &tk, (x * C::kChunksK + c) * 64, kvh, it.k0 + j * kM, &sh.k_full[st]);
           }
         }
       };
@@ -423,7 +441,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           const int from = max(0, it.limit(0, causal) - j * kM);     // rows before it are seen by all
           // A guard takes every second four rows; four loads at once (one by
           // one this took 3 us of every edge tile).
-          uint8_t* tile = smem + C::kQ + kSlotsK * kChunk + sv * C::kV + (lane & 7) * 16;
+          uint8_t* tile = smem + C::kQ + kSlotsK * kPart + sv * C::kV + (lane & 7) * 16;
           constexpr int kDeep = 4;
           for (int c = 0; c < DV / 64; ++c) {
             for (int r0 = (from & ~7) + (warp - kGuardWarp) * 4 + (lane >> 3); r0 < kM; r0 += kDeep * 8) {
@@ -470,48 +488,39 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       constexpr uint32_t idesc_s = idesc_of<T>(kM, false), idesc_o = idesc_of<T>(DV, true);
       int nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ge = 0;
       bool ok = true;
-      // Descriptors are made where they are used: hoisted out of the loops, they
-      // would fill the registers many times over.
-      auto here = [](uint32_t x) {
-        asm volatile("" : "+r"(x));
-        return x;
+      // The tensor core holds few MMAs in advance, so what this warp executes
+      // between them is tensor time (8 cycles an MMA of 64 for the commits and
+      // branches alone): a descriptor is a low word, made once for a run of
+      // MMAs and stepped, and one high word for all; one elected region holds
+      // a tile's O and next S.  (`at`: not hoisted out of the loops, where the
+      // descriptors would fill the registers many times over.)
+      constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);  // SBO, version, SWIZZLE_128B
+      auto at = [](uint32_t saddr, uint32_t lbo) {
+        uint32_t lo = ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
+        asm volatile("" : "+r"(lo));
+        return lo;
       };
-      // The K chunks from nk on have landed.  (Even a wait that is over takes
-      // 120 cycles: none but P's stands between a softmax and its MMAs.)
+      // the K parts from nk on have landed
       auto keys = [&]() {
 #pragma unroll
-        for (int c = 0; c < kChunksQ && ok; ++c) ok = wait(&sh.k_full[(nk + c) % kSlotsK], ((nk + c) / kSlotsK) & 1);
+        for (int x = 0; x < kPartsK && ok; ++x) ok = wait(&sh.k_full[(nk + x) % kSlotsK], ((nk + x) / kSlotsK) & 1);
       };
-      // S_i = Q_i K^T from the K chunks from nk on; `last`: they are released
+      // S_i = Q_i K^T from them, by the elected thread; `last`: they are released
       auto scores = [&](int i, bool last) {
 #pragma unroll
-        for (int c = 0; c < kChunksQ; ++c) {
-          const int st = (nk + c) % kSlotsK;
-          const uint32_t q_at = here(q_s + i * (C::kQ / 2) + c * kChunk), k_at = here(k_s + st * kChunk);
-          if (elect_one()) {
+        for (int x = 0; x < kPartsK; ++x) {
+          const int st = (nk + x) % kSlotsK;
+#pragma unroll
+          for (int c = 0; c < C::kChunksK; ++c) {
+            const int chunk = x * C::kChunksK + c;
+            const uint32_t q_at = at(q_s + i * (C::kQ / 2) + chunk * kChunk, 16), k_at = at(k_s + st * kPart + c * kChunk, 16);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_bf16_ss(tmem + i * kM, sdesc_sw128(q_at + kk * 32, 16, 1024), sdesc_sw128(k_at + kk * 32, 16, 1024),
-                           idesc_s, (c | kk) != 0);
-            if (last) umma_commit(&sh.k_empty[st]);
-            if (c == kChunksQ - 1) umma_commit(&sh.s_full[i]);
+              umma_ss(tmem + i * kM, q_at + kk * 2, k_at + kk * 2, kDescHigh, idesc_s, (chunk | kk) != 0);
           }
-          __syncwarp();
+          if (last) umma_commit(&sh.k_empty[st]);
         }
-      };
-      auto values = [&](int i, int sv, bool first) {  // O_i += P_i V
-        const uint32_t v_at = here(v_s + sv * C::kV);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kM / 16; ++kk)
-            umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8, sdesc_sw128(v_at + kk * 2048, kChunk, 1024), idesc_o,
-                    !(first && kk == 0));
-        }
-        __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) umma_commit(bar);
-        __syncwarp();
+        umma_commit(&sh.s_full[i]);
       };
       for (int w = 0; ok; ++w) {
         const Item it = take(w);
@@ -525,11 +534,15 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           if (!ok || n[i] == 0) continue;
           if (!(ok = wait(&sh.q_full[i], nq[i] & 1))) continue;
           ++nq[i];
-          scores(i, i == 1 || n[1] == 0);
-          if (n[i] == 1) commit(&sh.q_empty[i]);
+          if (elect_one()) {
+            scores(i, i == 1 || n[1] == 0);
+            if (n[i] == 1) umma_commit(&sh.q_empty[i]);
+          }
+          __syncwarp();
         }
-        nk += kChunksQ;
+        nk += kPartsK;
         for (int j = 0; j < nt && ok; ++j) {
+          // all that this tile's MMAs need beside P, before P's waits
           const int sv = nv % kStagesV;
           ok = wait(&sh.v_full[sv], (nv / kStagesV) & 1);
           if (ok && j >= edge) {
@@ -543,22 +556,28 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             if (!(ok = wait(&sh.p_full[i], np[i] & 1))) continue;
             ++np[i];
             tc_fence_after();
-            values(i, sv, j == 0);
-            if (j + 1 < n[i]) {
-              scores(i, i == 1 || j + 1 >= n[1]);
-              if (j + 2 == n[i]) commit(&sh.q_empty[i]);
-            } else {
-              commit(&sh.o_full[i]);
+            if (elect_one()) {
+              const uint32_t v_at = at(v_s + sv * C::kV, kChunk);
+#pragma unroll
+              for (int kk = 0; kk < kM / 16; ++kk)  // O_i += P_i V
+                umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8, v_at + kk * 128, kDescHigh, idesc_o, (j | kk) != 0);
+              if (i == 1 || j >= n[1]) umma_commit(&sh.v_empty[sv]);
+              if (j + 1 < n[i]) {
+                scores(i, i == 1 || j + 1 >= n[1]);
+                if (j + 2 == n[i]) umma_commit(&sh.q_empty[i]);
+              } else {
+                umma_commit(&sh.o_full[i]);
+              }
             }
+            __syncwarp();
           }
-          if (!ok) break;
-          commit(&sh.v_empty[sv]);
           ++nv;
-          if (j + 1 < nt) nk += kChunksQ;
+          if (j + 1 < nt) nk += kPartsK;
         }
       }
       // every MMA has completed before TMEM is freed
-      commit(&sh.done);
+      if (elect_one()) umma_commit(&sh.done);
+      __syncwarp();
       const long long t = clock64();
       while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
       }
