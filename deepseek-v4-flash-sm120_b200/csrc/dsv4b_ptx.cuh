@@ -79,6 +79,23 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// The same by all lanes of a warp, with one answer: what follows is the work
+// of them all.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int* err_word) {
+  const uint32_t a = smem_u32(bar);
+  if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+    const bool late = clock64() - t0 > kWaitLimitCycles;
+    if (__any_sync(0xffffffffu, late || *cta_abort)) {
+      *cta_abort = 1;
+      if (late && err_word) atomicOr(err_word, kErrWaitTimeout);
+      return false;
+    }
+  }
+}
+
 // Arrive once on `bar` and add `bytes` to the transaction count the
 // current phase waits for (the bulk copies that complete_tx on it).
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {

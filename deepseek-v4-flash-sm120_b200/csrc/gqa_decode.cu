@@ -694,7 +694,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     bool edge = t0 + kUnit > all || now.held != (1 << kRuns) - 1;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) edge |= now.vs[i] == 0.f;
-    if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+    if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
 
     // s^T: s[mt][n]: positions 16 mt + perm(g) (0, 1) and 8 further (2, 3), rows 2c, 2c + 1
     float s[kRuns][NT][4];
@@ -792,7 +792,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         p[mt][n][1] = transpose8(pack_half(s[mt][n][2], s[mt][n][3]));
       }
     }
-    if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+    if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
     const uint32_t v_tile = ring + slot * kTile;
 #pragma unroll
     for (int mt = 0; mt < kRuns; ++mt) {
@@ -1207,7 +1207,7 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
           const int t = t_mine + 32 * x;
           before[x] = (a.accumulate || n0 > 0) && t < cur.len && t < a.width ? w[32 * x] : 0.f;
         }
-        if (!(ok = mbar_wait(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+        if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
         uint32_t f[ONE ? 1 : kRuns][ONE ? 1 : D / 64][4][4];
         float s[kN][kRuns][4];
         if constexpr (ONE) {

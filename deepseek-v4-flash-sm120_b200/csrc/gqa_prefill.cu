@@ -300,7 +300,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   const uint32_t tmem = sh.tmem;
   volatile int* abort = &sh.abort;
   int* status = &g_gqa_prefill_status;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort, status); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, abort, status); };
   // The w-th item, in every role but the load warp's: rows == 0 at the end
   // (or when a wait gave up).  Released when nothing of it is needed any more.
   auto take = [&](int w) {
