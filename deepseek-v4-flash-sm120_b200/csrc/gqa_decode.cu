@@ -531,7 +531,7 @@ __device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML 
     *reinterpret_cast<float4*>(part->o + e) = o;
     return;
   }
-  const bool none = m == -INFINITY;
+  const bool none = l == 0.f;  // (not by m: a row of NaN scores has none, and is NaN)
   const float inv = none ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) =
       make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
@@ -894,7 +894,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int row = 8 * n + 2 * c + k, r = r0 + row;
-          const bool none = m[n][k] == -INFINITY;
+          const bool none = l[n][k] == 0.f;
           const float f = whole ? (none ? 0.f : v_unit / l[n][k]) : v_unit;
           float v[2 * kSteps];
 #pragma unroll

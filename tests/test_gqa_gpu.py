@@ -161,6 +161,24 @@ def test_prefill_many_sequences():
     check_prefill(q, k, v, packed(lens), None, True)
 
 
+def test_prefill_offsets_past_32_bits():
+    """q, k, v and out of more than 2^31 elements: 90,000 tokens of 128 heads
+    of 192, in sequences of 200 (the last one looked at, and one in between)."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n, h, step = 90_000, 128, 200
+    q = torch.randn(n, h, 192, generator=g, device="cuda", dtype=torch.bfloat16)
+    k = torch.randn(n, h, 192, generator=g, device="cuda", dtype=torch.bfloat16)
+    v = torch.randn(n, h, 192, generator=g, device="cuda", dtype=torch.bfloat16)[..., 64:]
+    cu = torch.arange(0, n + 1, step, dtype=torch.int32, device="cuda")
+    out = torch.empty(n, h, 192, device="cuda", dtype=torch.bfloat16)[..., :128]
+    got, lse = dk.gqa_prefill_fwd(q, k, v, cu, out=out)
+    for at in (87_400, n - step):
+        part = [t[at:at + step, 125:].contiguous() for t in (q, k, v)]
+        one, one_lse = check_prefill(*part, [0, step], None, True)
+        assert torch.equal(got[at:at + step, 125:], one) and torch.equal(lse[at:at + step, 125:], one_lse)
+
+
 # ------------------------------------------------------------------ the cache
 class Cache:
     """Random pages for sequences of the given lengths; rows that hold no
@@ -309,6 +327,59 @@ def test_decode_nan_is_seen_only_by_those_who_see_it():
     c.kc[blk, 43 % 32, 0, 0] = 0xFF
     out, _ = check_decode(c, rand(g, 2, 3, 4, 128))
     assert torch.isfinite(out[0, 0]).all() and torch.isfinite(out[1, 0]).all() and torch.isnan(out[0, 2]).any()
+
+
+@pytest.mark.parametrize("lens", [[1, 40], [3000, 200]])
+def test_decode_nan_queries(lens):
+    """A query whose scores are all NaN gets NaN, its neighbours in the tile nothing of it."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    c = Cache(lens, 64, 1, 128, seed=10)
+    q = rand(g, 2, 1, 6, 128)
+    q[0, 0, 1, 7], q[1, 0, 4, 100] = float("nan"), float("inf")
+    out, lse = check_decode(c, q)
+    assert torch.isnan(out[0, 0, 1]).all() and torch.isnan(lse[0, 1, 0]) and int(torch.isnan(out).any(-1).sum()) == 2
+
+
+def test_decode_and_weights_far_into_a_pool():
+    """Blocks whose bytes lie past 2^32 of the pool, the tensors' strides included."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(14)
+    c = Cache([200, 100], 64, 2, 128, seed=11, spare=0)
+    used, far = c.kc.shape[0], 300_000  # of 16 KB
+    big = [torch.empty(far + used, 64, 2, 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.empty(far + used, 2, device="cuda") for _ in range(2)]
+    for t, x in zip(big + scales, (c.kc, c.vc, c.ks, c.vs)):
+        t[far:] = x.cuda()
+    table = torch.where(c.table >= 0, c.table + far, c.table).cuda()
+    q, near = rand(g, 2, 2, 8, 128), c.cuda()
+    res = []
+    for kc, vc, ks, vs, tab in ((*near[:4], near[4]), (*big, *scales, table)):
+        o, lse = dk.gqa_decode_fwd(q, kc, vc, ks, vs, tab, near[5])
+        res.append((o, lse, dk.gqa_attention_weights(q, lse, kc, ks, tab, near[5])))
+    for x, y in zip(*res):
+        assert torch.equal(x, y)
+    # and written there
+    k, v = rand(g, 70, 2, 128), rand(g, 70, 2, 128)
+    cu, ctx = torch.tensor([0, 10, 70], dtype=torch.int32, device="cuda"), torch.tensor([200, 100], dtype=torch.int32, device="cuda")
+    dk.gqa_cache_append(k, v, cu, ctx, near[4], *near[:4])
+    dk.gqa_cache_append(k, v, cu, ctx, table, *big, *scales)
+    new = torch.tensor([[0, far - 2], [far - 1, 7]], dtype=torch.int32, device="cuda")
+    w = res[0][2]
+    small = [torch.cat([t, torch.zeros_like(t[:4])]) for t in (x.view(torch.uint8) if x.element_size() == 1 else x for x in near[:4])]
+    new_near = torch.arange(used, used + 4, dtype=torch.int32, device="cuda").view(2, 2)
+    got = dk.gqa_cache_evict(*big, *scales, table, near[5], w, 90, 20, new)
+    want = dk.gqa_cache_evict(*small, near[4], near[5], w, 90, 20, new_near)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    for t, x, y in zip(big + scales, small, near[:4]):
+        y = y.view(torch.uint8) if y.element_size() == 1 else y
+        assert torch.equal(t[far:].view(torch.uint8), y.view(torch.uint8))
+        for i in range(2):
+            a, b = t[new[i].long()].flatten(0, 1), x[new_near[i].long()].flatten(0, 1)
+            n = 90 if t.dim() == 4 else len(a)
+            assert torch.equal(a[:n].view(torch.uint8), b[:n].view(torch.uint8))
+    torch.cuda.synchronize()
+    assert status() == 0
 
 
 # ------------------------------------------------------------------ weights
@@ -600,3 +671,167 @@ def test_graph_streams_and_two_at_once():
             assert torch.equal(got, want)
     torch.cuda.synchronize()
     assert status() == 0
+
+
+def test_the_same_call_twice():
+    """Bit for bit: no sum's order depends on who comes first."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(31)
+    c = Cache([9000, 40, 333], 64, 2, 128, seed=4, spare=20)
+    dev, q = c.cuda(), rand(g, 3, 2, 8, 128)
+    x, kv = rand(g, 1000, 8, 128), rand(g, 1000, 2, 128)
+    cu = torch.tensor([0, 900, 1000, 1000], dtype=torch.int32, device="cuda")
+    new = c.free[:12].int().view(3, 4).cuda()
+
+    def run():
+        o, lse = dk.gqa_decode_fwd(q, *dev)
+        w = dk.gqa_attention_weights(q, lse, dev[0], dev[2], dev[4], dev[5])
+        return (o, lse, w) + dk.gqa_prefill_fwd(x, kv, kv, cu) + dk.gqa_cache_evict(*dev, w, 200, 30, new)
+
+    first = run()
+    for _ in range(3):
+        for a, b in zip(first, run()):
+            assert torch.equal(a, b)
+
+
+def test_eviction_and_append_in_a_graph():
+    """A whole step of a cache that lives in a graph: append, decode, weights
+    added up, eviction into other blocks."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(32)
+    c = Cache([150, 64], 32, 2, 64, seed=6, spare=8)
+    q, k, v = rand(g, 2, 1, 4, 64), rand(g, 2, 2, 64), rand(g, 2, 2, 64)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    new = c.free[:8].int().view(2, 4).cuda()
+
+    def state():
+        return list(c.cuda()) + [torch.zeros(2, 2, 192, device="cuda")]
+
+    def step(kc, vc, ks, vs, table, ctx, w):
+        dk.gqa_cache_append(k, v, cu, ctx, table, kc, vc, ks, vs)
+        o, lse = dk.gqa_decode_fwd(q, kc, vc, ks, vs, table, ctx)
+        dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, weights=w, accumulate=True)
+        return (o, lse) + dk.gqa_cache_evict(kc, vc, ks, vs, table, ctx, w, 100, 10, new)
+
+    plain, held = state(), state()
+    keep = [t.clone() for t in held]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*held)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        res = step(*held)
+    for t, x in zip(held, keep):
+        t.copy_(x)
+    for _ in range(2):  # the second step adds its weights to the first's
+        want = step(*plain)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+    for t, x in zip(held, plain):
+        assert torch.equal(t.view(torch.uint8), x.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ refusals
+def test_python_refusals():
+    """What the Python checks refuse before anything is launched (RuntimeError)."""
+    import deepseek_v4_kernel as dk
+    c = Cache([70, 64], 32, 2, 128, seed=1, spare=8)
+    kc, vc, ks, vs, table, ctx = dev = c.cuda()
+    q = torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    new = c.free[:4].int().view(2, 2).cuda()
+    w = torch.zeros(2, 2, 96, device="cuda")
+    lse = torch.zeros(2, 4, 1, device="cuda")
+    k = torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    before = [t.clone() for t in dev]
+
+    def cache(**change):
+        names = ("k_cache", "v_cache", "k_scale", "v_scale", "block_table", "context_lens")
+        return {**dict(zip(names, dev)), **change}
+
+    bad_cache = [dict(k_cache=kc.view(torch.int8)), dict(k_cache=kc.cpu()), dict(v_cache=vc[:-1]), dict(k_cache=kc[..., :96], v_cache=vc[..., :96]),
+                 dict(k_cache=kc[:, :24], v_cache=vc[:, :24]), dict(v_cache=vc.transpose(0, 1).contiguous().transpose(0, 1)[:, :, :1]),
+                 dict(k_cache=kc[:1].expand(kc.shape)), dict(k_scale=ks.half()), dict(v_scale=vs.t().contiguous().t()),
+                 dict(v_scale=vs[:-1]), dict(block_table=table.long()), dict(block_table=table[:1]), dict(block_table=table[:, ::2]),
+                 dict(context_lens=ctx.long()), dict(context_lens=ctx.cpu()), dict(context_lens=ctx.repeat(2)[::2])]
+    for change in bad_cache:
+        args = cache(**change)
+        with pytest.raises(RuntimeError):
+            dk.gqa_decode_fwd(q, **args)
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_append(k, k, cu, **args)
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_evict(**args, weights=w, budget=40, recent=4, new_block_table=new)
+    for bad in (q.float(), q.cpu(), q[..., :64], q[:1], q[:, :, :3], q.view(2, 4, 128), q.new_zeros(2, 1, 4, 129)[..., 1:],
+                q.new_zeros(2, 1, 128, 4).transpose(2, 3)):
+        with pytest.raises(RuntimeError):
+            dk.gqa_decode_fwd(bad, *dev)
+        with pytest.raises(RuntimeError):
+            dk.gqa_attention_weights(bad, lse, kc, ks, table, ctx)
+    for kw in (dict(sm_scale=0.0), dict(sm_scale=-1.0), dict(sm_scale=float("nan")), dict(out=q.half()), dict(out=q[:1]),
+               dict(out=q[:, :, :1].expand(q.shape)), dict(out=q.new_zeros(2, 1, 4, 136)[..., 4:132])):
+        with pytest.raises(RuntimeError):
+            dk.gqa_decode_fwd(q, *dev, **kw)
+    for kw in (dict(accumulate=True), dict(max_context=0), dict(weights=w, max_context=96), dict(weights=w.double()),
+               dict(weights=w[:1]), dict(weights=w[:, :, ::2]), dict(weights=w[:, :1].expand(w.shape))):
+        with pytest.raises(RuntimeError):
+            dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, **kw)
+    for bad in (lse.half(), lse[:, :2], lse.cpu(), lse.transpose(1, 2).contiguous().transpose(1, 2).expand(2, 4, 1)[:1]):
+        with pytest.raises(RuntimeError):
+            dk.gqa_attention_weights(q, bad, kc, ks, table, ctx)
+    for kw in (dict(k=k.float()), dict(v=k[:2]), dict(v=k.half()), dict(k=k[:, :1], v=k[:, :1]), dict(k=k.cpu()), dict(cu_seqlens=cu[:2]),
+               dict(cu_seqlens=cu.long())):
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_append(**{**dict(k=k, v=k, cu_seqlens=cu), **kw}, **cache())
+    for kw in (dict(budget=0), dict(recent=41), dict(recent=-1), dict(budget=65), dict(new_block_table=table), dict(new_block_table=new[:1]),
+               dict(new_weights=w), dict(new_weights=w[:, :, 1:40]), dict(weights=w.half()), dict(new_weights=w.clone()[:, :1].expand(w.shape))):
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_evict(*dev, **{**dict(weights=w, budget=40, recent=4, new_block_table=new), **kw})
+    x, y = torch.zeros(9, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(9, 2, 128, dtype=torch.bfloat16, device="cuda")
+    cx = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    for args in ((x, y, y[:8], cx), (x, y.half(), y, cx), (x.float(), y.float(), y.float(), cx), (x[..., :96], y[..., :96], y[..., :96], cx),
+                 (x[:, :3], y, y, cx), (x, y, y, cx[:1]), (x, y, y, cx.long()), (x, y[:5], y[:5], cx), (x[:1].expand(x.shape), y, y, cx),
+                 (x, y[:, :1].expand(y.shape), y, cx), (x, y, y, cx.cpu()), (x[..., :64], y[..., :64], y, cx)):
+        with pytest.raises(RuntimeError):
+            dk.gqa_prefill_fwd(*args)
+    for kw in (dict(out=x.half()), dict(out=x[:5]), dict(sm_scale=float("inf")), dict(out=x[:1].expand(x.shape))):
+        with pytest.raises(RuntimeError):
+            dk.gqa_prefill_fwd(x, y, y, cx, **kw)
+    torch.cuda.synchronize()
+    for t, old in zip(dev, before):  # nothing was written
+        assert torch.equal(t.view(torch.uint8), old.view(torch.uint8))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("which", ["prefill", "decode"])
+def test_a_wait_that_runs_out_then_recovers(which):
+    """The first load of every CTA withheld: its wait gives up after about 2 s,
+    the kernel ends by itself, the status word says so, and the next call is right."""
+    import deepseek_v4_kernel as dk
+    from deepseek_v4_kernel import _lib
+    g = torch.Generator(device="cuda").manual_seed(33)
+    c = Cache([700, 90], 64, 2, 128, seed=2)
+    dev, q = c.cuda(), rand(g, 2, 1, 8, 128)
+    x, kv = rand(g, 600, 4, 128), rand(g, 600, 2, 128)
+    cu = torch.tensor([0, 450, 600], dtype=torch.int32, device="cuda")
+
+    def run():
+        return dk.gqa_prefill_fwd(x, kv, kv, cu) if which == "prefill" else dk.gqa_decode_fwd(q, *dev)
+
+    run()
+    assert status() == 0
+    try:
+        assert _lib.lib.dsv4b_set_test_stall(_lib.STALL_GQA) == 0
+        run()
+        torch.cuda.synchronize()
+        assert status() == 1
+    finally:
+        assert _lib.lib.dsv4b_set_test_stall(0) == 0
+    assert status() == 0
+    if which == "prefill":
+        check_prefill(x, kv, kv, [0, 450, 600], None, True)
+    else:
+        check_decode(c, q, dev=dev)
