@@ -119,12 +119,16 @@ inline bool gqa_rows(const void* p, int64_t block, int64_t row, int64_t head, in
   return p && aligned(p, 16);
 }
 
+// Positions of a sequence, and the width of its weights: an int numbers them, tiles past the end too.
+constexpr int kMaxGqaPositions = 1 << 30;
+
 int check_gqa_cache(const dsv4b_gqa_cache* c, bool with_v) {
   if (!c || c->b <= 0 || c->num_blocks <= 0 || c->h_kv <= 0 || c->table_width <= 0) return DSV4B_ERR_INVALID_ARGUMENT;
   if (c->b > dsv4b::kMaxGqaRequests || c->h_kv > 65535) return DSV4B_ERR_UNSUPPORTED;
   const int page = c->page_block_size;
   if (page < 16 || page > 1024 || (page & (page - 1))) return DSV4B_ERR_UNSUPPORTED;
   if (c->d != 64 && c->d != 128) return DSV4B_ERR_UNSUPPORTED;
+  if ((int64_t)c->table_width * page > kMaxGqaPositions) return DSV4B_ERR_UNSUPPORTED;
   if (!gqa_rows(c->k, c->stride_k_block, c->stride_k_row, c->stride_k_head, c->d)) return DSV4B_ERR_INVALID_ARGUMENT;
   if (!c->k_scale || !aligned(c->k_scale, 4) || !c->block_table || !aligned(c->block_table, 4) || !c->context_lens ||
       !aligned(c->context_lens, 4) || c->stride_block_table < 0)
@@ -563,6 +567,7 @@ int dsv4b_gqa_attention_weights(const dsv4b_gqa_cache* c, const dsv4b_gqa_query*
   if (rc || (rc = check_gqa_query(c, q))) return rc;
   if (!lse || !aligned(lse, 4) || !weights || !aligned(weights, 4) || width <= 0 || stride_w_b < 0 || stride_w_h < 0)
     return DSV4B_ERR_INVALID_ARGUMENT;
+  if (width > kMaxGqaPositions) return DSV4B_ERR_UNSUPPORTED;
   int dev = 0;
   DevInfo* info = nullptr;
   if ((rc = current_arch_ok())) return rc;
@@ -585,6 +590,7 @@ int dsv4b_gqa_cache_evict(const dsv4b_gqa_cache* c, const dsv4b_gqa_evict_params
   if (!aligned(e->weights, 4) || !aligned(e->new_weights, 4) || !aligned(e->kept, 4) || !aligned(e->new_lens, 4) ||
       !aligned(e->new_table, 4) || e->new_table == c->block_table)
     return DSV4B_ERR_INVALID_ARGUMENT;
+  if (e->new_width > kMaxGqaPositions) return DSV4B_ERR_UNSUPPORTED;
   if ((rc = current_arch_ok())) return rc;
   return cuda_rc(dsv4b::launch_gqa_evict(*c, *e, static_cast<cudaStream_t>(stream)));
 }

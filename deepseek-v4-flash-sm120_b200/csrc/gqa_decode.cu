@@ -53,12 +53,14 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <climits>
 #include <cstdint>
 #include <type_traits>
 
 #include "dsv4b.h"
 #include "dsv4b_kernels.h"
 #include "dsv4b_ptx.cuh"
+#include "gqa_tc.cuh"
 
 namespace dsv4b {
 
@@ -202,6 +204,15 @@ __device__ __forceinline__ float4 four(uint2 w) {
   }
 }
 
+// The largest magnitude of eight 16-bit values, as the bits of an fp32 (NaN counts as more).
+template <typename T>
+__device__ __forceinline__ uint32_t largest(uint4 w) {
+  const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
+  const uint32_t top = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+  return top << 16;
+}
+
 // The q^T fragments of 8 rows from row r0 on: thread (g, c) holds row g, for
 // k-step 4 h + s the dims 16 (4 h + c) + 4 s + {0, 1, 2, 3}, the same that
 // it reads of K.  Rows from `rows` on are zero.  factor[k] is what the
@@ -222,6 +233,13 @@ __device__ __forceinline__ void fetch_q(const GqaArgs& a, int b, int kvh, int r0
   for (int s = 0; s < D / 16; ++s)
     raw.w[s] = live ? __ldg(reinterpret_cast<const uint2*>(p + (s >> 2) * 64 + c * 16 + (s & 3) * 4)) : make_uint2(0, 0);
 }
+// A row of q's power of two (its largest value `top` becomes 2^13 .. 2^14; an
+// infinite one stays so), and what its products are multiplied by.
+__device__ __forceinline__ void row_scale(const GqaArgs& a, float top, float& up, float& down) {
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 240) - 127 - 13;
+  up = __uint_as_float((uint32_t)(127 - e) << 23);
+  down = a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+}
 template <typename T, int D>
 __device__ __forceinline__ void scale_q(const GqaArgs& a, const RawQ<D>& raw, uint32_t (&q)[D / 16][2],
                                         float (&factor)[2]) {
@@ -235,10 +253,8 @@ __device__ __forceinline__ void scale_q(const GqaArgs& a, const RawQ<D>& raw, ui
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  // the row's largest value becomes 2^13 .. 2^14 (an infinite one stays so)
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 240) - 127 - 13;
-  const float up = __uint_as_float((uint32_t)(127 - e) << 23);
-  const float down = a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+  float up, down;
+  row_scale(a, top, up, down);
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
     q[s][0] = pack_half(f[s].x * up, f[s].y * up);
@@ -1006,37 +1022,6 @@ __global__ void __launch_bounds__(kJoinThreads) gqa_join_kernel(const GqaArgs a)
 }
 
 // ------------------------------------------------------------------ weights
-// Up to 8 rows (one n-tile): every warp of the grid takes a contiguous piece
-// of the units of all (sequence, KV head) pairs and keeps the rows' q in
-// registers.  More: every CTA takes a piece, in it a warp a contiguous part
-// of each pair, and q stands in shared memory, up to kHeldTiles n-tiles of it
-// (further ones take further passes over the piece); K's fragments are
-// widened once per unit and multiplied with two n-tiles at a time.  A thread
-// adds p of its rows, then the four c are joined by a halving exchange that
-// leaves one position per lane.
-constexpr int kHeldTiles = 32;
-template <int D, bool ONE>
-struct Wts {
-  static constexpr int kUnit = ONE ? 64 : 32;
-  static constexpr int kWarps = 12;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = kUnit * D;
-  static constexpr int kSlots = 2;
-  static constexpr int kQBytes = ONE ? 0 : kHeldTiles * (D / 16) * 2 * 32 * 4;
-};
-template <int D, bool ONE>
-struct WeightsShared {
-  uint64_t full[Wts<D, ONE>::kWarps][Wts<D, ONE>::kSlots];
-  ListShared<Wts<D, ONE>::kWarps> list;
-  float factor[ONE ? 1 : kHeldTiles][8], lse[ONE ? 1 : kHeldTiles][8];
-  int abort;
-};
-template <int D, bool ONE>
-constexpr int weights_smem() {
-  using C = Wts<D, ONE>;
-  return 1024 + C::kWarps * C::kSlots * C::kTile + C::kQBytes + (int)sizeof(WeightsShared<D, ONE>);
-}
-
 // lse of row r in log2 units; +inf, which makes its p 0, for a row that is
 // not there or that saw nothing.
 __device__ __forceinline__ float lse_log2(const GqaArgs& a, int b, int kvh, int r, int rows) {
@@ -1045,17 +1030,98 @@ __device__ __forceinline__ float lse_log2(const GqaArgs& a, int b, int kvh, int 
   return x == -INFINITY ? INFINITY : x;
 }
 
-template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(Wts<D, ONE>::kThreads, 1)
+// Zeros behind every context, a warp for 512 positions at a time; this warp is the
+// `me`-th of n.
+__device__ __forceinline__ void zero_behind(const GqaArgs& a, int me, int n) {
+  constexpr int kSpan = 512;
+  const int lane = threadIdx.x & 31, spans = (a.width + kSpan - 1) / kSpan;
+  const long long items = (long long)a.b * a.h_kv * spans;
+  for (long long x = me; x < items; x += n) {
+    const int row = items < (1ll << 31) ? (int)((unsigned)x / (unsigned)spans) : (int)(x / spans);
+    const int from = (int)(x - (long long)row * spans) * kSpan, to = min(from + kSpan, a.width);
+    const int len = held_len(a, row / a.h_kv);
+    if (len >= to) continue;
+    float* w = a.weights + (int64_t)(row / a.h_kv) * a.stride_w_b + (int64_t)(row % a.h_kv) * a.stride_w_h;
+    if (len <= from && to - from == kSpan && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+#pragma unroll
+      for (int t = 0; t < kSpan; t += 128) *reinterpret_cast<float4*>(w + from + t + 4 * lane) = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      for (int t = max(from, len) + lane; t < to; t += 32) w[t] = 0.f;
+    }
+  }
+}
+
+// A walk over a piece's (sequence, KV head) pairs.
+template <int U>
+struct Walk {
+  int b, kvh, nu, len, end;  // nu: the pair's units; `end`: positions that its first query sees
+  int from, n;               // the piece's units of this pair
+  long long left;            // the piece's units from there on
+  __device__ __forceinline__ void enter(const GqaArgs& a) {  // b, kvh, from and left are set
+    len = held_len(a, b);
+    end = __ldg(a.ctx + b) - a.s_q + 1;
+    nu = units_of<U>(len);
+    n = (int)min(left, (long long)(nu - from));
+  }
+  // The i-th piece of the list, of `pieces` places that were found; left == 0: it is empty.
+  template <int W>
+  __device__ __forceinline__ void begin(const GqaArgs& a, const ListShared<W>& list, int parts, int part, int i) {
+    const Split split(list.total, parts);
+    left = split.each + (part < split.more ? 1 : 0);
+    if (left == 0) return;
+    b = list.b[i];
+    const int per_head = units_of<U>(held_len(a, b));
+    const long long u = list.u[i];
+    kvh = u < (1ll << 31) ? (int)((unsigned)u / (unsigned)per_head) : (int)(u / per_head);
+    from = (int)(u - (long long)kvh * per_head);
+    enter(a);
+  }
+  __device__ __forceinline__ bool next(const GqaArgs& a) {  // false: the piece ends
+    left -= n;
+    if (left == 0) return false;
+    from = 0;
+    if (++kvh == a.h_kv) {
+      kvh = 0;
+      ++b;
+    }
+    enter(a);
+    return true;
+  }
+};
+
+// Up to 8 rows (one n-tile of mma.sync): every warp of the grid takes a
+// contiguous piece of the units of all (sequence, KV head) pairs and keeps the
+// rows' q in registers.  A thread adds p of its rows, then the four c are
+// joined by a halving exchange that leaves one position per lane.
+template <int D>
+struct Wts {
+  static constexpr int kUnit = 64;
+  static constexpr int kWarps = 12;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kTile = kUnit * D;
+  static constexpr int kSlots = 2;
+};
+template <int D>
+struct WeightsShared {
+  uint64_t full[Wts<D>::kWarps][Wts<D>::kSlots];
+  ListShared<Wts<D>::kWarps> list;
+  int abort;
+};
+template <int D>
+constexpr int weights_smem() {
+  using C = Wts<D>;
+  return 1024 + C::kWarps * C::kSlots * C::kTile + (int)sizeof(WeightsShared<D>);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Wts<D>::kThreads, 1)
 gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
-  using C = Wts<D, ONE>;
+  using C = Wts<D>;
   constexpr int kWarps = C::kWarps, kSlots = C::kSlots, kTile = C::kTile, kSteps = D / 16;
   constexpr int kUnit = C::kUnit, kRuns = kUnit / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint4* q_held = reinterpret_cast<uint4*>(smem + kWarps * kSlots * kTile);  // [n-tile][two k-steps][lane]
-  WeightsShared<D, ONE>& sh =
-      *reinterpret_cast<WeightsShared<D, ONE>*>(smem + kWarps * kSlots * kTile + C::kQBytes);
+  WeightsShared<D>& sh = *reinterpret_cast<WeightsShared<D>*>(smem + kWarps * kSlots * kTile);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(smem + warp * kSlots * kTile);
   uint64_t* full = sh.full[warp];
@@ -1065,255 +1131,478 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
   }
   if (tid == 0) sh.abort = 0;
   const int rows = a.g * a.s_q;
-  // the piece of the list: the warp's own, or the CTA's
-  const int parts = ONE ? gridDim.x * kWarps : gridDim.x, part = ONE ? blockIdx.x * kWarps + warp : blockIdx.x;
-  find_places<kWarps, kUnit>(a, a.h_kv, ONE ? blockIdx.x * kWarps : blockIdx.x, ONE ? kWarps : 1, parts, sh.list);
-  const Split split(sh.list.total, parts);
+  const int parts = gridDim.x * kWarps;
+  find_places<kWarps, kUnit>(a, a.h_kv, blockIdx.x * kWarps, kWarps, parts, sh.list);
+  Walk<kUnit> cur = {};
+  cur.begin(a, sh.list, parts, blockIdx.x * kWarps + warp, warp);
 
-  // A walk over the piece's pairs, and in each over this warp's units.
-  struct Cursor {
-    int b, kvh, nu, len, end;
-    int from;             // the piece's first unit of this pair
-    long long left;       // the piece's units from there on
-    int u, to;            // this warp's next unit of the pair, and the end of its units
-    __device__ __forceinline__ bool in_pair() const { return u < to; }
-  };
-  auto enter = [&](Cursor& x) {  // b, kvh, from and left are set
-    x.len = held_len(a, x.b);
-    x.end = __ldg(a.ctx + x.b) - a.s_q + 1;
-    x.nu = units_of<kUnit>(x.len);
-    const int n = (int)min(x.left, (long long)(x.nu - x.from));
-    x.u = ONE ? x.from : x.from + (int)((long long)n * warp / kWarps);
-    x.to = ONE ? x.from + n : x.from + (int)((long long)n * (warp + 1) / kWarps);
-  };
-  auto next_pair = [&](Cursor& x) {  // false: the piece ends
-    x.left -= min(x.left, (long long)(x.nu - x.from));
-    if (x.left == 0) return false;
-    x.from = 0;
-    if (++x.kvh == a.h_kv) {
-      x.kvh = 0;
-      ++x.b;
-    }
-    enter(x);
-    return true;
-  };
-  Cursor first = {};
-  first.left = split.each + (part < split.more ? 1 : 0);
-  if (first.left > 0) {
-    const int i = ONE ? warp : 0;
-    first.b = sh.list.b[i];
-    first.nu = units_of<kUnit>(held_len(a, first.b));
-    const long long u = sh.list.u[i];
-    first.kvh = u < (1ll << 31) ? (int)((unsigned)u / (unsigned)first.nu) : (int)(u / first.nu);
-    first.from = (int)(u - (long long)first.kvh * first.nu);
-    enter(first);
-  }
-
-  constexpr int kN = ONE ? 1 : 2;  // n-tiles at a time
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
-  uint32_t q[kN][kSteps][2];
-  float factor[kN][2], lse2[kN][2];
+  uint32_t q[kSteps][2];
+  float factor[2], lse2[2];
   Info<kUnit> now, next;  // of the unit at the products' cursor, and of the one behind it
-  const int tiles = (rows + 8 * kN - 1) / (8 * kN) * kN;
-  for (int n0 = 0; n0 < tiles; n0 += kHeldTiles) {
-    const int nt = min(kHeldTiles, tiles - n0), q_first = n0 * 8 / a.g;
-    Cursor ld = first, cur = first;
-    bool more = first.left > 0 && ok;
-    int loaded = 0;  // and not yet used
-    Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
-    auto load_next = [&](int to) {
-      while (more && !ld.in_pair()) more = next_pair(ld);
-      if (!more) return;
-      fetch_pages<kUnit, false>(a, pages, ld.b, ld.kvh, ld.u, ld.len);
-      int ids[kRuns];
-      next.held = 0;
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i) {
-        ids[i] = __shfl_sync(0xffffffffu, pages.id, (ld.u - pages.base) * kRuns + i);
-        next.held |= (ids[i] >= 0 ? 1 : 0) << i;
-      }
-      if (lane == 0) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, ld.u, ring + to * kTile, &full[to]);
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i)  // after the load: these may still be on their way
-        next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, (ld.u - pages.base) * kRuns + i);
-      ++ld.u;
-      ++loaded;
-    };
-    RawQ<D> raw;
-    if constexpr (ONE) {  // the first rows of q, ahead of the tiles that would be in their way
-      if (first.left > 0) fetch_q<T, D>(a, cur.b, cur.kvh, 0, rows, raw);
+  Walk<kUnit> ld = cur;
+  int ld_u = 0;  // of ld.n
+  bool more = cur.left > 0;
+  int loaded = 0;  // and not yet used
+  Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
+  auto load_next = [&](int to) {
+    if (more && ld_u == ld.n) {
+      more = ld.next(a);
+      ld_u = 0;
     }
-    load_next(slot);
-    now = next;
-    load_next((slot + 1) % kSlots);
-    if (!a.accumulate && n0 == 0) {  // zeros behind each context, while the first tiles come
-      constexpr int kSpan = 512;  // of a row, one warp's
-      const int spans = (a.width + kSpan - 1) / kSpan;
-      const long long items = (long long)a.b * a.h_kv * spans;
-      for (long long x = blockIdx.x * kWarps + warp; x < items; x += gridDim.x * kWarps) {
-        const int row = items < (1ll << 31) ? (int)((unsigned)x / (unsigned)spans) : (int)(x / spans);
-        const int from = (int)(x - (long long)row * spans) * kSpan, to = min(from + kSpan, a.width);
-        const int len = held_len(a, row / a.h_kv);
-        if (len >= to) continue;
-        float* w = a.weights + (int64_t)(row / a.h_kv) * a.stride_w_b + (int64_t)(row % a.h_kv) * a.stride_w_h;
-        if (len <= from && to - from == kSpan && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+    if (!more) return;
+    const int u = ld.from + ld_u;
+    fetch_pages<kUnit, false>(a, pages, ld.b, ld.kvh, u, ld.len);
+    int ids[kRuns];
+    next.held = 0;
 #pragma unroll
-          for (int t = 0; t < kSpan; t += 128) *reinterpret_cast<float4*>(w + from + t + 4 * lane) = make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-          for (int t = max(from, len) + lane; t < to; t += 32) w[t] = 0.f;
+    for (int i = 0; i < kRuns; ++i) {
+      ids[i] = __shfl_sync(0xffffffffu, pages.id, (u - pages.base) * kRuns + i);
+      next.held |= (ids[i] >= 0 ? 1 : 0) << i;
+    }
+    if (lane == 0) load_tile<D, kUnit>(a, &tk, ids, ld.kvh, u, ring + to * kTile, &full[to]);
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i)  // after the load: these may still be on their way
+      next.ks[i] = __shfl_sync(0xffffffffu, pages.ks, (u - pages.base) * kRuns + i);
+    ++ld_u;
+    ++loaded;
+  };
+  RawQ<D> raw;  // the first rows of q, ahead of the tiles that would be in their way
+  if (more) fetch_q<T, D>(a, cur.b, cur.kvh, 0, rows, raw);
+  load_next(slot);
+  now = next;
+  load_next((slot + 1) % kSlots);
+  if (!a.accumulate) zero_behind(a, blockIdx.x * kWarps + warp, gridDim.x * kWarps);  // while the first tiles come
+  bool go = cur.left > 0, q_ready = true;
+  if (go) scale_q<T, D>(a, raw, q, factor);
+  while (go && ok) {  // the pairs of the piece, one after another
+    if (!q_ready) load_q<T, D>(a, cur.b, cur.kvh, 0, rows, q, factor);
+    q_ready = false;
+    lse2[0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
+    lse2[1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
+    for (int j = 0; j < cur.n; ++j) {
+      const int t0 = (cur.from + j) * kUnit;
+      const bool edge = t0 + kUnit > min(cur.len, cur.end) || now.held != (1 << kRuns) - 1;
+      // the positions whose weights this lane will hold
+      const int t_mine = t0 + 8 * c + Lay<D>::perm(g);
+      float* w = a.weights + (int64_t)cur.b * a.stride_w_b + (int64_t)cur.kvh * a.stride_w_h + t_mine;
+      float before[kUnit / 32];
+#pragma unroll
+      for (int x = 0; x < kUnit / 32; ++x) {
+        const int t = t_mine + 32 * x;
+        before[x] = a.accumulate && t < cur.len && t < a.width ? w[32 * x] : 0.f;
+      }
+      if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
+      uint32_t f[4][4];
+      float s[kRuns][4];
+#pragma unroll
+      for (int mt = 0; mt < kRuns; ++mt) {
+        s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          k_frags<D>(ring + slot * kTile, mt, h, f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16(s[mt], f[k][0], f[k][1], f[k][2], f[k][3], q[4 * h + k][0], q[4 * h + k][1]);
         }
       }
-    }
-    bool go = first.left > 0;
-    bool q_ready = false;
-    if constexpr (ONE) {
-      if (go) scale_q<T, D>(a, raw, q[0], factor[0]);
-      q_ready = true;
-    }
-    while (go) {  // the pairs of the piece, one after another
-      if constexpr (ONE) {
-        if (!q_ready) load_q<T, D>(a, cur.b, cur.kvh, 0, rows, q[0], factor[0]);
-        q_ready = false;
-        lse2[0][0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
-        lse2[0][1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
+      __syncwarp();
+      --loaded;
+      const Info<kUnit> here = now;
+      now = next;
+      load_next(slot);
+      if (++slot == kSlots) {
+        slot = 0;
+        phase ^= 1;
+      }
+      float sum[2 * kRuns];  // positions 8 i + perm(g)
+      if (!edge) {
+#pragma unroll
+        for (int i = 0; i < 2 * kRuns; ++i)
+          sum[i] = fast_exp2(fmaf(s[i >> 1][2 * (i & 1)], factor[0] * here.ks[i >> 1], -lse2[0])) +
+                   fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + 1], factor[1] * here.ks[i >> 1], -lse2[1]));
       } else {
-        __syncthreads();  // the last pair's fragments are read
-        for (int n = warp; n < nt; n += kWarps) {
-          uint32_t f[kSteps][2];
-          float fac[2];
-          load_q<T, D>(a, cur.b, cur.kvh, (n0 + n) * 8, rows, f, fac);
-#pragma unroll
-          for (int s = 0; s < kSteps; s += 2)
-            q_held[(n * (kSteps / 2) + s / 2) * 32 + lane] = make_uint4(f[s][0], f[s][1], f[s + 1][0], f[s + 1][1]);
-          if (g == 0) {
-            sh.factor[n][2 * c] = fac[0];
-            sh.factor[n][2 * c + 1] = fac[1];
-          }
-          if (lane < 8) sh.lse[n][lane] = lse_log2(a, cur.b, cur.kvh, (n0 + n) * 8 + lane, rows);
-        }
-        __syncthreads();
-      }
-      for (; ok && cur.in_pair(); ++cur.u) {
-        const int t0 = cur.u * kUnit;
-        const bool edge = t0 + kUnit > min(cur.len, cur.end + q_first) || now.held != (1 << kRuns) - 1;
-        // the positions whose weights this lane will hold
-        const int t_mine = t0 + 8 * c + Lay<D>::perm(g);
-        float* w = a.weights + (int64_t)cur.b * a.stride_w_b + (int64_t)cur.kvh * a.stride_w_h + t_mine;
-        float before[kUnit / 32];
-#pragma unroll
-        for (int x = 0; x < kUnit / 32; ++x) {
-          const int t = t_mine + 32 * x;
-          before[x] = (a.accumulate || n0 > 0) && t < cur.len && t < a.width ? w[32 * x] : 0.f;
-        }
-        if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
-        uint32_t f[ONE ? 1 : kRuns][ONE ? 1 : D / 64][4][4];
-        float s[kN][kRuns][4];
-        if constexpr (ONE) {
-#pragma unroll
-          for (int mt = 0; mt < kRuns; ++mt) {
-            s[0][mt][0] = s[0][mt][1] = s[0][mt][2] = s[0][mt][3] = 0.f;
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              k_frags<D>(ring + slot * kTile, mt, h, f[0][0]);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_f16(s[0][mt], f[0][0][k][0], f[0][0][k][1], f[0][0][k][2], f[0][0][k][3], q[0][4 * h + k][0],
-                        q[0][4 * h + k][1]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int mt = 0; mt < kRuns; ++mt)
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h) k_frags<D>(ring + slot * kTile, mt, h, f[mt][h]);
-        }
-        __syncwarp();
-        --loaded;
-        const Info<kUnit> here = now;
-        now = next;
-        load_next(slot);
-        if (++slot == kSlots) {
-          slot = 0;
-          phase ^= 1;
-        }
-        float sum[2 * kRuns];  // positions 8 i + perm(g)
 #pragma unroll
         for (int i = 0; i < 2 * kRuns; ++i) sum[i] = 0.f;
-        for (int n = 0; n < nt; n += kN) {
-          if constexpr (!ONE) {
 #pragma unroll
-            for (int x = 0; x < kN; ++x) {
+        for (int k = 0; k < 2; ++k) {
+          const int lim = cur.end + (2 * c + k) / a.g;
 #pragma unroll
-              for (int k = 0; k < kSteps; k += 2) {
-                const uint4 v = q_held[((n + x) * (kSteps / 2) + k / 2) * 32 + lane];
-                q[x][k][0] = v.x;
-                q[x][k][1] = v.y;
-                q[x][k + 1][0] = v.z;
-                q[x][k + 1][1] = v.w;
-              }
-              const float2 v = *reinterpret_cast<const float2*>(&sh.factor[n + x][2 * c]);
-              const float2 y = *reinterpret_cast<const float2*>(&sh.lse[n + x][2 * c]);
-              factor[x][0] = v.x;
-              factor[x][1] = v.y;
-              lse2[x][0] = y.x;
-              lse2[x][1] = y.y;
-#pragma unroll
-              for (int mt = 0; mt < kRuns; ++mt) s[x][mt][0] = s[x][mt][1] = s[x][mt][2] = s[x][mt][3] = 0.f;
-            }
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int x = 0; x < kN; ++x)
-#pragma unroll
-                  for (int mt = 0; mt < kRuns; ++mt)
-                    mma_f16(s[x][mt], f[mt][h][k][0], f[mt][h][k][1], f[mt][h][k][2], f[mt][h][k][3], q[x][4 * h + k][0],
-                            q[x][4 * h + k][1]);
+          for (int i = 0; i < 2 * kRuns; ++i) {
+            const bool there = (here.held >> (i >> 1)) & 1;
+            const float p = fast_exp2(fmaf(s[i >> 1][2 * (i & 1) + k], factor[k] * here.ks[i >> 1], -lse2[k]));
+            sum[i] += there && t0 + 8 * i + Lay<D>::perm(g) < lim ? p : 0.f;
           }
-#pragma unroll
-          for (int x = 0; x < kN; ++x) {
-            if (!edge) {
-#pragma unroll
-              for (int i = 0; i < 2 * kRuns; ++i)
-                sum[i] += fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1)], factor[x][0] * here.ks[i >> 1], -lse2[x][0])) +
-                          fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1) + 1], factor[x][1] * here.ks[i >> 1], -lse2[x][1]));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int lim = cur.end + ((n0 + n + x) * 8 + 2 * c + k) / a.g;
-#pragma unroll
-                for (int i = 0; i < 2 * kRuns; ++i) {
-                  const bool there = (here.held >> (i >> 1)) & 1;
-                  const float p = fast_exp2(fmaf(s[x][i >> 1][2 * (i & 1) + k], factor[x][k] * here.ks[i >> 1], -lse2[x][k]));
-                  sum[i] += there && t0 + 8 * i + Lay<D>::perm(g) < lim ? p : 0.f;
-                }
-              }
-            }
-          }
-        }
-        // four values over the four c: each step sends half of them
-#pragma unroll
-        for (int x = 0; x < kUnit / 32; ++x) {
-#pragma unroll
-          for (int h = 2; h >= 1; h >>= 1) {
-            const bool up = lane & h;
-#pragma unroll
-            for (int i = 4 * x; i < 4 * x + h; ++i) {
-              const float send = up ? sum[i] : sum[i + h], keep = up ? sum[i + h] : sum[i];
-              sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, h);
-            }
-          }
-          const int t = t_mine + 32 * x;
-          if (t < cur.len && t < a.width) w[32 * x] = before[x] + sum[4 * x];
         }
       }
-      go = next_pair(cur);
+      // four values over the four c: each step sends half of them
+#pragma unroll
+      for (int x = 0; x < kUnit / 32; ++x) {
+#pragma unroll
+        for (int h = 2; h >= 1; h >>= 1) {
+          const bool up = lane & h;
+#pragma unroll
+          for (int i = 4 * x; i < 4 * x + h; ++i) {
+            const float send = up ? sum[i] : sum[i + h], keep = up ? sum[i + h] : sum[i];
+            sum[i] = keep + __shfl_xor_sync(0xffffffffu, send, h);
+          }
+        }
+        const int t = t_mine + 32 * x;
+        if (t < cur.len && t < a.width) w[32 * x] = before[x] + sum[4 * x];
+      }
     }
-    if (!ok) drain(full, kSlots, slot, phase, loaded);
+    go = cur.next(a);
   }
+  if (!ok) drain(full, kSlots, slot, phase, loaded);
+}
+
+// More rows: S = K q^T on tcgen05, 128 positions by the rows, 64 of them at a
+// time.  A TMEM lane is a position, so a thread has all rows' scores of one
+// and adds their p by itself, without an exchange; K becomes fp16 on its way
+// from shared memory to TMEM (the A operand), a row of a tile per thread, and
+// q stands in shared memory, scaled as above, up to 256 rows of it (further
+// ones take further passes).  A CTA takes a contiguous piece of the list:
+//   warps 0-3, 4-7  p of every second unit each, and their sums;
+//   warps 8-11      q's rows, and K's conversion;
+//   warp 12         page ids, scales, K's loads;     warp 13  the MMAs.
+// Bound by the exponentials (16 a cycle and SM).
+constexpr int kWinUnit = 128, kWinRows = 256, kWinCols = 64;
+constexpr int kWinStages = 4, kWinBufs = 2;  // K tiles; S buffers of a group: 2 * 64 + 3 * 2 * 64 columns of TMEM
+constexpr int kWinInfos = 16;  // more than units can lie between load and sums: 4 + 2 + 6 (a buffer each) + 2
+constexpr int kWinGroups = 3;  // of four warps
+constexpr int kWinConvert = 4 * kWinGroups, kWinLoad = kWinConvert + 4, kWinMma = kWinLoad + 1, kWinWarps = kWinMma + 1;
+struct WindowShared {
+  float factor[2][kWinRows], minus_lse[2][kWinRows];
+  float common[2][kWinRows / 32];  // the factor of 32 rows; 0: each has its own
+  uint64_t k_full[kWinStages], k_empty[kWinStages], a_full[2], a_empty[2], s_full[kWinGroups][kWinBufs], s_empty[kWinGroups][kWinBufs];
+  uint64_t q_full[2], q_empty[2], done;
+  ListShared<kWinWarps> list;
+  Walk<kWinUnit> first;
+  float ks[kWinInfos][kWinUnit / 16];
+  int held[kWinInfos];
+  uint32_t tmem;
+  int abort;
+};
+template <int D>
+constexpr int window_smem() {
+  return 1024 + 2 * kWinRows * D * 2 + kWinStages * kWinUnit * D + (int)sizeof(WindowShared);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWinWarps * 32, 1)
+gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
+  constexpr int kTile = kWinUnit * D, kQ = kWinRows * D * 2, kQChunk = kWinRows * 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  WindowShared& sh = *reinterpret_cast<WindowShared*>(smem + 2 * kQ + kWinStages * kTile);
+  const uint32_t q_s = smem_u32(smem), ring = q_s + 2 * kQ;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kWinStages; ++i) {
+      mbar_init(&sh.k_full[i], 2);
+      mbar_init(&sh.k_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.a_full[i], 4);
+      mbar_init(&sh.a_empty[i], 1);
+      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.q_empty[i], 1 + kWinConvert);
+    }
+    for (int i = 0; i < kWinGroups * kWinBufs; ++i) {
+      mbar_init(&sh.s_full[0][0] + i, 1);
+      mbar_init(&sh.s_empty[0][0] + i, 4);
+    }
+    mbar_init(&sh.done, 1);
+    sh.abort = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == kWinMma) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  find_places<kWinWarps, kWinUnit>(a, a.h_kv, blockIdx.x, 1, gridDim.x, sh.list);  // synchronises
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem, tmem_s = tmem + 128;
+  if (tid == 0) sh.first.begin(a, sh.list, gridDim.x, blockIdx.x, 0);
+  __syncthreads();
+  const int rows = sh.first.left > 0 ? a.g * a.s_q : 0;  // an empty piece has nothing to do
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_warp(bar, parity, &sh.abort, &g_gqa_status); };
+  auto arrive = [&](uint64_t* bar) {  // the warp's
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  bool ok = true;
+  int nu = 0, np = 0;  // units and pairs so far
+
+  if (warp < kWinConvert) {
+    // ------------------------------------------------------------------ p
+    const int group = warp >> 2, p = (warp & 3) * 32 + lane;
+    const uint32_t s_at = tmem_s + ((uint32_t)((warp & 3) * 32) << 16) + group * kWinBufs * kWinCols;
+    int nc = 0;  // the group's S buffers so far
+    if (!a.accumulate) zero_behind(a, blockIdx.x * kWinConvert + warp, gridDim.x * kWinConvert);
+    for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
+      const int cols = (min(rows - r0, kWinRows) + 31) & ~31, chunks = (cols + kWinCols - 1) / kWinCols;
+      const bool add = a.accumulate || r0 > 0;
+      int skip = group;  // units until this group's next; the same ones in every pass
+      Walk<kWinUnit> x = sh.first;
+      do {
+        if (!(ok = wait(&sh.q_full[np & 1], (np >> 1) & 1))) break;
+        const float* factor = sh.factor[np & 1];
+        const float* minus_lse = sh.minus_lse[np & 1];
+        for (int j = 0; j < x.n; ++j, ++nu) {
+          if (skip > 0) {
+            --skip;
+            continue;
+          }
+          skip = kWinGroups - 1;
+          const int t = (x.from + j) * kWinUnit + p;
+          float* w = a.weights + (int64_t)x.b * a.stride_w_b + (int64_t)x.kvh * a.stride_w_h + t;
+          const bool live = t < x.len && t < a.width;
+          const float before = add && live ? *w : 0.f;
+          float ks = 0.f;
+          int r_min = 0;  // rows before it do not see the position
+          bool edge = false;
+          uint64_t sum[2] = {0, 0};  // pairs of zeros
+          for (int c = 0; c < chunks; ++c, ++nc) {
+            const int buf = nc % kWinBufs;
+            if (!(ok = wait(&sh.s_full[group][buf], (nc / kWinBufs) & 1))) break;
+            tc_fence_after();
+            const int n = min(kWinCols, cols - c * kWinCols);
+            if (c == 0) {
+              const int slot = nu % kWinInfos, held = sh.held[slot];
+              ks = sh.ks[slot][p >> 4];
+              edge = (x.from + j + 1) * (long long)kWinUnit > min(x.len, x.end + r0 / a.g) || held != 0xff;
+              r_min = (held >> (p >> 4)) & 1 ? min(max(t - x.end + 1, 0), a.s_q) * a.g - r0 : INT_MAX;
+            }
+            // 16 bytes of shared memory for every four scores (32 with each
+            // row's own factor) are half of what the exponentials take
+            auto add_up = [&](const float (&s)[32], int col, float by, auto general) {
+              const uint64_t scale = pair(by, by);
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(minus_lse + col + e);
+                uint64_t t[2] = {pair(s[e], s[e + 1]), pair(s[e + 2], s[e + 3])}, by2[2] = {scale, scale};
+                if constexpr (general) {
+                  const float4 f = *reinterpret_cast<const float4*>(factor + col + e);
+                  by2[0] = mul2(scale, pair(f.x, f.y));
+                  by2[1] = mul2(scale, pair(f.z, f.w));
+                }
+                float2 y[2] = {unpair(fma2(t[0], by2[0], pair(l.x, l.y))), unpair(fma2(t[1], by2[1], pair(l.z, l.w)))};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  y[i].x = fast_exp2(y[i].x);
+                  y[i].y = fast_exp2(y[i].y);
+                  if constexpr (general) {
+                    y[i].x = col + e + 2 * i >= r_min ? y[i].x : 0.f;
+                    y[i].y = col + e + 2 * i + 1 >= r_min ? y[i].y : 0.f;
+                  }
+                  sum[i] = add2(sum[i], pair(y[i].x, y[i].y));
+                }
+              }
+            };
+            for (int h = 0; h < n; h += 32) {
+              float s[32];
+              tmem_ld32(s_at + buf * kWinCols + h, s);
+              const int col = c * kWinCols + h;
+              const float f = sh.common[np & 1][col / 32];
+              tc_wait_ld();
+              if (h + 32 >= n) {
+                tc_fence_before();
+                arrive(&sh.s_empty[group][buf]);
+              }
+              if (edge || f == 0.f)
+                add_up(s, col, ks, std::true_type());
+              else
+                add_up(s, col, ks * f, std::false_type());
+            }
+          }
+          if (!ok) break;
+          const float2 v = unpair(add2(sum[0], sum[1]));
+          if (live) *w = before + (v.x + v.y);
+        }
+        if (!ok) break;
+        arrive(&sh.q_empty[np & 1]);
+        ++np;
+      } while (x.next(a));
+    }
+  } else if (warp < kWinLoad) {
+    // -------------------------------------------------------- q, conversion
+    const int w4 = warp - kWinConvert;
+    constexpr int kLanes = D / 8, kRowsOnce = 32 / kLanes;  // lanes of a row of q, rows of a load
+    for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
+      const int cols = (min(rows - r0, kWinRows) + 31) & ~31;
+      Walk<kWinUnit> x = sh.first;
+      do {
+        const int qb = np & 1;
+        if (np >= 2 && !(ok = wait(&sh.q_empty[qb], ((np >> 1) - 1) & 1))) break;
+        // 32 rows at a time, all their loads in flight.  Where their largest
+        // values are within 2^8 of one another they get one power of two.
+        const int piece = lane % kLanes;
+        for (int r1 = w4 * 32; r1 < cols; r1 += 4 * 32) {
+          uint4 raw[kLanes];
+#pragma unroll
+          for (int i = 0; i < kLanes; ++i) {
+            const int r = r0 + r1 + i * kRowsOnce + lane / kLanes;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (r < rows)
+              raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)x.b * a.stride_q_b +
+                                                            (int64_t)(r / a.g) * a.stride_q_s +
+                                                            (int64_t)(x.kvh * a.g + r % a.g) * a.stride_q_h) + piece);
+          }
+          sh.minus_lse[qb][r1 + lane] = -lse_log2(a, x.b, x.kvh, r0 + r1 + lane, rows);
+          // the rows' largest values as bits; each exchange halves them, until
+          // a lane has one row's
+          uint32_t top[kLanes];
+#pragma unroll
+          for (int i = 0; i < kLanes; ++i) top[i] = largest<T>(raw[i]);
+#pragma unroll
+          for (int o = kLanes / 2; o >= 1; o >>= 1) {
+            const bool upper = lane & o;
+#pragma unroll
+            for (int i = 0; i < o; ++i) {
+              const uint32_t send = upper ? top[i] : top[i + o], keep = upper ? top[i + o] : top[i];
+              top[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+            }
+          }
+          const uint32_t most = __reduce_max_sync(0xffffffffu, top[0]);
+          const uint32_t least = __reduce_min_sync(0xffffffffu, top[0] ? top[0] : most);
+          const bool one = most < 0x7F800000u && __uint_as_float(least) * 256.f >= __uint_as_float(most);
+          float up, down;
+          row_scale(a, __uint_as_float(most), up, down);
+#pragma unroll
+          for (int i = 0; i < kLanes; ++i) {
+            if (!one) row_scale(a, __uint_as_float(__shfl_sync(0xffffffffu, top[0], (lane & ~(kLanes - 1)) + i)), up, down);
+            const int r = r1 + i * kRowsOnce + lane / kLanes;
+            const float4 u = four<T>(make_uint2(raw[i].x, raw[i].y)), v = four<T>(make_uint2(raw[i].z, raw[i].w));
+            const uint4 h = make_uint4(pack_half(u.x * up, u.y * up), pack_half(u.z * up, u.w * up),
+                                       pack_half(v.x * up, v.y * up), pack_half(v.z * up, v.w * up));
+            sts_v4(q_s + qb * kQ + (piece >> 3) * kQChunk + r * 128 + (((piece & 7) ^ (r & 7)) << 4), h);
+            if (piece == 0) sh.factor[qb][r] = down;
+          }
+          if (lane == 0) sh.common[qb][r1 / 32] = one ? down : 0.f;
+        }
+        fence_proxy_async_smem();
+        arrive(&sh.q_full[qb]);
+        ++np;
+        for (int j = 0; j < x.n; ++j, ++nu) {
+          const int st = nu % kWinStages, row = w4 * 32 + lane;
+          if (!(ok = wait(&sh.k_full[st], (nu / kWinStages) & 1))) break;
+          if (nu >= 2 && !(ok = wait(&sh.a_empty[nu & 1], ((nu >> 1) - 1) & 1))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            uint4 k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = lds_v4(ring + st * kTile + Lay<D>::piece(row, 4 * i + e));
+            float h[32];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t words[4] = {k[e].x, k[e].y, k[e].z, k[e].w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                uint32_t lo, hi;
+                widen4(words[y], lo, hi);
+                h[8 * e + 2 * y] = __uint_as_float(lo);
+                h[8 * e + 2 * y + 1] = __uint_as_float(hi);
+              }
+            }
+            tmem_st32(tmem + ((uint32_t)(w4 * 32) << 16) + (nu & 1) * 64 + i * 32, h);
+          }
+          arrive(&sh.k_empty[st]);
+          tc_wait_st();
+          tc_fence_before();
+          arrive(&sh.a_full[nu & 1]);
+        }
+      } while (ok && x.next(a));
+    }
+  } else if (warp == kWinLoad) {
+    // -------------------------------------------------------------- loads
+    constexpr int kRuns = kWinUnit / 16;
+    Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
+    for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
+      Walk<kWinUnit> x = sh.first;
+      do {
+        for (int j = 0; j < x.n; ++j, ++nu) {
+          const int st = nu % kWinStages, u = x.from + j, slot = nu % kWinInfos;
+          if (nu >= kWinStages && !(ok = wait(&sh.k_empty[st], (nu / kWinStages - 1) & 1))) break;
+          fetch_pages<kWinUnit, false>(a, pages, x.b, x.kvh, u, x.len);
+          const int at = (u - pages.base) * kRuns;
+          int ids[kRuns];
+#pragma unroll
+          for (int i = 0; i < kRuns; ++i) ids[i] = __shfl_sync(0xffffffffu, pages.id, at + i);
+          const unsigned held = __ballot_sync(0xffffffffu, pages.id >= 0) >> at & 0xffu;
+          if (lane == 0) {
+            load_tile<D, kWinUnit>(a, &tk, ids, x.kvh, u, ring + st * kTile, &sh.k_full[st]);
+            sh.held[slot] = (int)held;
+          }
+          if (lane >= at && lane < at + kRuns) sh.ks[slot][lane - at] = pages.ks;
+          arrive(&sh.k_full[st]);
+        }
+      } while (ok && x.next(a));
+    }
+    if (sh.abort) {  // what is in flight lands (or its wait runs out) before the CTA's shared memory goes
+      for (int x = max(0, nu - kWinStages); x < nu; ++x) {
+        const long long t = clock64();
+        while (!mbar_try_wait(smem_u32(&sh.k_full[x % kWinStages]), (x / kWinStages) & 1, 1000u) &&
+               clock64() - t < kWaitLimitCycles) {
+        }
+      }
+    }
+  } else {
+    // --------------------------------------------------------------- MMAs
+    int used[kWinGroups] = {};  // S buffers so far
+    for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
+      const int cols = (min(rows - r0, kWinRows) + 31) & ~31, chunks = (cols + kWinCols - 1) / kWinCols;
+      int group = 0;
+      Walk<kWinUnit> x = sh.first;
+      do {
+        const int qb = np & 1;
+        if (!(ok = wait(&sh.q_full[qb], (np >> 1) & 1))) break;
+        for (int j = 0; j < x.n && ok; ++j, ++nu) {
+          if (!(ok = wait(&sh.a_full[nu & 1], (nu >> 1) & 1))) break;
+          int nc = 0;
+#pragma unroll
+          for (int i = 0; i < kWinGroups; ++i) nc = group == i ? used[i] : nc;
+          for (int c = 0; c < chunks; ++c, ++nc) {
+            const int buf = nc % kWinBufs;
+            if (nc >= kWinBufs && !(ok = wait(&sh.s_empty[group][buf], (nc / kWinBufs - 1) & 1))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t idesc = idesc_of<__half>(min(kWinCols, cols - c * kWinCols), false);
+              const uint32_t b = desc_low(q_s + qb * kQ + c * kWinCols * 128, 16);
+              const uint32_t d = tmem_s + (group * kWinBufs + buf) * kWinCols;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_ts(d, tmem + (nu & 1) * 64 + kk * 8, b + (kk >> 2) * (kQChunk >> 4) + (kk & 3) * 2, kSw128High, idesc,
+                        kk != 0);
+              umma_commit(&sh.s_full[group][buf]);
+              if (c + 1 == chunks) {
+                umma_commit(&sh.a_empty[nu & 1]);
+                if (j + 1 == x.n) umma_commit(&sh.q_empty[qb]);
+              }
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < kWinGroups; ++i) used[i] = group == i ? nc : used[i];
+          group = group + 1 == kWinGroups ? 0 : group + 1;
+        }
+        ++np;
+      } while (ok && x.next(a));
+    }
+    // every MMA has completed before TMEM is freed
+    if (elect_one()) umma_commit(&sh.done);
+    __syncwarp();
+    const long long t = clock64();
+    while (!mbar_try_wait(smem_u32(&sh.done), 0, 1000u) && clock64() - t < kWaitLimitCycles) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWinMma) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------ host
@@ -1398,21 +1687,19 @@ cudaError_t pick_decode(const CUtensorMap& tk, const CUtensorMap& tv, const GqaA
                           : launch_decode<T, D, 2>(tk, tv, a, grid, stream);
 }
 
-template <typename T, int D, bool ONE>
-cudaError_t launch_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cudaStream_t stream) {
-  constexpr int smem = weights_smem<D, ONE>();
-  static_assert(smem <= 227 * 1024, "weights kernel shared memory");
-  static bool done[64] = {};
-  cudaError_t e = allow_smem(&gqa_weights_kernel<T, D, ONE>, smem, done);
-  if (e != cudaSuccess) return e;
-  gqa_weights_kernel<T, D, ONE><<<grid, Wts<D, ONE>::kThreads, smem, stream>>>(tk, a);
-  return cudaGetLastError();
-}
-
 template <typename T, int D>
-cudaError_t pick_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cudaStream_t stream) {
-  return a.g * a.s_q <= 8 ? launch_weights<T, D, true>(tk, a, grid, stream)
-                          : launch_weights<T, D, false>(tk, a, grid, stream);
+cudaError_t launch_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cudaStream_t stream) {
+  static_assert(weights_smem<D>() <= 227 * 1024 && window_smem<D>() <= 227 * 1024, "weights kernels' shared memory");
+  static bool few_done[64] = {}, many_done[64] = {};
+  cudaError_t e;
+  if (a.g * a.s_q <= 8) {
+    if ((e = allow_smem(&gqa_weights_kernel<T, D>, weights_smem<D>(), few_done)) != cudaSuccess) return e;
+    gqa_weights_kernel<T, D><<<grid, Wts<D>::kThreads, weights_smem<D>(), stream>>>(tk, a);
+  } else {
+    if ((e = allow_smem(&gqa_window_weights_kernel<T, D>, window_smem<D>(), many_done)) != cudaSuccess) return e;
+    gqa_window_weights_kernel<T, D><<<grid, kWinWarps * 32, window_smem<D>(), stream>>>(tk, a);
+  }
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -1454,7 +1741,7 @@ cudaError_t launch_gqa_weights(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& 
                                cudaStream_t stream, int* bad_arg) {
   GqaArgs a = make_args(c, q);
   CUtensorMap tk;
-  const int unit = a.g * a.s_q <= 8 ? Wts<128, true>::kUnit : Wts<128, false>::kUnit;
+  const int unit = a.g * a.s_q <= 8 ? Wts<128>::kUnit : kWinUnit;
   if (!make_map(&tk, c.k, c.stride_k_block, c.stride_k_row, c.stride_k_head, unit, c)) {
     *bad_arg = 1;
     return cudaErrorInvalidValue;
@@ -1467,9 +1754,9 @@ cudaError_t launch_gqa_weights(const dsv4b_gqa_cache& c, const dsv4b_gqa_query& 
   a.accumulate = accumulate;
   const int grid = grid_of(sms);
   if (q.dtype == DSV4B_BF16)
-    return c.d == 128 ? pick_weights<__nv_bfloat16, 128>(tk, a, grid, stream)
-                      : pick_weights<__nv_bfloat16, 64>(tk, a, grid, stream);
-  return c.d == 128 ? pick_weights<__half, 128>(tk, a, grid, stream) : pick_weights<__half, 64>(tk, a, grid, stream);
+    return c.d == 128 ? launch_weights<__nv_bfloat16, 128>(tk, a, grid, stream)
+                      : launch_weights<__nv_bfloat16, 64>(tk, a, grid, stream);
+  return c.d == 128 ? launch_weights<__half, 128>(tk, a, grid, stream) : launch_weights<__half, 64>(tk, a, grid, stream);
 }
 
 cudaError_t read_gqa_status(int* flags, cudaStream_t stream) {

@@ -56,6 +56,7 @@
 #include "dsv4b.h"
 #include "dsv4b_kernels.h"
 #include "dsv4b_ptx.cuh"
+#include "gqa_tc.cuh"
 
 namespace dsv4b {
 
@@ -138,12 +139,6 @@ constexpr int smem_bytes() {
   return 1024 + C::kQ + C::kSlotsK * C::kChunksK * kChunk + C::kStagesV * C::kV + (int)sizeof(Shared);
 }
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
 // Cluster launch control: asks for a CTA of this grid that has not started
 // (16 bytes of answer, counted on `bar`), and reads the answer: the CTA's
 // number, or -1 when there are none left (then it must not be asked again).
@@ -165,56 +160,6 @@ __device__ __forceinline__ int read_next(uint32_t answer) {
   return r;
 }
 
-// D[tmem] (+)= A[smem] * B[smem], 16-bit operands, fp32 sums; descriptors as
-// their low words and a common high one.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t high, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(high), "r"(idesc), "r"(accumulate));
-}
-// The same with A from TMEM.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t high, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(high), "r"(idesc), "r"(accumulate));
-}
-
-template <typename T>
-__host__ __device__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
-  constexpr uint32_t types = (1u << 7) | (1u << 10);  // A, B: bf16 (0: fp16)
-  return std::is_same_v<T, __half> ? (idesc_bf16_f32(kM, n, false, b_mn_major) & ~types)
-                                   : idesc_bf16_f32(kM, n, false, b_mn_major);
-}
-
-// Two fp32 at once (Blackwell's packed forms; each half an ordinary fp32 operation).
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -494,9 +439,8 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       // MMAs and stepped, and one high word for all; one elected region holds
       // a tile's O and next S.  (`at`: not hoisted out of the loops, where the
       // descriptors would fill the registers many times over.)
-      constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);  // SBO, version, SWIZZLE_128B
       auto at = [](uint32_t saddr, uint32_t lbo) {
-        uint32_t lo = ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
+        uint32_t lo = desc_low(saddr, lbo);
         asm volatile("" : "+r"(lo));
         return lo;
       };
@@ -516,7 +460,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             const uint32_t q_at = at(q_s + i * (C::kQ / 2) + chunk * kChunk, 16), k_at = at(k_s + st * kPart + c * kChunk, 16);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_ss(tmem + i * kM, q_at + kk * 2, k_at + kk * 2, kDescHigh, idesc_s, (chunk | kk) != 0);
+              umma_ss(tmem + i * kM, q_at + kk * 2, k_at + kk * 2, kSw128High, idesc_s, (chunk | kk) != 0);
           }
           if (last) umma_commit(&sh.k_empty[st]);
         }
@@ -560,7 +504,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
               const uint32_t v_at = at(v_s + sv * C::kV, kChunk);
 #pragma unroll
               for (int kk = 0; kk < kM / 16; ++kk)  // O_i += P_i V
-                umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8, v_at + kk * 128, kDescHigh, idesc_o, (j | kk) != 0);
+                umma_ts(tmem + 256 + i * DV, tmem + i * kM + kk * 8, v_at + kk * 128, kSw128High, idesc_o, (j | kk) != 0);
               if (i == 1 || j >= n[1]) umma_commit(&sh.v_empty[sv]);
               if (j + 1 < n[i]) {
                 scores(i, i == 1 || j + 1 >= n[1]);

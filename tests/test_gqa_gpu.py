@@ -195,8 +195,7 @@ class Cache:
         used = torch.zeros(nb, page, dtype=torch.bool)
         for i, (n, c) in enumerate(zip(lens, counts)):
             self.table[i, :c] = perm[at:at + c]
-            for t in range(n):
-                used[perm[at + t // page], t % page] = True
+            used[perm[at:at + c]] = (torch.arange(c * page) < n).view(c, page)
             at += c
         self.free = perm[at:]
         make = []
@@ -414,6 +413,48 @@ def test_weights(h, hkv, sq, d, page, dtype):
     live = c.ctx >= sq
     total = w.sum(2).cpu()[live]
     torch.testing.assert_close(total, torch.full_like(total, h // hkv * sq), rtol=2e-4, atol=0)
+
+
+@pytest.mark.parametrize("h,hkv,sq,d", [(1, 1, 9, 64), (4, 2, 40, 128), (4, 2, 100, 64), (4, 1, 90, 128), (8, 2, 1, 128)])
+def test_weights_many_units_of_every_cta(h, hkv, sq, d):
+    """One row up to more than are held at once, over contexts that wrap every
+    ring; the 64-bit sums on the GPU (tolerances as in check_weights)."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(sq)
+    c = Cache([130000, 63, 70001], 256, hkv, d, seed=h)
+    kc, vc, ks, vs, table, ctx = dev = c.cuda()
+    q = rand(g, 3, sq, h, d)
+    _, lse = dk.gqa_decode_fwd(q, *dev)
+    got = dk.gqa_attention_weights(q, lse, kc, ks, table, ctx)
+    for i, n in enumerate(c.ctx.tolist()):
+        t = torch.arange(n, device="cuda")
+        blk = table[i, t // 256].long()
+        assert (got[i, :, n:] == 0).all()
+        for kvh in range(hkv):
+            k = kc[blk, t % 256, kvh].double() * ks[blk, kvh].double()[:, None]
+            want, tol = torch.zeros(n, device="cuda", dtype=torch.float64), torch.zeros(n, device="cuda", dtype=torch.float64)
+            for x in range(sq):
+                rows = q[i, x, kvh * (h // hkv):(kvh + 1) * (h // hkv)].double()
+                row_lse = lse[i, kvh * (h // hkv):(kvh + 1) * (h // hkv), x].double()[:, None]
+                p = torch.exp(rows @ k.T * d ** -0.5 - row_lse)
+                p = torch.where((t <= n - sq + x) & torch.isfinite(row_lse), p, 0)
+                want += p.sum(0)
+                tol += (p * (1 + row_lse.abs() + rows.abs() @ k.abs().T * d ** -0.5)).nan_to_num(0, 0, 0).sum(0)
+            assert ((got[i, kvh, :n].double() - want).abs() <= 2.0 ** -18 * tol + 1e-30).all()
+    torch.cuda.synchronize()
+    assert status() == 0
+
+
+def test_weights_rows_of_many_sizes():
+    """Rows of q whose magnitudes lie far apart, beside equal ones, and rows of zeros."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    c = Cache([500, 129], 64, 2, 128, seed=5)
+    q = rand(g, 2, 40, 4, 128)
+    q *= torch.exp2(torch.randint(-12, 2, (2, 40, 4, 1), generator=g, device="cuda").float()).bfloat16()
+    q[0, :, :, :] = rand(g, 40, 4, 128)
+    q[0, 20:, 1] = 0
+    q[1, 30:, 3] = 0
+    check_weights(c, q)
 
 
 def test_weights_into_a_tensor():

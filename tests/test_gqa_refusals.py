@@ -54,7 +54,7 @@ CACHE_BAD = [("b", 0, -1), ("b", 70000, -2), ("num_blocks", 0, -1), ("page_block
              ("page_block_size", 2048, -2), ("d", 96, -2), ("h_kv", 0, -1), ("table_width", 0, -1), ("k", None, -1),
              ("stride_k_row", 136, -1), ("stride_k_head", 64, -1), ("stride_k_block", -256, -1),
              ("stride_k_block", 1 << 41, -1), ("k_scale", None, -1), ("block_table", None, -1), ("context_lens", None, -1),
-             ("stride_block_table", -1, -1)]
+             ("stride_block_table", -1, -1), ("table_width", (1 << 24) + 1, -2)]
 
 
 @pytest.mark.parametrize("field,value,rc", CACHE_BAD + [("v", None, -1), ("v_scale", None, -1), ("stride_v_row", 24, -1)])
@@ -95,6 +95,9 @@ def test_other_refusals(args):
     assert lib.dsv4b_gqa_decode(r(c), r(q), a, 512, 512, 128, None, a, 1 << 30, None) == -1
     assert lib.dsv4b_gqa_attention_weights(r(c), r(q), None, a, 512, 256, 256, 0, None) == -1
     assert lib.dsv4b_gqa_attention_weights(r(c), r(q), a, a, 512, 256, 0, 0, None) == -1
+    assert lib.dsv4b_gqa_attention_weights(r(c), r(q), a, a, 512, 256, (1 << 30) + 1, 0, None) == -2
+    e = gqa.GqaEvictParams(**{**evict, "new_width": (1 << 30) + 1})
+    assert lib.dsv4b_gqa_cache_evict(r(c), r(e), None) == -2
     assert lib.dsv4b_gqa_cache_append(r(c), 5, a, 256, 128, a, 256, 128, a, 1, None) == -2
     assert lib.dsv4b_gqa_cache_append(r(c), 0, a, 256, 127, a, 256, 128, a, 1, None) == -1
     assert lib.dsv4b_gqa_cache_append(r(c), 0, a, 256, 128, a, 256, 128, None, 1, None) == -1
