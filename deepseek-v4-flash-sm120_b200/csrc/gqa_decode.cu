@@ -1258,25 +1258,27 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
   if (!ok) drain(full, kSlots, slot, phase, loaded);
 }
 
-// More rows: S = K q^T on tcgen05, 128 positions by the rows, 64 of them at a
-// time.  A TMEM lane is a position, so a thread has all rows' scores of one
-// and adds their p by itself, without an exchange; K becomes fp16 on its way
-// from shared memory to TMEM (the A operand), a row of a tile per thread, and
-// q stands in shared memory, scaled as above, up to 256 rows of it (further
-// ones take further passes).  A CTA takes a contiguous piece of the list:
-//   warps 0-3, 4-7  p of every second unit each, and their sums;
-//   warps 8-11      q's rows, and K's conversion;
-//   warp 12         page ids, scales, K's loads;     warp 13  the MMAs.
-// Bound by the exponentials (16 a cycle and SM).
-constexpr int kWinUnit = 128, kWinRows = 256, kWinCols = 64;
-constexpr int kWinStages = 4, kWinBufs = 2;  // K tiles; S buffers of a group: 2 * 64 + 3 * 2 * 64 columns of TMEM
-constexpr int kWinInfos = 16;  // more than units can lie between load and sums: 4 + 2 + 6 (a buffer each) + 2
-constexpr int kWinGroups = 3;  // of four warps
+// More rows: S = K q^T on tcgen05, 128 positions by up to 128 rows (further
+// rows take further passes).  A TMEM lane is a position, so a thread has all
+// rows' scores of one and adds their p by itself, without an exchange; K
+// becomes fp16 on its way from shared memory to TMEM (the A operand), a row of
+// a tile per thread, and q stands in shared memory, scaled as above.  A CTA
+// takes a contiguous piece of the list:
+//   warps 0-11      p of every third unit a group of four, and their sums;
+//   warps 12-15     q's rows, and K's conversion;
+//   warp 16         page ids, scales, K's loads;     warp 17  the MMAs.
+// TMEM: K of two units (2 x 64 columns), S of three (3 x 128).
+constexpr int kWinUnit = 128, kWinRows = 128;
+constexpr int kWinStages = 4;  // K tiles
+// Groups and S buffers: as many, so that a group that waits for its next unit
+// has seen the buffer's last one complete (a parity tells only two apart).
+constexpr int kWinGroups = 3;
+constexpr int kWinInfos = 16;  // more than units can lie between load and sums: 4 + 2 + 3
 constexpr int kWinConvert = 4 * kWinGroups, kWinLoad = kWinConvert + 4, kWinMma = kWinLoad + 1, kWinWarps = kWinMma + 1;
 struct WindowShared {
   float factor[2][kWinRows], minus_lse[2][kWinRows];
   float common[2][kWinRows / 32];  // the factor of 32 rows; 0: each has its own
-  uint64_t k_full[kWinStages], k_empty[kWinStages], a_full[2], a_empty[2], s_full[kWinGroups][kWinBufs], s_empty[kWinGroups][kWinBufs];
+  uint64_t k_full[kWinStages], k_empty[kWinStages], a_full[2], a_empty[2], s_full[kWinGroups], s_empty[kWinGroups];
   uint64_t q_full[2], q_empty[2], done;
   ListShared<kWinWarps> list;
   Walk<kWinUnit> first;
@@ -1310,9 +1312,9 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
       mbar_init(&sh.q_full[i], 4);
       mbar_init(&sh.q_empty[i], 1 + kWinConvert);
     }
-    for (int i = 0; i < kWinGroups * kWinBufs; ++i) {
-      mbar_init(&sh.s_full[0][0] + i, 1);
-      mbar_init(&sh.s_empty[0][0] + i, 4);
+    for (int i = 0; i < kWinGroups; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_empty[i], 4);
     }
     mbar_init(&sh.done, 1);
     sh.abort = 0;
@@ -1340,93 +1342,80 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
   if (warp < kWinConvert) {
     // ------------------------------------------------------------------ p
     const int group = warp >> 2, p = (warp & 3) * 32 + lane;
-    const uint32_t s_at = tmem_s + ((uint32_t)((warp & 3) * 32) << 16) + group * kWinBufs * kWinCols;
-    int nc = 0;  // the group's S buffers so far
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     if (!a.accumulate) zero_behind(a, blockIdx.x * kWinConvert + warp, gridDim.x * kWinConvert);
     for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
-      const int cols = (min(rows - r0, kWinRows) + 31) & ~31, chunks = (cols + kWinCols - 1) / kWinCols;
+      const int cols = (min(rows - r0, kWinRows) + 31) & ~31;
       const bool add = a.accumulate || r0 > 0;
-      int skip = group;  // units until this group's next; the same ones in every pass
       Walk<kWinUnit> x = sh.first;
       do {
         if (!(ok = wait(&sh.q_full[np & 1], (np >> 1) & 1))) break;
         const float* factor = sh.factor[np & 1];
         const float* minus_lse = sh.minus_lse[np & 1];
         for (int j = 0; j < x.n; ++j, ++nu) {
-          if (skip > 0) {
-            --skip;
-            continue;
-          }
-          skip = kWinGroups - 1;
+          const int buf = nu % kWinGroups;
+          if (buf != group) continue;
           const int t = (x.from + j) * kWinUnit + p;
           float* w = a.weights + (int64_t)x.b * a.stride_w_b + (int64_t)x.kvh * a.stride_w_h + t;
           const bool live = t < x.len && t < a.width;
-          const float before = add && live ? *w : 0.f;
-          float ks = 0.f;
-          int r_min = 0;  // rows before it do not see the position
-          bool edge = false;
           uint64_t sum[2] = {0, 0};  // pairs of zeros
-          for (int c = 0; c < chunks; ++c, ++nc) {
-            const int buf = nc % kWinBufs;
-            if (!(ok = wait(&sh.s_full[group][buf], (nc / kWinBufs) & 1))) break;
-            tc_fence_after();
-            const int n = min(kWinCols, cols - c * kWinCols);
-            if (c == 0) {
-              const int slot = nu % kWinInfos, held = sh.held[slot];
-              ks = sh.ks[slot][p >> 4];
-              edge = (x.from + j + 1) * (long long)kWinUnit > min(x.len, x.end + r0 / a.g) || held != 0xff;
-              r_min = (held >> (p >> 4)) & 1 ? min(max(t - x.end + 1, 0), a.s_q) * a.g - r0 : INT_MAX;
-            }
-            // 16 bytes of shared memory for every four scores (32 with each
-            // row's own factor) are half of what the exponentials take
-            auto add_up = [&](const float (&s)[32], int col, float by, auto general) {
-              const uint64_t scale = pair(by, by);
+          if (!(ok = wait(&sh.s_full[buf], (nu / kWinGroups) & 1))) break;
+          tc_fence_after();
+          const int held = sh.held[nu % kWinInfos];
+          const float ks = sh.ks[nu % kWinInfos][p >> 4];
+          const bool edge = (x.from + j + 1) * kWinUnit > min(x.len, x.end + r0 / a.g) || held != 0xff;
+          // rows before it do not see the position
+          const int r_min = (held >> (p >> 4)) & 1 ? min(max(t - x.end + 1, 0), a.s_q) * a.g - r0 : INT_MAX;
+          // 16 bytes of shared memory for every four scores (32 with each
+          // row's own factor) are half of what the exponentials take
+          auto add_up = [&](const float (&s)[32], int col, float by, auto general) {
+            const uint64_t scale = pair(by, by);
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(minus_lse + col + e);
-                uint64_t t[2] = {pair(s[e], s[e + 1]), pair(s[e + 2], s[e + 3])}, by2[2] = {scale, scale};
+            for (int e = 0; e < 32; e += 4) {
+              const float4 l = *reinterpret_cast<const float4*>(minus_lse + col + e);
+              uint64_t t[2] = {pair(s[e], s[e + 1]), pair(s[e + 2], s[e + 3])}, by2[2] = {scale, scale};
+              if constexpr (general) {
+                const float4 f = *reinterpret_cast<const float4*>(factor + col + e);
+                by2[0] = mul2(scale, pair(f.x, f.y));
+                by2[1] = mul2(scale, pair(f.z, f.w));
+              }
+              float2 y[2] = {unpair(fma2(t[0], by2[0], pair(l.x, l.y))), unpair(fma2(t[1], by2[1], pair(l.z, l.w)))};
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                y[i].x = fast_exp2(y[i].x);
+                y[i].y = fast_exp2(y[i].y);
                 if constexpr (general) {
-                  const float4 f = *reinterpret_cast<const float4*>(factor + col + e);
-                  by2[0] = mul2(scale, pair(f.x, f.y));
-                  by2[1] = mul2(scale, pair(f.z, f.w));
+                  y[i].x = col + e + 2 * i >= r_min ? y[i].x : 0.f;
+                  y[i].y = col + e + 2 * i + 1 >= r_min ? y[i].y : 0.f;
                 }
-                float2 y[2] = {unpair(fma2(t[0], by2[0], pair(l.x, l.y))), unpair(fma2(t[1], by2[1], pair(l.z, l.w)))};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  y[i].x = fast_exp2(y[i].x);
-                  y[i].y = fast_exp2(y[i].y);
-                  if constexpr (general) {
-                    y[i].x = col + e + 2 * i >= r_min ? y[i].x : 0.f;
-                    y[i].y = col + e + 2 * i + 1 >= r_min ? y[i].y : 0.f;
-                  }
-                  sum[i] = add2(sum[i], pair(y[i].x, y[i].y));
-                }
+                sum[i] = add2(sum[i], pair(y[i].x, y[i].y));
               }
-            };
-            for (int h = 0; h < n; h += 32) {
-              float s[32];
-              tmem_ld32(s_at + buf * kWinCols + h, s);
-              const int col = c * kWinCols + h;
-              const float f = sh.common[np & 1][col / 32];
-              tc_wait_ld();
-              if (h + 32 >= n) {
-                tc_fence_before();
-                arrive(&sh.s_empty[group][buf]);
-              }
-              if (edge || f == 0.f)
-                add_up(s, col, ks, std::true_type());
-              else
-                add_up(s, col, ks * f, std::false_type());
             }
+          };
+          for (int col = 0; col < cols; col += 32) {
+            float s[32];
+            tmem_ld32(tmem_s + lanes + buf * kWinRows + col, s);
+            const float f = sh.common[np & 1][col / 32];
+            tc_wait_ld();
+            if (col + 32 >= cols) {
+              tc_fence_before();
+              arrive(&sh.s_empty[buf]);
+            }
+            if (edge || f == 0.f)
+              add_up(s, col, ks, std::true_type());
+            else
+              add_up(s, col, ks * f, std::false_type());
           }
-          if (!ok) break;
           const float2 v = unpair(add2(sum[0], sum[1]));
-          if (live) *w = before + (v.x + v.y);
+          if (live) *w = (add ? *w : 0.f) + (v.x + v.y);
         }
         if (!ok) break;
         arrive(&sh.q_empty[np & 1]);
         ++np;
       } while (x.next(a));
+      // the next pass adds to what another group may have written (once per
+      // pass by every warp, whether its waits gave up or not)
+      if (r0 + kWinRows < rows) ok = !named_bar_or(1, kWinConvert * 32, !ok);
     }
   } else if (warp < kWinLoad) {
     // -------------------------------------------------------- q, conversion
@@ -1438,49 +1427,61 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
       do {
         const int qb = np & 1;
         if (np >= 2 && !(ok = wait(&sh.q_empty[qb], ((np >> 1) - 1) & 1))) break;
-        // 32 rows at a time, all their loads in flight.  Where their largest
-        // values are within 2^8 of one another they get one power of two.
+        // 32 rows at a time, in two short passes (unrolled as one, its cold code
+        // took longer than its loads): the 16-bit values as they are to where
+        // they belong, then each thread's own in place.  Where the rows'
+        // largest values are within 2^8 of one another they get one power of two.
         const int piece = lane % kLanes;
         for (int r1 = w4 * 32; r1 < cols; r1 += 4 * 32) {
-          uint4 raw[kLanes];
+          const T* q = static_cast<const T*>(a.q) + (int64_t)x.b * a.stride_q_b + (int64_t)x.kvh * a.g * a.stride_q_h + piece * 8;
+          const int sub = lane / kLanes;
+          const uint32_t to = q_s + qb * kQ + (piece >> 3) * kQChunk + (r1 + sub) * 128;  // + 128 a row
+          auto at = [&](int i) { return to + i * kRowsOnce * 128 + (((piece & 7) ^ ((sub + i * kRowsOnce) & 7)) << 4); };
+          auto row_top = [&](const uint4& w) {
+            uint32_t top = largest<T>(w);
 #pragma unroll
-          for (int i = 0; i < kLanes; ++i) {
-            const int r = r0 + r1 + i * kRowsOnce + lane / kLanes;
-            raw[i] = make_uint4(0, 0, 0, 0);
-            if (r < rows)
-              raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)x.b * a.stride_q_b +
-                                                            (int64_t)(r / a.g) * a.stride_q_s +
-                                                            (int64_t)(x.kvh * a.g + r % a.g) * a.stride_q_h) + piece);
-          }
-          sh.minus_lse[qb][r1 + lane] = -lse_log2(a, x.b, x.kvh, r0 + r1 + lane, rows);
-          // the rows' largest values as bits; each exchange halves them, until
-          // a lane has one row's
-          uint32_t top[kLanes];
+            for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            return top;
+          };
+          int r = r0 + r1 + sub, row_q = r / a.g, row_h = r - row_q * a.g;
+          uint32_t most = 0, least = 0xFFFFFFFFu;
+          constexpr int kDeep = 4;
+#pragma unroll 1
+          for (int i = 0; i < kLanes; i += kDeep) {
+            uint4 raw[kDeep];
 #pragma unroll
-          for (int i = 0; i < kLanes; ++i) top[i] = largest<T>(raw[i]);
+            for (int k = 0; k < kDeep; ++k) {
+              raw[k] = make_uint4(0, 0, 0, 0);
+              if (r < rows) raw[k] = __ldg(reinterpret_cast<const uint4*>(q + (int64_t)row_q * a.stride_q_s + (int64_t)row_h * a.stride_q_h));
+              r += kRowsOnce;
+              row_h += kRowsOnce;
+              while (row_h >= a.g) {
+                row_h -= a.g;
+                ++row_q;
+              }
+            }
 #pragma unroll
-          for (int o = kLanes / 2; o >= 1; o >>= 1) {
-            const bool upper = lane & o;
-#pragma unroll
-            for (int i = 0; i < o; ++i) {
-              const uint32_t send = upper ? top[i] : top[i + o], keep = upper ? top[i + o] : top[i];
-              top[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, o));
+            for (int k = 0; k < kDeep; ++k) {
+              sts_v4(at(i + k), raw[k]);
+              const uint32_t top = row_top(raw[k]);
+              most = max(most, top);
+              least = min(least, top ? top : 0xFFFFFFFFu);
             }
           }
-          const uint32_t most = __reduce_max_sync(0xffffffffu, top[0]);
-          const uint32_t least = __reduce_min_sync(0xffffffffu, top[0] ? top[0] : most);
+          sh.minus_lse[qb][r1 + lane] = -lse_log2(a, x.b, x.kvh, r0 + r1 + lane, rows);
+          most = __reduce_max_sync(0xffffffffu, most);
+          least = min(__reduce_min_sync(0xffffffffu, least), most);
           const bool one = most < 0x7F800000u && __uint_as_float(least) * 256.f >= __uint_as_float(most);
           float up, down;
           row_scale(a, __uint_as_float(most), up, down);
-#pragma unroll
+#pragma unroll 2
           for (int i = 0; i < kLanes; ++i) {
-            if (!one) row_scale(a, __uint_as_float(__shfl_sync(0xffffffffu, top[0], (lane & ~(kLanes - 1)) + i)), up, down);
-            const int r = r1 + i * kRowsOnce + lane / kLanes;
-            const float4 u = four<T>(make_uint2(raw[i].x, raw[i].y)), v = four<T>(make_uint2(raw[i].z, raw[i].w));
-            const uint4 h = make_uint4(pack_half(u.x * up, u.y * up), pack_half(u.z * up, u.w * up),
-                                       pack_half(v.x * up, v.y * up), pack_half(v.z * up, v.w * up));
-            sts_v4(q_s + qb * kQ + (piece >> 3) * kQChunk + r * 128 + (((piece & 7) ^ (r & 7)) << 4), h);
-            if (piece == 0) sh.factor[qb][r] = down;
+            const uint4 w = lds_v4(at(i));
+            if (!one) row_scale(a, __uint_as_float(row_top(w)), up, down);
+            const float4 u = four<T>(make_uint2(w.x, w.y)), v = four<T>(make_uint2(w.z, w.w));
+            sts_v4(at(i), make_uint4(pack_half(u.x * up, u.y * up), pack_half(u.z * up, u.w * up),
+                                     pack_half(v.x * up, v.y * up), pack_half(v.z * up, v.w * up)));
+            if (piece == 0) sh.factor[qb][r1 + sub + i * kRowsOnce] = down;
           }
           if (lane == 0) sh.common[qb][r1 / 32] = one ? down : 0.f;
         }
@@ -1553,42 +1554,28 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
     }
   } else {
     // --------------------------------------------------------------- MMAs
-    int used[kWinGroups] = {};  // S buffers so far
     for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
-      const int cols = (min(rows - r0, kWinRows) + 31) & ~31, chunks = (cols + kWinCols - 1) / kWinCols;
-      int group = 0;
+      const uint32_t idesc = idesc_of<__half>((min(rows - r0, kWinRows) + 31) & ~31, false);
       Walk<kWinUnit> x = sh.first;
       do {
         const int qb = np & 1;
         if (!(ok = wait(&sh.q_full[qb], (np >> 1) & 1))) break;
-        for (int j = 0; j < x.n && ok; ++j, ++nu) {
+        for (int j = 0; j < x.n; ++j, ++nu) {
+          const int buf = nu % kWinGroups;
+          if (nu >= kWinGroups && !(ok = wait(&sh.s_empty[buf], (nu / kWinGroups - 1) & 1))) break;
           if (!(ok = wait(&sh.a_full[nu & 1], (nu >> 1) & 1))) break;
-          int nc = 0;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t b = desc_low(q_s + qb * kQ, 16);
 #pragma unroll
-          for (int i = 0; i < kWinGroups; ++i) nc = group == i ? used[i] : nc;
-          for (int c = 0; c < chunks; ++c, ++nc) {
-            const int buf = nc % kWinBufs;
-            if (nc >= kWinBufs && !(ok = wait(&sh.s_empty[group][buf], (nc / kWinBufs - 1) & 1))) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t idesc = idesc_of<__half>(min(kWinCols, cols - c * kWinCols), false);
-              const uint32_t b = desc_low(q_s + qb * kQ + c * kWinCols * 128, 16);
-              const uint32_t d = tmem_s + (group * kWinBufs + buf) * kWinCols;
-#pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk)
-                umma_ts(d, tmem + (nu & 1) * 64 + kk * 8, b + (kk >> 2) * (kQChunk >> 4) + (kk & 3) * 2, kSw128High, idesc,
-                        kk != 0);
-              umma_commit(&sh.s_full[group][buf]);
-              if (c + 1 == chunks) {
-                umma_commit(&sh.a_empty[nu & 1]);
-                if (j + 1 == x.n) umma_commit(&sh.q_empty[qb]);
-              }
-            }
-            __syncwarp();
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_ts(tmem_s + buf * kWinRows, tmem + (nu & 1) * 64 + kk * 8, b + (kk >> 2) * (kQChunk >> 4) + (kk & 3) * 2,
+                      kSw128High, idesc, kk != 0);
+            umma_commit(&sh.s_full[buf]);
+            umma_commit(&sh.a_empty[nu & 1]);
+            if (j + 1 == x.n) umma_commit(&sh.q_empty[qb]);
           }
-#pragma unroll
-          for (int i = 0; i < kWinGroups; ++i) used[i] = group == i ? nc : used[i];
-          group = group + 1 == kWinGroups ? 0 : group + 1;
+          __syncwarp();
         }
         ++np;
       } while (ok && x.next(a));
