@@ -5,10 +5,11 @@
 //   s[r][t] = sm_scale * k_scale * sum_d q[r][d] * k[t][d]
 //   out[r]  = sum_t exp(s[r][t] - lse[r]) * v_scale * v[t]
 // for the rows r = (query, head) that share a KV head: h_q / h_kv * s_q of
-// them, few against the positions.  Every cached byte is used for all rows
-// at once and only once, so the kernels are bound by the cache's bytes.
+// them, in decode few against the positions.  Every cached byte is used for
+// all rows (of a group of 8 or 16) at once and only once, so decode and the
+// weights of few rows are bound by the cache's bytes.
 //
-// Work.  A unit is 32 positions of one (sequence, KV head, group of 8 or 16
+// Work.  A unit is 64 positions of one (sequence, KV head, group of 8 or 16
 // rows).  All units stand in one list, and every warp of the grid (one CTA
 // per SM) takes an equal, contiguous piece of it, so ragged batches balance
 // without a plan made ahead.  A warp runs the softmax of its piece by
@@ -16,10 +17,17 @@
 // head, group) are joined; those that reach over CTAs are joined by a second
 // kernel.
 //
-// Loads.  Each warp has its own ring of 32-position tiles, K and V in turn
-// (4 KB each at d = 128), filled by TMA tiled loads that swizzle the rows
+// Loads.  Each warp has its own ring of 64-position tiles, K and V in turn
+// (8 KB each at d = 128), filled by TMA tiled loads that swizzle the rows
 // and counted on mbarriers: up to 192 KB are in flight on an SM, without a
 // register or an issue slot spent on them.
+//
+// Measured, d = 128, against 6.5 TB/s of a copy: 16 sequences of 131,072
+// positions, 8 KV heads of 16 rows (4.1 GB) 720 us, 5.7 TB/s; 32 of 1,000 to
+// 32,768 with 8 rows (554 MB) 124 us, 4.5 TB/s; one of 4,096 (8.4 MB) 18 us.
+// The last is what a call takes whatever its size (launch, the list, the
+// first tiles behind their page ids, the joins), of which the middle one
+// shows about 15 us; it also loses to warps of a CTA that end apart.
 //
 // Products.  mma.sync m16n8k16 with fp16 operands, positions (or dims of V)
 // as M and rows as N = 8: s^T = k q^T, out^T = v^T p^T.  The operands of
@@ -412,14 +420,14 @@ __device__ __forceinline__ void load_tile(const GqaArgs& a, const CUtensorMap* m
     mbar_arrive_expect_tx(bar, ids[0] >= 0 ? kBytes : 0);
     if (ids[0] >= 0) tma_load_4d(tile, map, 0, (u * U) & (a.page - 1), kvh, ids[0], bar);
   } else {
-    const int runs = a.page / 16;  // of a block: 1 or 2
+    const int runs = a.page >> 4;  // of a block: 1, 2 or 4
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < U / 16; ++i) n += (i % runs == 0 && ids[i] >= 0) ? 1 : 0;
+    for (int i = 0; i < U / 16; ++i) n += ((i & (runs - 1)) == 0 && ids[i] >= 0) ? 1 : 0;
     mbar_arrive_expect_tx(bar, n * a.page * D);
 #pragma unroll
     for (int i = 0; i < U / 16; ++i)
-      if (i % runs == 0 && ids[i] >= 0) tma_load_4d(tile + i * 16 * D, map, 0, 0, kvh, ids[i], bar);
+      if ((i & (runs - 1)) == 0 && ids[i] >= 0) tma_load_4d(tile + i * 16 * D, map, 0, 0, kvh, ids[i], bar);
   }
 }
 
@@ -1092,7 +1100,9 @@ struct Walk {
 // Up to 8 rows (one n-tile of mma.sync): every warp of the grid takes a
 // contiguous piece of the units of all (sequence, KV head) pairs and keeps the
 // rows' q in registers.  A thread adds p of its rows, then the four c are
-// joined by a halving exchange that leaves one position per lane.
+// joined by a halving exchange that leaves one position per lane.  Bound by
+// its start and K's bytes: 32 sequences of 500 to 16,384, 8 KV heads, d = 64
+// (95 MB) 31 us.
 template <int D>
 struct Wts {
   static constexpr int kUnit = 64;
@@ -1268,12 +1278,20 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
 //   warps 12-15     q's rows, and K's conversion;
 //   warp 16         page ids, scales, K's loads;     warp 17  the MMAs.
 // TMEM: K of two units (2 x 64 columns), S of three (3 x 128).
+//
+// With many rows the exponentials bound it, 16 a cycle and SM: 128 rows of
+// 105,000 positions and 8 heads are 108 M of them, 27 us; it takes 59, of
+// which 6 pass before the first S.  (S in tiles of 64 rows took 63: an MMA
+// whose A is in TMEM takes 64 cycles whatever N is.  Two groups: 68.)  With
+// few it is K's bytes.  mma.sync, an n-tile of rows after another, was the
+// quicker only up to 16 rows.  32 sequences of 16,000, d = 128, us (this;
+// mma.sync):  8 rows 195, 104;  16 117, 114;  32 122, 152;  128 199, 397.
 constexpr int kWinUnit = 128, kWinRows = 128;
-constexpr int kWinStages = 4;  // K tiles
+constexpr int kWinStages = 8;  // K tiles
 // Groups and S buffers: as many, so that a group that waits for its next unit
 // has seen the buffer's last one complete (a parity tells only two apart).
 constexpr int kWinGroups = 3;
-constexpr int kWinInfos = 16;  // more than units can lie between load and sums: 4 + 2 + 3
+constexpr int kWinInfos = 16;  // more than units can lie between load and sums: 8 + 2 + 3
 constexpr int kWinConvert = 4 * kWinGroups, kWinLoad = kWinConvert + 4, kWinMma = kWinLoad + 1, kWinWarps = kWinMma + 1;
 struct WindowShared {
   float factor[2][kWinRows], minus_lse[2][kWinRows];
@@ -1521,26 +1539,53 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
     }
   } else if (warp == kWinLoad) {
     // -------------------------------------------------------------- loads
-    constexpr int kRuns = kWinUnit / 16;
-    Pages pages = {-1, -1, -1, -1, 1.f, 1.f};
+    // 512 positions at a time, a lane for 16 of them: four units, whose blocks
+    // are loaded by as many lanes at once (one lane for all took 1,300 cycles
+    // of a unit).
+    constexpr int kRuns = kWinUnit / 16, kUnits = 32 / kRuns;
+    const int unit = lane / kRuns, run = lane % kRuns, box = min(a.page, kWinUnit);
+    // every lane's stage is free (a unit's own one; the first ones are)
+    auto wait_free = [&](int nth, int st) {
+      const uint32_t bar = smem_u32(&sh.k_empty[st]), parity = (nth / kWinStages - 1) & 1;
+      volatile int* abort = &sh.abort;
+      const long long t0 = clock64();
+      for (;;) {
+        if (__all_sync(0xffffffffu, nth < kWinStages || mbar_try_wait(bar, parity))) return true;
+        const bool late = clock64() - t0 > kWaitLimitCycles;
+        if (__any_sync(0xffffffffu, late || *abort)) {
+          *abort = 1;
+          if (late) atomicOr(&g_gqa_status, kErrWaitTimeout);
+          return false;
+        }
+      }
+    };
     for (int r0 = 0; r0 < rows && ok; r0 += kWinRows) {
       Walk<kWinUnit> x = sh.first;
       do {
-        for (int j = 0; j < x.n; ++j, ++nu) {
-          const int st = nu % kWinStages, u = x.from + j, slot = nu % kWinInfos;
-          if (nu >= kWinStages && !(ok = wait(&sh.k_empty[st], (nu / kWinStages - 1) & 1))) break;
-          fetch_pages<kWinUnit, false>(a, pages, x.b, x.kvh, u, x.len);
-          const int at = (u - pages.base) * kRuns;
-          int ids[kRuns];
-#pragma unroll
-          for (int i = 0; i < kRuns; ++i) ids[i] = __shfl_sync(0xffffffffu, pages.id, at + i);
-          const unsigned held = __ballot_sync(0xffffffffu, pages.id >= 0) >> at & 0xffu;
-          if (lane == 0) {
-            load_tile<D, kWinUnit>(a, &tk, ids, x.kvh, u, ring + st * kTile, &sh.k_full[st]);
-            sh.held[slot] = (int)held;
+        for (int u0 = x.from & ~(kUnits - 1); u0 < x.from + x.n; u0 += kUnits) {
+          const int u = u0 + unit, t = u * kWinUnit + run * 16;
+          int id = -1;
+          float ks = 1.f;
+          if (t < x.len) {
+            id = __ldg(a.table + (int64_t)x.b * a.stride_table + (t >> a.page_shift));
+            if (id < 0 || id >= a.num_blocks) id = -1;
+            if (id >= 0) ks = __ldg(a.k_scale + (int64_t)id * a.h_kv + x.kvh);
           }
-          if (lane >= at && lane < at + kRuns) sh.ks[slot][lane - at] = pages.ks;
-          arrive(&sh.k_full[st]);
+          const int skip = max(x.from - u0, 0), n = min(x.from + x.n - u0, kUnits) - skip;
+          const bool mine = unit >= skip && unit < skip + n;
+          const int nth = nu + (mine ? unit - skip : 0), st = nth % kWinStages, slot = nth % kWinInfos;
+          const unsigned held = __ballot_sync(0xffffffffu, id >= 0) >> (unit * kRuns) & 0xffu;
+          const bool load = mine && id >= 0 && (run * 16 & (box - 1)) == 0;
+          const unsigned loads = __ballot_sync(0xffffffffu, load) >> (unit * kRuns) & 0xffu;
+          if (!(ok = wait_free(nth, st))) break;
+          if (mine && run == 0) mbar_arrive_expect_tx(&sh.k_full[st], __popc(loads) * box * D);
+          __syncwarp();
+          if (load) tma_load_4d(ring + st * kTile + run * 16 * D, &tk, 0, t & (a.page - 1), x.kvh, id, &sh.k_full[st]);
+          if (mine) sh.ks[slot][run] = ks;
+          if (mine && run == 0) sh.held[slot] = (int)held;
+          __syncwarp();
+          if (mine && run == 0) mbar_arrive(&sh.k_full[st]);
+          nu += n;
         }
       } while (ok && x.next(a));
     }
@@ -1679,7 +1724,7 @@ cudaError_t launch_weights(const CUtensorMap& tk, const GqaArgs& a, int grid, cu
   static_assert(weights_smem<D>() <= 227 * 1024 && window_smem<D>() <= 227 * 1024, "weights kernels' shared memory");
   static bool few_done[64] = {}, many_done[64] = {};
   cudaError_t e;
-  if (a.g * a.s_q <= 8) {
+  if (a.g * a.s_q <= 8) {  // (one n-tile)
     if ((e = allow_smem(&gqa_weights_kernel<T, D>, weights_smem<D>(), few_done)) != cudaSuccess) return e;
     gqa_weights_kernel<T, D><<<grid, Wts<D>::kThreads, weights_smem<D>(), stream>>>(tk, a);
   } else {
