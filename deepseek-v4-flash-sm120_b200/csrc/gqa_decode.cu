@@ -1285,7 +1285,7 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
 // whose A is in TMEM takes 64 cycles whatever N is.  Two groups: 68.)  With
 // few it is K's bytes.  mma.sync, an n-tile of rows after another, was the
 // quicker only up to 16 rows.  32 sequences of 16,000, d = 128, us (this;
-// mma.sync):  8 rows 195, 104;  16 117, 114;  32 122, 152;  128 199, 397.
+// mma.sync):  8 rows 115, 104;  16 117, 114;  32 122, 152;  128 199, 397.
 constexpr int kWinUnit = 128, kWinRows = 128;
 constexpr int kWinStages = 8;  // K tiles
 // Groups and S buffers: as many, so that a group that waits for its next unit

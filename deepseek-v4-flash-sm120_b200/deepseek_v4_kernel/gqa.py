@@ -17,8 +17,9 @@ pool is passed as ``pool.transpose(1, 2)``), P a power of two from 16 to
 1024, d 64 or 128; ``k_scale`` and ``v_scale`` fp32 [num_blocks, h_kv]: a
 stored value stands for e4m3 * scale of its block and head.  Position t of
 sequence i lies in block ``block_table[i, t // P]``, row t % P;
-``context_lens`` int32 [b] counts each sequence's positions.  Block ids out
-of range hold nothing: reads leave them out, writes skip them.
+``context_lens`` int32 [b] counts each sequence's positions, a table holds at
+most 2^30.  Block ids out of range hold nothing: reads leave them out, writes
+skip them.
 
 All run on the current stream without a host synchronisation and can be
 captured in CUDA graphs.  Errors raise RuntimeError.  See include/dsv4b.h

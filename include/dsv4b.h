@@ -316,7 +316,9 @@ DSV4B_API int dsv4b_mqa_logits_status(int* flags, void* stream);
  * for e4m3 * scale.  Position t of sequence i lies in block
  * block_table[i][t / page_block_size], row t % page_block_size.  A block id
  * that is negative or >= num_blocks, or past the table's width, holds
- * nothing: reads leave its positions out, writes to it are skipped. */
+ * nothing: reads leave its positions out, writes to it are skipped.  A table
+ * holds at most 2^30 positions (DSV4B_ERR_UNSUPPORTED), weights are at most
+ * as wide. */
 typedef struct dsv4b_gqa_cache {
   void* k;                   /* e4m3 */
   void* v;
