@@ -36,6 +36,7 @@ _EXPORTS = {
     "gqa_cache_evict": ("gqa", "gqa_cache_evict"),
     "gqa_decode_fwd": ("gqa", "gqa_decode_fwd"),
     "gqa_prefill_fwd": ("gqa", "gqa_prefill_fwd"),
+    "gqa_status": ("gqa", "gqa_status"),
     "gather_dequant": ("ops", "gather_dequant"),
     "read_kernel_status": ("ops", "read_kernel_status"),
     "sparse_decode_fwd": ("ops", "sparse_decode_fwd"),

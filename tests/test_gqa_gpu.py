@@ -665,6 +665,53 @@ def test_a_serving_run():
     assert (kept >= 0).sum() == hkv * int(c.ctx.sum())
 
 
+@pytest.mark.parametrize("page", [512, 1024])
+def test_large_pages(page):
+    """Every operator over the largest blocks: whole, cut short, and shared by old and new rows."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    old, new = [page - 1, 0, 700], [600, 3, page]
+    c = Cache(old, page, 2, 128, seed=4, spare=12, width=3)
+    for i in range(3):  # room for the new ones
+        have = -(-old[i] // page)
+        want = -(-(old[i] + new[i]) // page)
+        c.table[i, have:want] = c.free[2 * i:2 * i + want - have]
+    c.ctx = torch.tensor([x + y for x, y in zip(old, new)], dtype=torch.int32)
+    kv = rand(g, sum(new), 2, 128), rand(g, sum(new), 2, 128)
+    dev = check_append(c, kv, packed(new), c.ctx.tolist(), torch.bfloat16)
+    q = rand(g, 3, 2, 8, 128)
+    check_decode(c, q, dev=dev)
+    w = check_weights(c, q[:, -1:])
+    check_weights(c, rand(g, 3, 12, 8, 128))
+    c.free = c.free[6:]
+    check_evict(c, w.cpu(), page + 50, 64)
+
+
+def test_evict_into_bad_blocks():
+    """New blocks that are not there are not written, the rest is as without them."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator().manual_seed(22)
+    c = Cache([300, 200], 32, 2, 64, seed=3, spare=8)
+    w = torch.rand(2, 2, 320, generator=g).cuda()
+    new = c.free[:8].int().view(2, 4).cuda()
+    good, bad = c.cuda(), c.cuda()
+    want = dk.gqa_cache_evict(*good, w, 100, 10, new)
+    hole = new.clone()
+    hole[0, 1], hole[1, 3], hole[1, 0] = -1, 2 ** 31 - 1, c.kc.shape[0]
+    got = dk.gqa_cache_evict(*bad, w, 100, 10, hole)
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+    kept = torch.tensor([new[0, 0], new[0, 2], new[0, 3], new[1, 1], new[1, 2]], device="cuda").long()
+    lost = torch.tensor([new[0, 1], new[1, 3], new[1, 0]], device="cuda").long()
+    first = c.cuda()
+    for i in range(4):
+        x, y, z = (t[i].view(torch.uint8) for t in (good, bad, first))
+        assert torch.equal(x[kept], y[kept]) and torch.equal(y[lost], z[lost])
+        rest = torch.ones(len(x), dtype=torch.bool, device="cuda")
+        rest[new.flatten().long()] = False
+        assert torch.equal(y[rest], z[rest])
+    assert status() == 0
+
+
 def test_graph_streams_and_two_at_once():
     """Captured in two graphs that share nothing, replayed on two streams at
     once, with inputs that changed in place; the results are those of plain
