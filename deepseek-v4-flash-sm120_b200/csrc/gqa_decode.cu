@@ -317,7 +317,7 @@ struct Split {
 
 template <int W>
 struct ListShared {
-  long long sum[W];
+  long long sum[W], pre[W * 32];
   long long total;
   int b[W];
   long long u[W];
@@ -327,7 +327,9 @@ struct ListShared {
 // sequences' units (per_seq times over for a sequence's heads and groups)
 // begin: sh.b[k] the sequence (-1: past the end), sh.u[k] the unit among all
 // of the sequence's.  Every thread sums a run of sequences, the sums are
-// scanned, and the thread whose run holds a beginning walks to it.
+// scanned, and a thread per piece searches the scan and walks the run that
+// holds its beginning (the run's own thread, for all pieces in it, took 2,000
+// cycles more where one sequence holds them all).
 template <int W, int U>
 __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int part0, int n, int parts,
                                             ListShared<W>& sh) {
@@ -343,7 +345,6 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int p
     if (lane >= o) incl += v;
   }
   if (lane == 31) sh.sum[warp] = incl;
-  if (tid < n) sh.b[tid] = -1;
   __syncthreads();
   long long pre = incl - sum, total = 0;
 #pragma unroll
@@ -352,17 +353,22 @@ __device__ __forceinline__ void find_places(const GqaArgs& a, int per_seq, int p
     total += sh.sum[i];
   }
   if (tid == 0) sh.total = total;
-  if (sum > 0) {
-    const Split split(total, parts);
-    for (int k = 0; k < n; ++k) {
-      const long long x = split.begin(part0 + k);
-      if (x < pre || x >= pre + sum) continue;
-      long long at = pre;
-      for (int i = i0; i < i1; ++i) {
+  sh.pre[tid] = pre;
+  __syncthreads();
+  if (tid < n) {
+    const long long x = Split(total, parts).begin(part0 + tid);
+    sh.b[tid] = -1;
+    if (x < total) {
+      int j = 0;  // the last run that begins at or before x (an empty one begins where the next does)
+#pragma unroll 1
+      for (int o = 512; o; o >>= 1)
+        if (j + o < W * 32 && sh.pre[j + o] <= x) j += o;
+      long long at = sh.pre[j];
+      for (int i = j * run; i < a.b; ++i) {
         const long long m = (long long)units_of<U>(held_len(a, i)) * per_seq;
         if (x < at + m) {
-          sh.b[k] = i;
-          sh.u[k] = x - at;
+          sh.b[tid] = i;
+          sh.u[tid] = x - at;
           break;
         }
         at += m;
