@@ -24,10 +24,10 @@
 //
 // Measured, d = 128, against 6.5 TB/s of a copy: 16 sequences of 131,072
 // positions, 8 KV heads of 16 rows (4.1 GB) 720 us, 5.7 TB/s; 32 of 1,000 to
-// 32,768 with 8 rows (554 MB) 124 us, 4.5 TB/s; one of 4,096 (8.4 MB) 18 us.
+// 32,768 with 8 rows (554 MB) 123 us, 4.5 TB/s; one of 4,096 (8.4 MB) 16.5.
 // The last is what a call takes whatever its size (launch, the list, the
 // first tiles behind their page ids, the joins), of which the middle one
-// shows about 15 us; it also loses to warps of a CTA that end apart.
+// shows about 14 us; it also loses to warps of a CTA that end apart.
 //
 // Products.  mma.sync m16n8k16 with fp16 operands, positions (or dims of V)
 // as M and rows as N = 8: s^T = k q^T, out^T = v^T p^T.  The operands of
@@ -1108,7 +1108,7 @@ struct Walk {
 // rows' q in registers.  A thread adds p of its rows, then the four c are
 // joined by a halving exchange that leaves one position per lane.  Bound by
 // its start and K's bytes: 32 sequences of 500 to 16,384, 8 KV heads, d = 64
-// (95 MB) 31 us.
+// (95 MB) 29 us.
 template <int D>
 struct Wts {
   static constexpr int kUnit = 64;
