@@ -53,7 +53,11 @@
 // <= 2^8; p is rounded to fp16 for p.v (2^-11 of each term), sums and the
 // softmax's denominator are fp32 of the unrounded p.  The accumulator is
 // kept in units of the current block's v_scale and rescaled when that or m
-// changes, so that no scale enters an fp16.
+// changes, so that no scale enters an fp16.  A v_scale may be anything (append
+// gives a block of zeros 2^-100), so the unit stays within 2^64 of the
+// largest so far: sums of 2^30 positions keep below 2^112 units.  Blocks
+// further down are added position by position, in fp32, if they hold anything
+// but zeros.  A piece's values are kept divided by their sum, as large as V.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -82,6 +86,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;  // log2 of how far m may be outgrown
+constexpr float kUnitSpan = 5.421010862427522e-20f;  // 2^-64: the least unit of o beside the largest v_scale
 
 struct GqaArgs {
   const void* q;
@@ -465,7 +470,7 @@ struct Dec {
 };
 
 // A piece of one (sequence, head, group of rows): id numbers these; last:
-// the CTA that holds its last unit.  o is not divided by l, both are relative to
+// the CTA that holds its last unit.  o is divided by l, which is relative to
 // 2^m.
 template <int D, int NT>
 struct Partial {
@@ -492,6 +497,9 @@ struct DecodeShared {
   int id[2 * C::kWarps];  // -1: none
   int from[2 * C::kWarps], to[2 * C::kWarps], nu[2 * C::kWarps], in_ring[2 * C::kWarps];
   float ml[2 * C::kWarps][2 * C::kRows];  // m, l
+  // A warp's unit of o (0: o holds nothing), and the least one that it may
+  // take: kUnitSpan times the largest v_scale so far.  Here for want of registers.
+  float unit[C::kWarps], least_unit[C::kWarps];
   int list_of[2 * C::kWarps], run[2 * C::kWarps + 1], n_runs;
   int abort;
 };
@@ -520,6 +528,8 @@ __device__ __forceinline__ float* lse_at(const GqaArgs& a, int b, int kvh, int r
   return a.lse + ((int64_t)b * a.h_q + kvh * a.g + r % a.g) * a.s_q + r / a.g;
 }
 
+constexpr int kMaxCtas = 192;
+
 // Joins n pieces of one (sequence, head, group), in order, for the four
 // consecutive values from e on of its [rows][D]: piece i has maxima and sums
 // ml_of(i) (m, then l) and values o_of(i).  Writes the result, or the joined
@@ -531,9 +541,15 @@ __device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML 
   const int row = e / D, d0 = e % D;
   const int r = grp * kRows + row;
   if (r >= a.g * a.s_q) return;
-  float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, ml_of(i)[row]);
+  float m = -INFINITY, most = 0.f;
+  for (int i = 0; i < n; ++i) {
+    m = fmaxf(m, ml_of(i)[row]);
+    most = fmaxf(most, ml_of(i)[kRows + row]);
+  }
   const float base = m == -INFINITY ? 0.f : m;
+  // Sums of up to 192 pieces that weigh 2^-8 at most are no larger than V (a
+  // power of two: no division).
+  const float scale = __uint_as_float((254u << 23) - (__float_as_uint(most) & 0x7F800000u)) * 0x1p-9f;
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kDeep = 8;  // loads in flight
@@ -544,8 +560,9 @@ __device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML 
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
       if (i0 + i < n) {
-        const float f = fast_exp2(ml_of(i0 + i)[row] - base);  // 0 where nothing was seen
-        l += f * ml_of(i0 + i)[kRows + row];
+        const float w = fast_exp2(ml_of(i0 + i)[row] - base) * ml_of(i0 + i)[kRows + row];  // 0 where nothing was seen
+        const float f = w * scale;
+        l += w;
         o.x += f * x[i].x;
         o.y += f * x[i].y;
         o.z += f * x[i].z;
@@ -553,6 +570,9 @@ __device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML 
       }
     }
   }
+  const bool none = l == 0.f;  // (not by m: a row of NaN scores has none, and is NaN)
+  const float inv = none ? 0.f : 1.f / (l * scale);
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   if (part) {
     if (d0 == 0) {
       part->m[row] = m;
@@ -561,10 +581,7 @@ __device__ __forceinline__ void join(const GqaArgs& a, int e, int n, int id, ML 
     *reinterpret_cast<float4*>(part->o + e) = o;
     return;
   }
-  const bool none = l == 0.f;  // (not by m: a row of NaN scores has none, and is NaN)
-  const float inv = none ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) =
-      make_uint2(pack16<T>(o.x * inv, o.y * inv), pack16<T>(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(out_row<T>(a, b, kvh, r) + d0) = make_uint2(pack16<T>(o.x, o.y), pack16<T>(o.z, o.w));
   if (d0 == 0) *lse_at(a, b, kvh, r) = none ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -674,8 +691,8 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
   uint32_t q[NT][kSteps][2];
   float factor[NT][2];
-  float o[kSteps][NT][4];  // (dim col(g) + 2 i, rows 2c, 2c + 1), (dim col(g) + 2 i + 1, the same), in units of v_unit
-  float m[NT][2], l[NT][2], v_unit = 1.f;
+  float o[kSteps][NT][4];  // (dim col(g) + 2 i, rows 2c, 2c + 1), (dim col(g) + 2 i + 1, the same), in units of sh.unit
+  float m[NT][2], l[NT][2];
   int from = 0, q_first = 0, q_of[NT][2];  // the first row's query, and those of rows 2c, 2c + 1
   bool fresh = true, ok = true, first = true;
   if (left > 0) {
@@ -714,7 +731,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int i = 0; i < kSteps; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
-      v_unit = 1.f;
+      sh.unit[warp] = sh.least_unit[warp] = 0.f;
       from = cur.u;
       fresh = false;
     }
@@ -824,13 +841,18 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     if (!(ok = mbar_wait_warp(&full[slot], phase, &sh.abort, &g_gqa_status))) break;
     const uint32_t v_tile = ring + slot * kTile;
+    float v_unit = sh.unit[warp];
 #pragma unroll
     for (int mt = 0; mt < kRuns; ++mt) {
-      // o into units of these positions' v_scale (0: they add nothing)
+      // o into units of these positions' v_scale (0: they add nothing), or
+      // into the least one if that is larger
       const bool there = (now.held >> mt) & 1 && now.vs[mt] != 0.f;
       if (there && now.vs[mt] != v_unit) {  // the same in all lanes
-        const float r = v_unit / now.vs[mt];
-        v_unit = now.vs[mt];
+        const float least = sh.least_unit[warp], size = fabsf(now.vs[mt]), old = v_unit;
+        v_unit = size < least ? least : now.vs[mt];
+        edge |= size < least;
+        sh.least_unit[warp] = fmaxf(least, size * kUnitSpan);
+        const float r = old / v_unit;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -846,11 +868,12 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int k = 0; k < 4; ++k) lds_v_row<D>(v_tile, row[k], g, w[k]);
       // A position that some row does not see stays out of the product:
       // 0 * NaN of a stale or masked value would reach that row.  Zero
-      // values here, added below for the rows that see them.
+      // values here, added below for the rows that see them; so are those of
+      // a scale below the unit.
       if (edge) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const bool in = there && t0 + row[k] < all;
+          const bool in = there && now.vs[mt] == v_unit && t0 + row[k] < all;
 #pragma unroll
           for (int e = 0; e < D / 32; ++e) w[k][e] = in ? w[k][e] : 0u;
         }
@@ -869,8 +892,23 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
       }
       if (edge && there) {
-        // the drafts' own positions: at most s_q - 1, one by one
-        const int lo = max(max(all, 0), t0 + 16 * mt), hi = min(cur.len, t0 + 16 * mt + 16);
+        // the drafts' own positions (at most s_q - 1), or all of a scale below
+        // the unit if they hold anything, one by one
+        int lo = max(all, 0);
+        if (now.vs[mt] != v_unit) {
+          uint32_t any = 0;
+#pragma unroll 1
+          for (int x = c; x < 16; x += 4) {
+            uint32_t v[D / 32];
+            lds_v_row<D>(v_tile, 16 * mt + x, g, v);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) any |= v[e] & 0x7F7F7F7Fu;
+          }
+          if (__any_sync(0xffffffffu, any != 0)) lo = 0;
+        }
+        lo = max(lo, t0 + 16 * mt);
+        const int hi = min(cur.len, t0 + 16 * mt + 16);
+        const float by = now.vs[mt] / v_unit;
         for (int x = lo; x < hi; ++x) {
           const int in8 = (x - t0) & 7, h = ((x - t0) >> 3) & 1;
           const int from_lane = Lay<D>::unperm(in8) * 4 + c;
@@ -880,7 +918,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const float px = __shfl_sync(0xffffffffu, h ? s[mt][n][2 + k] : s[mt][n][k], from_lane);
+              const float px = by * __shfl_sync(0xffffffffu, h ? s[mt][n][2 + k] : s[mt][n][k], from_lane);
               if (x < cur.end + q_of[n][k]) {
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
@@ -894,6 +932,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
       }
     }
+    sh.unit[warp] = v_unit;
     __syncwarp();
     now = next;
     load_next(slot);
@@ -925,12 +964,12 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         for (int k = 0; k < 2; ++k) {
           const int row = 8 * n + 2 * c + k, r = r0 + row;
           const bool none = l[n][k] == 0.f;
-          const float f = whole ? (none ? 0.f : v_unit / l[n][k]) : v_unit;
+          const float inv = none ? 0.f : 1.f / l[n][k];
           float v[2 * kSteps];
 #pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            v[2 * i] = o[i][n][k] * f;
-            v[2 * i + 1] = o[i][n][2 + k] * f;
+          for (int i = 0; i < kSteps; ++i) {  // (v_unit / l might not be a normal number)
+            v[2 * i] = o[i][n][k] * inv * v_unit;
+            v[2 * i + 1] = o[i][n][2 + k] * inv * v_unit;
           }
           if (whole) {
             if (r < rows) {
@@ -1006,7 +1045,6 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 // Joins what several CTAs have of one (sequence, head, group): CTA i's, if
 // it begins there.  The pieces lie in the CTAs up to `last` (a short list
 // leaves some of them without a unit).
-constexpr int kMaxCtas = 192;
 constexpr int kJoinThreads = 256;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) gqa_join_kernel(const GqaArgs a) {

@@ -1,0 +1,125 @@
+"""Grouped-query operators on the GPU at the ends of their range: magnitudes
+and scales far apart, contexts that give every warp many units, rows that are
+left out, tensors that share memory.  Tolerances as in test_gqa_gpu.py, where
+nothing else is said."""
+import math
+
+import pytest
+import torch
+
+from test_gqa_gpu import U, rand, status
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ decode
+def pool(nb, page, hkv, d, seed):
+    """A filled cache: k_cache, v_cache, k_scale, v_scale."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = [(torch.randn(nb, page, hkv, d, generator=g, device="cuda") * 60).clamp_(-448, 448).to(torch.float8_e4m3fn)
+         for _ in range(2)]
+    return x + [torch.exp2(torch.randint(-8, -4, (nb, hkv), generator=g, device="cuda").float()) for _ in range(2)]
+
+
+def check_decode_on_gpu(dev, q, scale=None):
+    """check_decode for long contexts, with the 64-bit sums on the GPU.  A
+    weight's rounding to fp16 is off by no more than the weight itself, and
+    a warp's sums have four steps for each of its units, off by 2^-23 each."""
+    import deepseek_v4_kernel as dk
+    kc, vc, ks, vs, table, ctx = dev
+    b, s_q, h, d = q.shape
+    page, hkv = kc.shape[1:3]
+    g = h // hkv
+    scale = d ** -0.5 if scale is None else scale
+    got, lse = dk.gqa_decode_fwd(q, *dev, sm_scale=scale)
+    torch.cuda.synchronize()
+    assert status() == 0
+    lens = ctx.tolist()
+    units = sum(max(1, -(-n // 64)) for n in lens) * hkv * -(-g * s_q // 16)
+    pieces = torch.cuda.get_device_properties(0).multi_processor_count * 8
+    steps = 2.0 ** -23 * (4 * -(-units // pieces) + 32)
+    u = U[q.dtype]
+    for i, n in enumerate(lens):
+        if n == 0:
+            assert (got[i] == 0).all() and torch.isneginf(lse[i]).all()
+            continue
+        t = torch.arange(n, device="cuda")
+        blk = table[i, t // page].long()
+        sees = t <= n - s_q + torch.arange(s_q, device="cuda")[:, None]
+        for kvh in range(hkv):
+            k, v = (x[blk, t % page, kvh].double() * y[blk, kvh].double()[:, None] for x, y in ((kc, ks), (vc, vs)))
+            rows = q[i, :, kvh * g:(kvh + 1) * g].double()
+            s = torch.where(sees[:, None], rows @ k.T * scale, -math.inf)
+            size = torch.where(sees[:, None], rows.abs() @ k.abs().T * scale, 0).amax(-1)
+            wl = torch.logsumexp(s, -1)
+            p = torch.where(sees[:, None], torch.exp(s - wl[..., None]), 0)
+            want, mag, rest = p @ v, p @ v.abs(), p.clamp(max=2.0 ** -25) @ v.abs()
+            e = 2.0 ** -19 * size + 2.0 ** -20 + steps
+            tol = u * want.abs() + (2.0 ** -11 + 2 * e)[..., None] * mag + rest + 1e-30
+            o, l = got[i, :, kvh * g:(kvh + 1) * g].double(), lse[i, kvh * g:(kvh + 1) * g].T.double()
+            off = (o - want).abs()
+            assert (off <= tol).all(), (i, kvh, off.max().item(), int((~(off <= tol)).sum()))
+            none = ~sees.any(-1)
+            assert torch.isneginf(l[none]).all()
+            assert ((l - wl).abs() <= e + 2.0 ** -22 * wl.abs())[~none].all(), (i, kvh)
+    return got, lse
+
+
+Z = "zero"
+SCALES = {"zero blocks": [17, Z, -8, 17, Z], "large": [119, -8, 119, Z, 3], "upwards": [-8, 60, 119],
+          "downwards": [100, 50, 0, -50, -100, -126], "tiny": [0, -127, -140, -8], "near": [-8, -30, -7, -50]}
+
+
+@pytest.mark.parametrize("h,d,page", [(4, 128, 16), (16, 128, 64), (3, 64, 32), (12, 64, 16)])
+@pytest.mark.parametrize("kind", SCALES)
+def test_decode_value_scales_far_apart(kind, h, d, page):
+    """Blocks whose v_scale differ by up to 2^219, subnormal ones and blocks of zeros (Z) among them."""
+    g = torch.Generator(device="cuda").manual_seed(40)
+    lens = [(211 * i) % 1900 for i in range(120)] + [9000]
+    counts = [-(-n // page) for n in lens]
+    kc, vc, ks, vs = pool(sum(counts), page, 1, d, 41)
+    table = torch.zeros(len(lens), max(counts), dtype=torch.int32)
+    at = 0
+    exps = torch.zeros(sum(counts), dtype=torch.float64)
+    zero = torch.zeros(sum(counts), dtype=torch.bool)
+    for i, c in enumerate(counts):
+        table[i, :c] = torch.arange(at, at + c)
+        for j in range(c):
+            x = SCALES[kind][(i + j) % len(SCALES[kind])]
+            zero[at + j] = x == Z
+            exps[at + j] = -100 if x == Z else x
+        at += c
+    vs[:, 0] = torch.exp2(exps).float().cuda()
+    vc.view(torch.uint8)[zero.cuda()] = 0
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check_decode_on_gpu((kc, vc, ks, vs, table.cuda(), ctx), rand(g, len(lens), 1, h, d))
+
+
+def test_decode_after_append_of_zeros():
+    """A block of zeros, which append gives the scale 2^-100, behind large values."""
+    import deepseek_v4_kernel as dk
+    kc, vc, ks, vs = pool(4, 16, 1, 128, 42)
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    ctx = torch.tensor([48], dtype=torch.int32, device="cuda")
+    k, v = (torch.zeros(48, 1, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    v[:16] = 3e7
+    v[32:] = 1.0
+    cu = torch.tensor([0, 48], dtype=torch.int32, device="cuda")
+    dk.gqa_cache_append(k, v, cu, ctx, table, kc, vc, ks, vs)
+    check_decode_on_gpu((kc, vc, ks, vs, table, ctx), torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_decode_large_values_out_of_sight(first):
+    """V of 2^119 units at positions of weight 2^-261, ordinary ones elsewhere."""
+    kc, vc, ks, vs = pool(64, 16, 1, 128, 43)
+    ks.fill_(1.0)
+    kc.zero_()
+    far = torch.zeros(64, dtype=torch.bool)
+    far[0 if first else 9] = far[20:23] = True
+    far = far.cuda()
+    kc.view(torch.uint8)[far] = 0x38  # 1.0
+    vs[far], vs[~far] = 2.0 ** 119, 2.0 ** -8
+    table = torch.arange(64, dtype=torch.int32, device="cuda")[None]
+    ctx = torch.tensor([1020], dtype=torch.int32, device="cuda")
+    check_decode_on_gpu((kc, vc, ks, vs, table, ctx), torch.full((1, 1, 3, 128), -16.0, dtype=torch.bfloat16, device="cuda"))
