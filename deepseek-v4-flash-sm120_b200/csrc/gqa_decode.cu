@@ -249,7 +249,7 @@ __device__ __forceinline__ void fetch_q(const GqaArgs& a, int b, int kvh, int r0
 // A row of q's power of two (its largest value `top` becomes 2^13 .. 2^14; an
 // infinite one stays so), and what its products are multiplied by.
 __device__ __forceinline__ void row_scale(const GqaArgs& a, float top, float& up, float& down) {
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 240) - 127 - 13;
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 40), 254) - 127 - 13;
   up = __uint_as_float((uint32_t)(127 - e) << 23);
   down = a.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
 }

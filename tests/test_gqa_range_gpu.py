@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gqa_gpu import U, rand, status
+from test_gqa_gpu import Cache, U, check_decode, check_weights, rand, status
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,18 @@ def test_decode_large_values_out_of_sight(first):
     table = torch.arange(64, dtype=torch.int32, device="cuda")[None]
     ctx = torch.tensor([1020], dtype=torch.int32, device="cuda")
     check_decode_on_gpu((kc, vc, ks, vs, table, ctx), torch.full((1, 1, 3, 128), -16.0, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("top", [116, 120, 127])
+def test_queries_near_the_largest(top):
+    """bf16 queries of up to 2^top beside keys as small: ordinary scores, in
+    decode and in both kernels of the weights."""
+    g = torch.Generator(device="cuda").manual_seed(44)
+    c = Cache([300, 64], 16, 2, 128, seed=12)
+    c.ks *= 2.0 ** -top
+    for s_q in (1, 10):
+        x = (torch.randn(2, s_q, 8, 128, generator=g, device="cuda") * 0.25).clamp(-0.99, 0.99)
+        q = (x.double() * 2.0 ** top).bfloat16()
+        assert q.isfinite().all()
+        check_decode(c, q)
+        check_weights(c, q)
