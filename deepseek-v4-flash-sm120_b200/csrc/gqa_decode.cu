@@ -1236,9 +1236,12 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
     q_ready = false;
     lse2[0] = lse_log2(a, cur.b, cur.kvh, 2 * c, rows);
     lse2[1] = lse_log2(a, cur.b, cur.kvh, 2 * c + 1, rows);
+    // a row that saw nothing adds nothing, whatever its scores are
+    const bool left_out = __any_sync(0xffffffffu, (2 * c < rows && lse2[0] == INFINITY) ||
+                                                      (2 * c + 1 < rows && lse2[1] == INFINITY));
     for (int j = 0; j < cur.n; ++j) {
       const int t0 = (cur.from + j) * kUnit;
-      const bool edge = t0 + kUnit > min(cur.len, cur.end) || now.held != (1 << kRuns) - 1;
+      const bool edge = left_out || t0 + kUnit > min(cur.len, cur.end) || now.held != (1 << kRuns) - 1;
       // the positions whose weights this lane will hold
       const int t_mine = t0 + 8 * c + Lay<D>::perm(g);
       float* w = a.weights + (int64_t)cur.b * a.stride_w_b + (int64_t)cur.kvh * a.stride_w_h + t_mine;
@@ -1282,7 +1285,7 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
         for (int i = 0; i < 2 * kRuns; ++i) sum[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int lim = cur.end + (2 * c + k) / a.g;
+          const int lim = lse2[k] == INFINITY ? INT_MIN : cur.end + (2 * c + k) / a.g;
 #pragma unroll
           for (int i = 0; i < 2 * kRuns; ++i) {
             const bool there = (here.held >> (i >> 1)) & 1;
@@ -1339,7 +1342,7 @@ constexpr int kWinInfos = 16;  // more than units can lie between load and sums:
 constexpr int kWinConvert = 4 * kWinGroups, kWinLoad = kWinConvert + 4, kWinMma = kWinLoad + 1, kWinWarps = kWinMma + 1;
 struct WindowShared {
   float factor[2][kWinRows], minus_lse[2][kWinRows];
-  float common[2][kWinRows / 32];  // the factor of 32 rows; 0: each has its own
+  float common[2][kWinRows / 32];  // the factor of 32 rows; 0: each has its own, or some are left out
   uint64_t k_full[kWinStages], k_empty[kWinStages], a_full[2], a_empty[2], s_full[kWinGroups], s_empty[kWinGroups];
   uint64_t q_full[2], q_empty[2], done;
   ListShared<kWinWarps> list;
@@ -1447,8 +1450,9 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
                 y[i].x = fast_exp2(y[i].x);
                 y[i].y = fast_exp2(y[i].y);
                 if constexpr (general) {
-                  y[i].x = col + e + 2 * i >= r_min ? y[i].x : 0.f;
-                  y[i].y = col + e + 2 * i + 1 >= r_min ? y[i].y : 0.f;
+                  const float2 from = i ? make_float2(l.z, l.w) : make_float2(l.x, l.y);
+                  y[i].x = col + e + 2 * i >= r_min && from.x != -INFINITY ? y[i].x : 0.f;
+                  y[i].y = col + e + 2 * i + 1 >= r_min && from.y != -INFINITY ? y[i].y : 0.f;
                 }
                 sum[i] = add2(sum[i], pair(y[i].x, y[i].y));
               }
@@ -1530,10 +1534,13 @@ gqa_window_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs 
               least = min(least, top ? top : 0xFFFFFFFFu);
             }
           }
-          sh.minus_lse[qb][r1 + lane] = -lse_log2(a, x.b, x.kvh, r0 + r1 + lane, rows);
+          const float minus_lse = -lse_log2(a, x.b, x.kvh, r0 + r1 + lane, rows);
+          sh.minus_lse[qb][r1 + lane] = minus_lse;
+          // a row that saw nothing adds nothing, whatever its scores are
+          const bool left_out = __any_sync(0xffffffffu, r0 + r1 + lane < rows && minus_lse == -INFINITY);
           most = __reduce_max_sync(0xffffffffu, most);
           least = min(__reduce_min_sync(0xffffffffu, least), most);
-          const bool one = most < 0x7F800000u && __uint_as_float(least) * 256.f >= __uint_as_float(most);
+          const bool one = !left_out && most < 0x7F800000u && __uint_as_float(least) * 256.f >= __uint_as_float(most);
           float up, down;
           row_scale(a, __uint_as_float(most), up, down);
 #pragma unroll 2

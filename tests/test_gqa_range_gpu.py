@@ -138,3 +138,24 @@ def test_queries_near_the_largest(top):
         assert q.isfinite().all()
         check_decode(c, q)
         check_weights(c, q)
+
+
+# ------------------------------------------------------------------ weights
+@pytest.mark.parametrize("s_q", [1, 3, 40, 60])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), 1.0])
+def test_weights_of_queries_that_are_left_out(s_q, what):
+    """An lse of -inf: the query adds nothing, whatever it holds; nor do
+    positions that hold NaN where no query is left."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(45)
+    c = Cache([300, 128, 90], 32, 2, 128, seed=13)
+    q = rand(g, 3, s_q, 4, 128)
+    _, lse = dk.gqa_decode_fwd(q, *c.cuda())
+    lse[0, 1, s_q // 2] = -math.inf
+    q[0, s_q // 2, 1, 5:7] = what
+    q[0, s_q // 2, 1, 9] = -what
+    lse[2] = -math.inf
+    q[2] = what
+    c.kc[c.table[2, 0].item(), 3, :, 0] = 0x7F
+    w = check_weights(c, q, lse=lse)
+    assert (w[2] == 0).all()
