@@ -140,6 +140,37 @@ def test_queries_near_the_largest(top):
         check_weights(c, q)
 
 
+LONG = [(4, 1, 1, 128, 256, [130001, 0, 70, 1, 64, 33000, 8193, 60000]),
+        (16, 2, 1, 64, 16, [65, 50000, 0, 128, 12345, 70007]),
+        (1, 1, 2, 64, 64, [300000, 3, 100000, 1]),
+        (24, 2, 3, 128, 64, [20011, 5, 0, 40000, 64]),
+        (16, 1, 1, 128, 16, [400000, 31, 250000]),
+        (12, 1, 1, 64, 64, [1000003, 77, 0, 500000]),
+        (32, 8, 1, 128, 32, [9000 + 77 * i for i in range(24)]),
+        (64, 8, 1, 128, 64, [20000 + 3001 * i for i in range(20)]),
+        (40, 8, 2, 64, 128, [1 + 531 * i for i in range(40)])]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("h,hkv,sq,d,page,lens", LONG)
+@pytest.mark.parametrize("grow", [False, True])
+def test_decode_many_units_of_every_warp(h, hkv, sq, d, page, lens, grow, dtype):
+    """Rings that wrap, running maxima and sums carried from unit to unit, one
+    (sequence, head, group) after another in a warp, pieces joined over warps
+    and CTAs: 2 to 68 units of a warp, scales that differ from block to block."""
+    g = torch.Generator(device="cuda").manual_seed(46)
+    nb = 700
+    kc, vc, ks, vs = pool(nb, page, hkv, d, 47)
+    width = max(-(-n // page) for n in lens)
+    table = torch.randint(nb, (len(lens), width), generator=g, device="cuda", dtype=torch.int32)
+    if grow:  # scores that grow along the context
+        table = table.sort(1)[0]
+        ks *= torch.exp2(torch.linspace(-4, 3, nb, device="cuda"))[:, None]
+    q = rand(g, len(lens), sq, h, d, dtype=dtype)
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check_decode_on_gpu((kc, vc, ks, vs, table, ctx), q)
+
+
 # ------------------------------------------------------------------ weights
 @pytest.mark.parametrize("s_q", [1, 3, 40, 60])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), 1.0])
