@@ -49,13 +49,16 @@
 //
 // Numbers.  q is scaled by a power of two per row so that fp16 holds it
 // (bf16 has fewer digits; what lies 2^-27 below the row's largest is lost).
-// The running maximum m is moved only when a score outgrows it by 2^8, so p
-// <= 2^8; p is rounded to fp16 for p.v (2^-11 of each term), sums and the
-// softmax's denominator are fp32 of the unrounded p.  The accumulator is
+// p is relative to m, which lies 2^7 below the running maximum and is moved
+// only when a score outgrows that by 2^8, so p <= 2^15: fp16's range is used
+// up to its end, for the small p of a long context (2^-14 of the maximum and
+// less would lose digits, 2^-25 be gone with m at the maximum).  p is rounded
+// to fp16 for p.v (2^-11 of each term, 2^-32 of the maximum at least), sums and
+// the softmax's denominator are fp32 of the unrounded p.  The accumulator is
 // kept in units of the current block's v_scale and rescaled when that or m
 // changes, so that no scale enters an fp16.  A v_scale may be anything (append
 // gives a block of zeros 2^-100), so the unit stays within 2^64 of the
-// largest so far: sums of 2^30 positions keep below 2^112 units.  Blocks
+// largest so far: sums of 2^30 positions keep below 2^119 units.  Blocks
 // further down are added position by position, in fp32, if they hold anything
 // but zeros.  A piece's values are kept divided by their sum, as large as V.
 #include <cuda.h>
@@ -85,7 +88,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRescale = 8.f;  // log2 of how far m may be outgrown
+constexpr float kBelow = 7.f;    // log2 of how far m is put below the largest score
+constexpr float kRescale = 8.f;  // log2 of how far that may be outgrown: p <= 2^15
 constexpr float kUnitSpan = 5.421010862427522e-20f;  // 2^-64: the least unit of o beside the largest v_scale
 
 struct GqaArgs {
@@ -789,7 +793,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
       }
     }
-    // the running maxima, moved only where a score outgrows one by 2^8
+    // the rows' m, moved only where a score outgrows one by 2^15
     float top[NT][2];
     bool grew = false;
 #pragma unroll
@@ -799,7 +803,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         top[n][k] = fmaxf(s[0][n][k], s[0][n][2 + k]);
 #pragma unroll
         for (int mt = 1; mt < kRuns; ++mt) top[n][k] = fmaxf(top[n][k], fmaxf(s[mt][n][k], s[mt][n][2 + k]));
-        grew |= top[n][k] > m[n][k] + kRescale;
+        grew |= top[n][k] > m[n][k] + (kBelow + kRescale);
       }
     if (__any_sync(0xffffffffu, grew)) {
       float alpha[NT][2];
@@ -811,6 +815,7 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+          t -= kBelow;
           alpha[n][k] = 1.f;
           if (t > m[n][k]) {
             alpha[n][k] = fast_exp2(m[n][k] - t);

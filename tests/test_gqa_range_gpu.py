@@ -171,6 +171,26 @@ def test_decode_many_units_of_every_warp(h, hkv, sq, d, page, lens, grow, dtype)
     check_decode_on_gpu((kc, vc, ks, vs, table, ctx), q)
 
 
+def test_decode_long_tail_of_small_weights():
+    """2^14 weights of 2^-26.5 of the largest, whose own value is zero, make the
+    output.  In fp16 the largest weight is 2^7 at least, so that each of them is
+    off by 2^-25 of that at most; a warp has a whole context."""
+    import deepseek_v4_kernel as dk
+    n, b = 1 << 14, 12 * torch.cuda.get_device_properties(0).multi_processor_count
+    kc, vc = (torch.zeros(16, 1024, 1, 64, dtype=torch.uint8, device="cuda") for _ in range(2))
+    kc[0, 0], vc[:] = 0x38, 0x38  # 1.0
+    vc[0, 0] = 0
+    one = torch.ones(16, 1, device="cuda")
+    table = torch.arange(16, dtype=torch.int32, device="cuda").expand(b, 16).contiguous()
+    ctx = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    q = torch.ones(b, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    out, _ = dk.gqa_decode_fwd(q, kc, vc, one, one, table, ctx, sm_scale=26.5 * math.log(2) / 64)
+    tail = (n - 1) * 2.0 ** -26.5
+    want = tail / (1 + tail)
+    assert (out.double() - want).abs().max() <= U[q.dtype] * want + n * 2.0 ** -32
+    assert status() == 0
+
+
 # ------------------------------------------------------------------ weights
 @pytest.mark.parametrize("s_q", [1, 3, 40, 60])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), 1.0])
