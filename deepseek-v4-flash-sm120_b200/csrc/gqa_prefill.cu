@@ -86,6 +86,10 @@ constexpr int kEdgeRing = 2 * kMaxEdge;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;      // log2 of how far a maximum may be outgrown
+// P is 2^kBelow at the maximum, 2^15 at most: in fp16, where the small P of a
+// long prompt would else lose digits from 2^-14 and vanish from 2^-25 on, this
+// uses its range up to the end (to bf16 it is all the same).
+constexpr float kBelow = 7.f;  // and 0x1p-7f at the end
 constexpr int64_t kGroupBytes = 40 << 20;  // K and V of the heads that run at a time: a third of L2
 
 struct PrefillArgs {
@@ -598,7 +602,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : -m * c;
+        const float mc = kBelow - (m == -INFINITY ? 0.f : m * c);
         const uint64_t cc = pair(c, c), mm = pair(mc, mc);
         uint64_t l2[2] = {0, 0};  // two pairs of zeros
 #pragma unroll
@@ -687,7 +691,7 @@ gqa_prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           }
         }
       }
-      if (live) a.lse[(int64_t)(it.q0 + r) * a.h_q + it.head] = none ? -INFINITY : (m * c + log2f(l)) * kLn2;
+      if (live) a.lse[(int64_t)(it.q0 + r) * a.h_q + it.head] = none ? -INFINITY : (m * c + log2f(l * 0x1p-7f)) * kLn2;
       tc_fence_before();  // O is read before the arrival that lets the next item's MMAs write it
       release(w);
     }

@@ -12,6 +12,26 @@ from test_gqa_gpu import Cache, U, check_decode, check_weights, rand, status
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------ prompts
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prefill_long_tail_of_small_weights(dtype):
+    """As test_decode_long_tail_of_small_weights, of one query over a long
+    context; P is rounded to the inputs' type."""
+    import deepseek_v4_kernel as dk
+    n = 1 << 14
+    q = torch.ones(1, 1, 64, dtype=dtype, device="cuda")
+    k, v = torch.zeros(n, 1, 64, dtype=dtype, device="cuda"), torch.ones(n, 1, 64, dtype=dtype, device="cuda")
+    k[0], v[0] = 1, 0
+    cq, ck = (torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (1, n))
+    out, lse = dk.gqa_prefill_fwd(q, k, v, cq, ck, sm_scale=26.5 * math.log(2) / 64)
+    tail = (n - 1) * 2.0 ** -26.5
+    want = tail / (1 + tail)
+    assert (out.double() - want).abs().max() <= 2 * U[dtype] * want + n * 2.0 ** -32
+    size = 26.5 * math.log(2)  # T, and nearly the lse: 2^-19 T + 2^-20 + 2^-22 |lse|
+    assert abs(lse.item() - size - math.log1p(tail)) <= (2.0 ** -19 + 2.0 ** -22) * size + 2.0 ** -20
+    assert status() == 0
+
+
 # ------------------------------------------------------------------ decode
 def pool(nb, page, hkv, d, seed):
     """A filled cache: k_cache, v_cache, k_scale, v_scale."""
