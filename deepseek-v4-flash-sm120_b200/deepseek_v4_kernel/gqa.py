@@ -416,7 +416,10 @@ def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch
 def gqa_status(device: Optional[torch.device] = None) -> int:
     """Status word of the grouped-query kernels (0 = no error; 1 = a wait
     timed out and a call's outputs are invalid); clears it.  Synchronises."""
-    device = device or torch.device("cuda", torch.cuda.current_device())
+    device = torch.device("cuda" if device is None else device)
+    _require(device.type == "cuda", f"{device} is not a CUDA device")
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
     flags = ctypes.c_int()
     with torch.cuda.device(device):
         check("dsv4b_gqa_status", lib.dsv4b_gqa_status(ctypes.byref(flags), _stream(device)))

@@ -230,3 +230,11 @@ def test_weights_of_queries_that_are_left_out(s_q, what):
     c.kc[c.table[2, 0].item(), 3, :, 0] = 0x7F
     w = check_weights(c, q, lse=lse)
     assert (w[2] == 0).all()
+
+
+# ------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("device", [None, "cuda", "cuda:0"])
+def test_status_takes_any_form_of_a_device(device):
+    import deepseek_v4_kernel as dk
+    assert dk.gqa_status(device) == 0
+    assert dk.gqa_status(None if device is None else torch.device(device)) == 0
