@@ -371,6 +371,30 @@ def _weights(t: torch.Tensor, c: _Cache, name: str, written: bool) -> int:
     return t.size(2)
 
 
+def _row_starts(t: torch.Tensor, base: int) -> torch.Tensor:
+    """Where the rows of a tensor begin, in elements from ``base`` on, ascending (on the host)."""
+    at = torch.tensor([(t.data_ptr() - base) // t.element_size()], device="cpu")
+    for n, x in zip(t.shape[:-1], t.stride()):
+        at = (at[:, None] + torch.arange(n, device="cpu") * x).view(-1)
+    return at.sort()[0]
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [b, h_kv, width] tensors of one type share no element."""
+    pa, pb, sa, sb = a.data_ptr(), b.data_ptr(), a.stride(), b.stride()
+
+    def end(t, p, st):
+        return p + t.element_size() * (sum((n - 1) * x for n, x in zip(t.shape, st)) + 1)
+
+    if end(a, pa, sa) <= pb or end(b, pb, sb) <= pa:
+        return True
+    x, y = _row_starts(a, pa), _row_starts(b, pa)
+    behind = torch.searchsorted(x, y)  # the first row of a at or behind each of b's
+    after = torch.where(behind < len(x), x[behind.clamp(max=len(x) - 1)], y + b.size(2))
+    before = torch.where(behind > 0, x[(behind - 1).clamp(min=0)], y - a.size(2))
+    return bool((after >= y + b.size(2)).all() and (before + a.size(2) <= y).all())
+
+
 def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                     block_table: torch.Tensor, context_lens: torch.Tensor, weights: torch.Tensor, budget: int,
                     recent: int, new_block_table: torch.Tensor, new_weights: Optional[torch.Tensor] = None
@@ -381,6 +405,9 @@ def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch
     first), all of them where there are no more.  They become, in order, the
     first positions of the blocks of ``new_block_table`` [b, >= ceil(budget /
     P)], which must be blocks that the call does not read, none twice.
+
+    ``new_weights``, if given, must share no memory with ``weights``.  A
+    sequence counts as at most width positions long.
 
     Returns (kept int32 [b, h_kv, budget], -1 behind the new length;
     new_weights fp32 [b, h_kv, >= budget], the kept positions' weights, 0
@@ -402,7 +429,7 @@ def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch
     else:
         new_width = _weights(new_weights, c, "new_weights", True)
         _require(new_width >= budget, "new_weights is narrower than the budget")
-        _require(new_weights.data_ptr() != weights.data_ptr(), "new_weights must not be weights")
+        _require(_apart(weights, new_weights), "new_weights must not share memory with weights")
     kept = torch.empty((c.b, c.h_kv, budget), dtype=torch.int32, device=dev)
     new_lens = torch.empty((c.b,), dtype=torch.int32, device=dev)
     ws, ns = weights.stride(), new_weights.stride()

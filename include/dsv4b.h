@@ -427,7 +427,9 @@ DSV4B_API int dsv4b_gqa_attention_weights(const dsv4b_gqa_cache* c, const dsv4b_
  * new_weights fp32 [b, h_kv, new_width >= budget] (0 behind it) and
  * new_lens int32 [b] = min(context_lens, budget).  No block of new_table
  * may be one that the call reads, or be there twice.  weights fp32 [b,
- * h_kv, width]: a sequence counts as at most `width` positions long. */
+ * h_kv, width]: a sequence counts as at most `width` positions long.
+ * new_weights, kept and new_lens must share no memory with the inputs:
+ * they are written while those are read. */
 typedef struct dsv4b_gqa_evict_params {
   int32_t budget, recent;    /* 0 <= recent <= budget, budget >= 1 */
   const float* weights;

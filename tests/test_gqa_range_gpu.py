@@ -238,3 +238,27 @@ def test_status_takes_any_form_of_a_device(device):
     import deepseek_v4_kernel as dk
     assert dk.gqa_status(device) == 0
     assert dk.gqa_status(None if device is None else torch.device(device)) == 0
+
+
+def test_evict_weights_and_new_weights_of_one_tensor():
+    """Column ranges of one tensor are taken, ranges that share an element are
+    refused before anything is written."""
+    import deepseek_v4_kernel as dk
+    c = Cache([300, 150], 32, 2, 64, seed=15, spare=8)
+    g = torch.Generator(device="cuda").manual_seed(50)
+    w = torch.rand(2, 2, 300, generator=g, device="cuda")
+    new = c.free[:8].int().view(2, 4).cuda()
+    want = dk.gqa_cache_evict(*c.cuda(), w, 100, 10, new)
+    both = torch.full((2, 2, 420), 3.0, device="cuda")
+    both[..., :300] = w
+    for into in (both[..., 300:410], both.transpose(0, 1)[..., 300:410]):
+        got = dk.gqa_cache_evict(*c.cuda(), both[..., :300], 100, 10, new, new_weights=into)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][..., :100], want[1]) and torch.equal(got[2], want[2])
+        assert (both[..., 400:410] == 0).all() and (both[..., 410:] == 3.0).all() and torch.equal(both[..., :300], w)
+    dev = c.cuda()
+    before = [t.clone() for t in dev]
+    for bad in (both[..., 4:104], both[..., 299:410], both[:, 1:].expand(2, 2, 420)):
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_evict(*dev, both[..., :300], 100, 10, new, new_weights=bad)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.view(torch.uint8), x.view(torch.uint8)) for t, x in zip(dev, before)) and status() == 0
