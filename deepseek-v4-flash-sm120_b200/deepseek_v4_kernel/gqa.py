@@ -143,6 +143,27 @@ def _rows16(t: torch.Tensor, name: str, distinct: bool = False):
     return ptr, st
 
 
+def _row_starts(t: torch.Tensor, base: int) -> torch.Tensor:
+    """Where the rows of a tensor begin, in elements from ``base`` on, ascending (on the host)."""
+    at = torch.tensor([(t.data_ptr() - base) // t.element_size()], device="cpu")
+    for n, x in zip(t.shape[:-1], t.stride()):
+        at = (at[:, None] + torch.arange(n, device="cpu") * x).view(-1)
+    return at.sort()[0]
+
+
+def _own_rows(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor, to be written, of which two rows share an element."""
+    if t.is_contiguous():
+        return
+    width = need = t.size(-1)
+    for x, n in sorted((x, n) for x, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        if x < need:  # rows inside one another's gaps?
+            at = _row_starts(t, t.data_ptr())
+            _require(bool((at[1:] - at[:-1] >= width).all()), f"{name}'s rows overlap: strides {t.stride()}")
+            return
+        need += x * (n - 1)
+
+
 def _fp8_cache(t: torch.Tensor, scale: torch.Tensor, name: str, dev: torch.device):
     """The pointers and the three byte strides of a cache tensor and its scales."""
     if t.dtype not in _FP8 or t.dim() != 4 or t.device != dev:
@@ -246,6 +267,8 @@ def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
         out = q.new_empty((total_q, h_q, d_v))
     elif out.dtype != q.dtype or out.shape != (total_q, h_q, d_v) or out.device != dev:
         raise RuntimeError(f"out must be {q.dtype} {[total_q, h_q, d_v]} on {dev}")
+    else:
+        _own_rows(out, "out")
     lse = torch.empty((total_q, h_q), dtype=torch.float32, device=dev)
     if total_q == 0:
         return out, lse
@@ -318,6 +341,8 @@ def gqa_decode_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         out = q.new_empty(q.shape)
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev:
         raise RuntimeError(f"out must be {q.dtype} {list(q.shape)} on {dev}")
+    else:
+        _own_rows(out, "out")
     op, so = _rows16(out, "out", True)
     lse = torch.empty((c.b, h_q, s_q), dtype=torch.float32, device=dev)
     with _on_device(dev):
@@ -366,17 +391,9 @@ def _weights(t: torch.Tensor, c: _Cache, name: str, written: bool) -> int:
     if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (c.b, c.h_kv) or t.size(2) < 1 or \
             t.stride(2) != 1 or t.device != c.dev:
         raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width] on {c.dev} with a contiguous last dim")
-    if written and any(s < t.size(2) and n > 1 for s, n in zip(t.stride()[:2], t.shape)):
-        raise RuntimeError(f"{name}'s rows overlap: strides {t.stride()}")
+    if written:
+        _own_rows(t, name)
     return t.size(2)
-
-
-def _row_starts(t: torch.Tensor, base: int) -> torch.Tensor:
-    """Where the rows of a tensor begin, in elements from ``base`` on, ascending (on the host)."""
-    at = torch.tensor([(t.data_ptr() - base) // t.element_size()], device="cpu")
-    for n, x in zip(t.shape[:-1], t.stride()):
-        at = (at[:, None] + torch.arange(n, device="cpu") * x).view(-1)
-    return at.sort()[0]
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:

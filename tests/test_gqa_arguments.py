@@ -32,3 +32,18 @@ def test_tensors_apart():
     for a, x in zip(views, sets):
         for b, y in zip(views, sets):
             assert _apart(a, b) == (not x & y), (a.shape, a.stride(), b.shape, b.stride())
+
+
+@pytest.mark.parametrize("shape,strides", [((2, 3, 8), (24, 8, 1)), ((2, 3, 8), (8, 16, 1)), ((2, 3, 8), (8, 8, 1)), ((2, 3, 8), (7, 40, 1)),
+                                           ((2, 3, 8), (40, 4, 1)), ((1, 3, 8), (0, 8, 1)), ((2, 1, 8), (8, 3, 1)), ((2, 3, 8), (0, 8, 1)),
+                                           ((2, 2, 8), (24, 32, 1)), ((2, 2, 8), (24, 30, 1)), ((2, 2, 8), (8, 15, 1)), ((4, 3, 8), (48, 16, 1)),
+                                           ((4, 3, 8), (40, 16, 1)), ((2, 3, 4, 8), (96, 8, 24, 1)), ((2, 3, 4, 8), (88, 8, 24, 1)), ((3, 2, 2, 8), (8, 24, 48, 1))])
+def test_written_rows_must_not_overlap(shape, strides):
+    from deepseek_v4_kernel.gqa import _own_rows
+    t = torch.zeros(4096).as_strided(shape, strides)
+    at = sum(torch.arange(n).view([-1 if i == j else 1 for j in range(len(shape))]) * x for i, (n, x) in enumerate(zip(shape, strides)))
+    if at.unique().numel() == at.numel():
+        _own_rows(t, "out")
+    else:
+        with pytest.raises(RuntimeError, match="overlap"):
+            _own_rows(t, "out")

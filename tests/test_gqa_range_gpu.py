@@ -262,3 +262,20 @@ def test_evict_weights_and_new_weights_of_one_tensor():
             dk.gqa_cache_evict(*dev, both[..., :300], 100, 10, new, new_weights=bad)
     torch.cuda.synchronize()
     assert all(torch.equal(t.view(torch.uint8), x.view(torch.uint8)) for t, x in zip(dev, before)) and status() == 0
+
+
+def test_written_tensors_whose_rows_overlap_are_refused():
+    import deepseek_v4_kernel as dk
+    c = Cache([70, 64], 32, 2, 128, seed=1)
+    kc, vc, ks, vs, table, ctx = dev = c.cuda()
+    q = torch.zeros(2, 2, 4, 128, dtype=torch.bfloat16, device="cuda")
+    lse = torch.zeros(2, 4, 2, device="cuda")
+    half = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        dk.gqa_decode_fwd(q, *dev, out=half.as_strided(q.shape, (512, 512, 128, 1)))
+    with pytest.raises(RuntimeError, match="overlap"):
+        dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, weights=torch.zeros(500, device="cuda").as_strided((2, 2, 96), (96, 96, 1)))
+    x = torch.zeros(9, 4, 128, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        dk.gqa_prefill_fwd(x, x, x, cu, out=half.as_strided(x.shape, (128, 128, 1)))
