@@ -39,6 +39,8 @@ from .ops import _on_device
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _FP8 = (torch.float8_e4m3fn, torch.uint8)
+_MAX_FP32 = torch.finfo(torch.float32).max
+_MAX_POSITIONS = 1 << 30  # of a sequence, its weights and its budget
 
 
 class GqaCache(ctypes.Structure):
@@ -213,6 +215,13 @@ class _Cache:
 _PAGES = (16, 32, 64, 128, 256, 512, 1024)
 
 
+def _scale(sm_scale: Optional[float], d: int) -> float:
+    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 0.0 < scale < _MAX_FP32:
+        raise RuntimeError(f"sm_scale must be positive, in fp32 too, got {scale}")
+    return scale
+
+
 def _query(q, c: _Cache, sm_scale: Optional[float]):
     """The packed query, s_q and h_q."""
     if q.dim() != 4 or q.dtype not in _DTYPES or q.device != c.dev:
@@ -221,9 +230,7 @@ def _query(q, c: _Cache, sm_scale: Optional[float]):
     if b != c.b or d != c.d or s_q < 1 or h_q < 1 or h_q % c.h_kv:
         raise RuntimeError(f"q {tuple(q.shape)} does not match {c.b} sequences, {c.h_kv} KV heads, d {c.d}")
     ptr, st = _rows16(q, "q")
-    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale < float("inf"):
-        raise RuntimeError(f"sm_scale must be positive, got {scale}")
+    scale = _scale(sm_scale, d)
     return _PACK_QUERY(_DTYPES[q.dtype], s_q, h_q, scale, ptr, st[0], st[1], st[2]), s_q, h_q
 
 
@@ -252,9 +259,7 @@ def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
         raise RuntimeError(f"(d_qk, d_v) = {(d_qk, d_v)}: (64, 64), (128, 128) or (192, 128) is supported")
     if h_kv < 1 or h_q < 1 or h_q % h_kv:
         raise RuntimeError(f"{h_q} query heads are not a multiple of {h_kv} KV heads")
-    scale = d_qk ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale < float("inf"):
-        raise RuntimeError(f"sm_scale must be positive, got {scale}")
+    scale = _scale(sm_scale, d_qk)
     b = cu_seqlens_q.numel() - 1
     _require(b >= 1, "cu_seqlens_q must have b + 1 >= 2 entries")
     cq = _int32(cu_seqlens_q, b + 1, "cu_seqlens_q", dev)
@@ -297,7 +302,7 @@ def gqa_cache_append(k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
     be written by two sequences of one call."""
     c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
     dev = c.dev
-    n = k.size(0)
+    n = k.size(0) if k.dim() else 0
     if k.dim() != 3 or k.dtype not in _DTYPES or v.dtype != k.dtype or k.shape != (n, c.h_kv, c.d) or \
             v.shape != k.shape or k.device != dev or v.device != dev:
         raise RuntimeError(f"k and v must be bf16 / fp16 [n, {c.h_kv}, {c.d}] on {dev}")
@@ -373,7 +378,8 @@ def gqa_attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Ten
     if weights is None:
         _require(not accumulate, "accumulate needs weights to add to")
         width = c.width * c.page if max_context is None else int(max_context)
-        _require(width > 0, "max_context must be positive")
+        if not 0 < width <= _MAX_POSITIONS:
+            raise RuntimeError(f"max_context must be positive and at most 2^30, got {width}")
         weights = torch.empty((c.b, c.h_kv, width), dtype=torch.float32, device=dev)
     else:
         _require(max_context is None, "max_context is for a new tensor: weights has a width already")
@@ -389,8 +395,8 @@ def gqa_attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Ten
 def _weights(t: torch.Tensor, c: _Cache, name: str, written: bool) -> int:
     """The width of a weights tensor."""
     if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (c.b, c.h_kv) or t.size(2) < 1 or \
-            t.stride(2) != 1 or t.device != c.dev:
-        raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width] on {c.dev} with a contiguous last dim")
+            t.size(2) > _MAX_POSITIONS or t.stride(2) != 1 or t.device != c.dev:
+        raise RuntimeError(f"{name} must be float32 [{c.b}, {c.h_kv}, width <= 2^30] on {c.dev} with a contiguous last dim")
     if written:
         _own_rows(t, name)
     return t.size(2)
@@ -433,8 +439,8 @@ def gqa_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch
     c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
     dev = c.dev
     budget, recent = int(budget), int(recent)
-    if budget < 1 or not 0 <= recent <= budget:
-        raise RuntimeError(f"budget {budget}, recent {recent}: 0 <= recent <= budget, 1 <= budget")
+    if not 1 <= budget <= _MAX_POSITIONS or not 0 <= recent <= budget:
+        raise RuntimeError(f"budget {budget}, recent {recent}: 0 <= recent <= budget, 1 <= budget <= 2^30")
     width = _weights(weights, c, "weights", False)
     new_table, new_stride, new_blocks = _table(new_block_table, c.b, "new_block_table", dev)
     _require(new_table != c.table_ptr, "new_block_table must not be block_table")

@@ -279,3 +279,34 @@ def test_written_tensors_whose_rows_overlap_are_refused():
     cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="overlap"):
         dk.gqa_prefill_fwd(x, x, x, cu, out=half.as_strided(x.shape, (128, 128, 1)))
+
+
+def test_arguments_past_their_types_are_refused():
+    """Numbers that fp32 or 32 bits do not hold, tensors without dims: RuntimeError, before any memory is asked for."""
+    import deepseek_v4_kernel as dk
+    c = Cache([70, 64], 32, 2, 128, seed=1, spare=8)
+    kc, vc, ks, vs, table, ctx = dev = c.cuda()
+    q = torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    lse, w = torch.zeros(2, 4, 1, device="cuda"), torch.zeros(2, 2, 96, device="cuda")
+    cu, new = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), c.free[:4].int().view(2, 2).cuda()
+    x = torch.zeros(9, 4, 128, dtype=torch.bfloat16, device="cuda")
+    cx = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    for scale in (3.5e38, 1e300, 1e-46):
+        with pytest.raises(RuntimeError):
+            dk.gqa_decode_fwd(q, *dev, sm_scale=scale)
+        with pytest.raises(RuntimeError):
+            dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, sm_scale=scale)
+        with pytest.raises(RuntimeError):
+            dk.gqa_prefill_fwd(x, x, x, cx, sm_scale=scale)
+    for width in ((1 << 30) + 1, (1 << 32) + 96, -(1 << 32) + 96):
+        with pytest.raises(RuntimeError, match="max_context"):
+            dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, max_context=width)
+        with pytest.raises(RuntimeError, match="budget"):
+            dk.gqa_cache_evict(*dev, w, width, 4, new)
+    wide = torch.zeros(1, device="cuda").expand(2, 2, (1 << 32) + 96)
+    with pytest.raises(RuntimeError):
+        dk.gqa_attention_weights(q, lse, kc, ks, table, ctx, weights=wide)
+    for bad in (q[0, 0, 0, 0], q[0, 0, 0]):
+        with pytest.raises(RuntimeError):
+            dk.gqa_cache_append(bad, bad, cu, ctx, table, kc, vc, ks, vs)
+    assert status() == 0
