@@ -90,9 +90,10 @@ SCALES = {"zero blocks": [17, Z, -8, 17, Z], "large": [119, -8, 119, Z, 3], "upw
           "downwards": [100, 50, 0, -50, -100, -126], "tiny": [0, -127, -140, -8], "near": [-8, -30, -7, -50]}
 
 
-@pytest.mark.parametrize("h,d,page", [(4, 128, 16), (16, 128, 64), (3, 64, 32), (12, 64, 16)])
+@pytest.mark.parametrize("h,d,page,s_q", [(4, 128, 16, 1), (16, 128, 64, 1), (3, 64, 32, 1), (12, 64, 16, 1), (2, 128, 16, 4),
+                                          (5, 64, 16, 5), (1, 128, 32, 70)])
 @pytest.mark.parametrize("kind", SCALES)
-def test_decode_value_scales_far_apart(kind, h, d, page):
+def test_decode_value_scales_far_apart(kind, h, d, page, s_q):
     """Blocks whose v_scale differ by up to 2^219, subnormal ones and blocks of zeros (Z) among them."""
     g = torch.Generator(device="cuda").manual_seed(40)
     lens = [(211 * i) % 1900 for i in range(120)] + [9000]
@@ -112,7 +113,7 @@ def test_decode_value_scales_far_apart(kind, h, d, page):
     vs[:, 0] = torch.exp2(exps).float().cuda()
     vc.view(torch.uint8)[zero.cuda()] = 0
     ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
-    check_decode_on_gpu((kc, vc, ks, vs, table.cuda(), ctx), rand(g, len(lens), 1, h, d))
+    check_decode_on_gpu((kc, vc, ks, vs, table.cuda(), ctx), rand(g, len(lens), s_q, h, d))
 
 
 def test_decode_after_append_of_zeros():
