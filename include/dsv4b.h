@@ -399,7 +399,9 @@ DSV4B_API int dsv4b_gqa_decode_workspace_bytes(int device, int d, size_t* bytes)
 
 /* Attention over the cache.  out [b, s_q, h_q, d] in q's type (element
  * strides, positive multiples of 8), lse fp32 [b, h_q, s_q]; a query that sees no
- * position gets out = 0 and lse = -inf. */
+ * position gets out = 0 and lse = -inf.  Scales may be of any size, 0 and
+ * subnormal ones too; what lies 2^139 below the largest v_scale of a
+ * sequence's blocks may be lost. */
 DSV4B_API int dsv4b_gqa_decode(const dsv4b_gqa_cache* c, const dsv4b_gqa_query* q, void* out, int64_t stride_o_b,
                                int64_t stride_o_s, int64_t stride_o_h, float* lse, void* workspace,
                                size_t workspace_bytes, void* stream);

@@ -44,7 +44,10 @@ def pool(nb, page, hkv, d, seed):
 def check_decode_on_gpu(dev, q, scale=None):
     """check_decode for long contexts, with the 64-bit sums on the GPU.  A
     weight's rounding to fp16 is off by no more than the weight itself, and
-    a warp's sums have four steps for each of its units, off by 2^-23 each."""
+    a warp's sums have four steps for each of its units, off by 2^-23 each.  The
+    sums are fp32 in units of up to the sequence's largest v_scale S, whether a
+    row sees it or not: a factor between two units is off by 2^-150 at least,
+    that times 448 S, and 2^16 sums of steps of 2^-149 S over 2^7: 2^-139 S."""
     import deepseek_v4_kernel as dk
     kc, vc, ks, vs, table, ctx = dev
     b, s_q, h, d = q.shape
@@ -74,8 +77,9 @@ def check_decode_on_gpu(dev, q, scale=None):
             wl = torch.logsumexp(s, -1)
             p = torch.where(sees[:, None], torch.exp(s - wl[..., None]), 0)
             want, mag, rest = p @ v, p @ v.abs(), p.clamp(max=2.0 ** -25) @ v.abs()
+            most = vs[blk, kvh].double().max()
             e = 2.0 ** -19 * size + 2.0 ** -20 + steps
-            tol = u * want.abs() + (2.0 ** -11 + 2 * e)[..., None] * mag + rest + 1e-30
+            tol = u * want.abs() + (2.0 ** -11 + 2 * e)[..., None] * mag + rest + 2.0 ** -139 * most + 1e-30
             o, l = got[i, :, kvh * g:(kvh + 1) * g].double(), lse[i, kvh * g:(kvh + 1) * g].T.double()
             off = (o - want).abs()
             assert (off <= tol).all(), (i, kvh, off.max().item(), int((~(off <= tol)).sum()))
@@ -114,6 +118,19 @@ def test_decode_value_scales_far_apart(kind, h, d, page, s_q):
     vc.view(torch.uint8)[zero.cuda()] = 0
     ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
     check_decode_on_gpu((kc, vc, ks, vs, table.cuda(), ctx), rand(g, len(lens), s_q, h, d))
+
+
+@pytest.mark.parametrize("exps", [[-80, 40], [118, -8], [-8, -8, 118, 60], [0, 100, -30]])
+@pytest.mark.parametrize("h,d", [(2, 128), (8, 64)])
+def test_decode_drafts_that_do_not_see_the_largest_values(exps, h, d):
+    """Blocks of 16 whose v_scale lie up to 2^130 apart, queries that see one, two and more of them."""
+    lens = list(range(1, 131))
+    kc, vc, ks, vs = pool(9 * len(lens), 16, 1, d, 43)
+    table = torch.arange(9 * len(lens), dtype=torch.int32, device="cuda").view(len(lens), 9)
+    vs.view(len(lens), 9)[:] = torch.exp2(torch.tensor([exps[i % len(exps)] for i in range(9)]).float())
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(51)
+    check_decode_on_gpu((kc, vc, ks, vs, table, ctx), rand(g, len(lens), 64, h, d))
 
 
 def test_decode_after_append_of_zeros():
