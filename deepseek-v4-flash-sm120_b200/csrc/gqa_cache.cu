@@ -134,8 +134,10 @@ __device__ __forceinline__ int owner_of(int w, int b, F f) {
 // twice (the second time from L2).
 //
 // 16 prompts of 60 to 4,100 tokens, 8 heads, d = 128 (111 MB): 27 us, 4.1
-// TB/s against 6.5 of a copy; 256 tokens of as many sequences: 6.3 us, a
-// chain of dependent loads (offsets, block id, scale, row) behind a launch.
+// TB/s against 6.5 of a copy: 124 registers leave two CTAs to an SM, 4.2 waves
+// of them that begin with a chain of dependent loads (offsets, block id, scale,
+// row); the issue slots are half full.  256 tokens of as many sequences: 6.3
+// us, that chain behind a launch.
 //
 // Which blocks a sequence touches is not known on the host.  Sequence i
 // with n_i new tokens touches at most n_i / P + 2 blocks, so the items
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) gqa_evict_select_kernel(const 
 // the rows of K and V, 16 bytes per thread and load, and, while those are on
 // their way, the largest of the sources' scales.  Bound by the kept bytes,
 // read (rows at random places) and written once: with the selection, 4,096
-// of up to 32,768 positions of 32 sequences, 8 heads (560 MB in all) take 128
+// of up to 32,768 positions of 32 sequences, 8 heads (560 MB in all) take 129
 // us, 97 of them here, 5.5 TB/s; 2,048 of 8,192 of one sequence 14.5 us, two
 // launches' and chains' latency.
 constexpr int kGatherThreads = 128;

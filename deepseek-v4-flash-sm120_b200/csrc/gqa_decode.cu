@@ -23,11 +23,12 @@
 // register or an issue slot spent on them.
 //
 // Measured, d = 128, against 6.5 TB/s of a copy: 16 sequences of 131,072
-// positions, 8 KV heads of 16 rows (4.1 GB) 720 us, 5.7 TB/s; 32 of 1,000 to
-// 32,768 with 8 rows (554 MB) 123 us, 4.5 TB/s; one of 4,096 (8.4 MB) 16.5.
-// The last is what a call takes whatever its size (launch, the list, the
-// first tiles behind their page ids, the joins), of which the middle one
-// shows about 14 us; it also loses to warps of a CTA that end apart.
+// positions, 8 KV heads of 16 rows (4.1 GB) 722 us, 5.7 TB/s (835 where it runs
+// for long, at the power limit's 1.7 GHz); 32 of 1,000 to 32,768 with 8 rows
+// (554 MB) 126 us, 4.4 TB/s; one of 4,096 (8.4 MB) 16.6.  The last is what a
+// call takes whatever its size (launch, the list, the first tiles behind their
+// page ids, the joins), of which the middle one shows about 14 us; for the rest
+// its warps wait on memory for 40 % of their time and at barriers for 4 %.
 //
 // Products.  mma.sync m16n8k16 with fp16 operands, positions (or dims of V)
 // as M and rows as N = 8: s^T = k q^T, out^T = v^T p^T.  The operands of
@@ -48,7 +49,8 @@
 // blocks (movmatrix) gives p^T's fragments.
 //
 // Numbers.  q is scaled by a power of two per row so that fp16 holds it
-// (bf16 has fewer digits; what lies 2^-27 below the row's largest is lost).
+// (bf16 has fewer digits; what lies 2^-27 below the row's largest loses some,
+// 2^-37 below it all).
 // p is relative to m, which lies 2^7 below the running maximum and is moved
 // only when a score outgrows that by 2^8, so p <= 2^15: fp16's range is used
 // up to its end, for the small p of a long context (2^-14 of the maximum and
@@ -1151,7 +1153,7 @@ struct Walk {
 // rows' q in registers.  A thread adds p of its rows, then the four c are
 // joined by a halving exchange that leaves one position per lane.  Bound by
 // its start and K's bytes: 32 sequences of 500 to 16,384, 8 KV heads, d = 64
-// (95 MB) 29 us.
+// (95 MB) 30 us.
 template <int D>
 struct Wts {
   static constexpr int kUnit = 64;
@@ -1332,7 +1334,7 @@ gqa_weights_kernel(const __grid_constant__ CUtensorMap tk, const GqaArgs a) {
 // TMEM: K of two units (2 x 64 columns), S of three (3 x 128).
 //
 // With many rows the exponentials bound it, 16 a cycle and SM: 128 rows of
-// 105,000 positions and 8 heads are 108 M of them, 27 us; it takes 59, of
+// 105,000 positions and 8 heads are 108 M of them, 27 us; it takes 60, of
 // which 6 pass before the first S.  (S in tiles of 64 rows took 63: an MMA
 // whose A is in TMEM takes 64 cycles whatever N is.  Two groups: 68.)  With
 // few it is K's bytes.  mma.sync, an n-tile of rows after another, was the

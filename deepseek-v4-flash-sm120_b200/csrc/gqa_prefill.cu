@@ -40,13 +40,16 @@
 // latter: a query that does see one has the value added at the end.
 //
 // Measured (bf16 GEMM of a library on this GPU: 1,663 TFLOP/s in a burst,
-// 1,404 for seconds): one prompt of 16,384, 32 heads over 8, d = 128, 1.81 ms,
-// 1,215 TFLOP/s (1,096 when it runs for long, at the power limit's clock); 24
-// prompts of up to 4,099, 64 heads, 0.76 ms; two of up to 2,600, 128 heads of
-// 192 / 128, 0.59 ms.  The tensor core is the bound: its MMAs of 64 cycles
-// take 70 beside busy warps, and P is always there when it waits.  The shorter
-// prompts lose what their edge tiles' masked halves and the items' starts and
-// ends take.
+// 1,404 for seconds), in a burst at 1,965 MHz and for seconds at the power
+// limit's 1,665 to 1,750: one prompt of 16,384, 32 heads over 8, d = 128, 1.82
+// ms, 1,210 TFLOP/s, and 2.10; 24 prompts of up to 4,099, 64 heads, 0.75 and
+// 0.84; two of up to 2,600, 128 heads of 192 / 128, 0.60 and 0.69.  A pair of
+// tiles takes 4,000 cycles: its MMAs need 2,048 of the tensor core (2,330 as
+// they are issued), its exponentials 2,048 of their unit.  Both are busy for 48
+// % of the time (4,096 tokens), the issue slots for 30: no unit is full, the
+// chain from S over P to O of the two tiles is what takes the time.  The
+// shorter prompts also lose their edge tiles' masked halves and the items'
+// starts and ends.
 //
 // The list of items needs no lengths on the host: sequence i has the tiles
 // from cu_i / 256 + i on, at least as many as it can fill.  The last tiles

@@ -246,7 +246,7 @@ def gqa_prefill_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlen
     all its keys, the one before it one less, and so on.  Returns (out
     [total_q, h_q, d_v], lse fp32 [total_q, h_q], natural log); a query that
     sees no key gets 0 and -inf.  Rows behind the last sequence are not
-    written."""
+    written.  ``out`` may be q itself, but share no memory with k or v."""
     dev = q.device
     _require(q.is_cuda, "q must be a CUDA tensor")
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
@@ -338,7 +338,7 @@ def gqa_decode_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q bf16 / fp16 [b, s_q, h_q, d]; ``context_lens`` counts the queries' own
     positions, and query x sees those up to its own.  Returns (out [b, s_q,
     h_q, d] in q's type, lse fp32 [b, h_q, s_q], natural log); a query that
-    sees no position gets 0 and -inf."""
+    sees no position gets 0 and -inf.  ``out`` may be q itself."""
     c = _Cache(k_cache, v_cache, k_scale, v_scale, block_table, context_lens)
     dev = c.dev
     qq, s_q, h_q = _query(q, c, sm_scale)

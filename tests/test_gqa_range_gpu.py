@@ -328,3 +328,37 @@ def test_arguments_past_their_types_are_refused():
         with pytest.raises(RuntimeError):
             dk.gqa_cache_append(bad, bad, cu, ctx, table, kc, vc, ks, vs)
     assert status() == 0
+
+
+# ------------------------------------------------------------------ together
+def test_out_may_be_q():
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(48)
+    c = Cache([3000, 40, 900], 64, 2, 128, seed=14)
+    dev, q = c.cuda(), rand(g, 3, 5, 8, 128)
+    x, kv = rand(g, 1500, 8, 128), rand(g, 1500, 2, 128)
+    cu = torch.tensor([0, 900, 1000, 1500], dtype=torch.int32, device="cuda")
+    want = dk.gqa_decode_fwd(q, *dev) + dk.gqa_prefill_fwd(x, kv, kv, cu)
+    got = dk.gqa_decode_fwd(q, *dev, out=q) + dk.gqa_prefill_fwd(x, kv, kv, cu, out=x)
+    assert got[0].data_ptr() == q.data_ptr() and got[2].data_ptr() == x.data_ptr()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and status() == 0
+
+
+@pytest.mark.parametrize("s", [1, 24])
+def test_weights_of_a_prompts_last_queries(s):
+    """A prompt, its append, and the weights that its last queries gave the
+    cached positions, with the prompt's own lse."""
+    import deepseek_v4_kernel as dk
+    g = torch.Generator(device="cuda").manual_seed(52)
+    lens, h, hkv, d, page = [300, 24, 131], 8, 2, 128, 32
+    cu = torch.tensor([0, 300, 324, 455], dtype=torch.int32, device="cuda")
+    q, k, v = rand(g, 455, h, d), rand(g, 455, hkv, d), rand(g, 455, hkv, d)
+    _, lse = dk.gqa_prefill_fwd(q, k, v, cu)
+    c = Cache([0, 0, 0], page, hkv, d, seed=1, spare=30, width=10)
+    c.table[:] = c.free[:30].view(3, 10)
+    c.ctx = torch.tensor(lens, dtype=torch.int32)
+    kc, vc, ks, vs, table, ctx = c.cuda()
+    dk.gqa_cache_append(k, v, cu, ctx, table, kc, vc, ks, vs)
+    c.kc, c.ks = kc.view(torch.uint8).cpu(), ks.cpu()
+    rows = cu[1:, None].long() - s + torch.arange(s, device="cuda")
+    check_weights(c, q[rows], lse=lse[rows].transpose(1, 2).contiguous())
