@@ -23,7 +23,7 @@
 // register or an issue slot spent on them.
 //
 // Measured, d = 128, against 6.5 TB/s of a copy: 16 sequences of 131,072
-// positions, 8 KV heads of 16 rows (4.1 GB) 722 us, 5.7 TB/s (835 where it runs
+// positions, 8 KV heads of 16 rows (4.1 GB) 728 us, 5.6 TB/s (835 where it runs
 // for long, at the power limit's 1.7 GHz); 32 of 1,000 to 32,768 with 8 rows
 // (554 MB) 126 us, 4.4 TB/s; one of 4,096 (8.4 MB) 16.6.  The last is what a
 // call takes whatever its size (launch, the list, the first tiles behind their
@@ -60,8 +60,9 @@
 // kept in units of the current block's v_scale and rescaled when that or m
 // changes, so that no scale enters an fp16.  A v_scale may be anything (append
 // gives a block of zeros 2^-100), so the unit stays within 2^64 of the
-// largest so far: sums of 2^30 positions keep below 2^119 units.  Blocks
-// further down are added position by position, in fp32, if they hold anything
+// largest so far: sums of 2^30 positions keep below 2^119 units, and go up to
+// any larger unit by factors of 2^-100 at least.  Blocks further down leave
+// the unit and are added position by position, in fp32, if they hold anything
 // but zeros.  A piece's values are kept divided by their sum, as large as V.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -851,21 +852,28 @@ gqa_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     float v_unit = sh.unit[warp];
 #pragma unroll
     for (int mt = 0; mt < kRuns; ++mt) {
-      // o into units of these positions' v_scale (0: they add nothing), or
-      // into the least one if that is larger
+      // o into units of these positions' v_scale (0: they add nothing) unless it
+      // is too small for one; a factor below 2^-126 would lose digits that o has
       const bool there = (now.held >> mt) & 1 && now.vs[mt] != 0.f;
       if (there && now.vs[mt] != v_unit) {  // the same in all lanes
-        const float least = sh.least_unit[warp], size = fabsf(now.vs[mt]), old = v_unit;
-        v_unit = size < least ? least : now.vs[mt];
-        edge |= size < least;
-        sh.least_unit[warp] = fmaxf(least, size * kUnitSpan);
-        const float r = old / v_unit;
+        const float least = sh.least_unit[warp], size = fabsf(now.vs[mt]);
+        if (size < least) {
+          edge = true;
+        } else {
+          sh.least_unit[warp] = fmaxf(least, size * kUnitSpan);
+#pragma unroll 1
+          for (int i = 0; i < 3 && v_unit != now.vs[mt]; ++i) {
+            const bool far = fabsf(v_unit) * 0x1p100f < size && v_unit != 0.f;
+            const float next = far ? v_unit * 0x1p100f : now.vs[mt], r = far ? 0x1p-100f : v_unit / next;
+            v_unit = next;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+            for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+              for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[i][n][k] *= r;
+                for (int k = 0; k < 4; ++k) o[j][n][k] *= r;
+          }
+        }
       }
       // the four positions whose p this thread holds
       const int row[4] = {16 * mt + Lay<D>::perm(2 * c), 16 * mt + Lay<D>::perm(2 * c + 1),

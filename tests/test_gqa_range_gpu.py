@@ -46,8 +46,8 @@ def check_decode_on_gpu(dev, q, scale=None):
     weight's rounding to fp16 is off by no more than the weight itself, and
     a warp's sums have four steps for each of its units, off by 2^-23 each.  The
     sums are fp32 in units of up to the sequence's largest v_scale S, whether a
-    row sees it or not: a factor between two units is off by 2^-150 at least,
-    that times 448 S, and 2^16 sums of steps of 2^-149 S over 2^7: 2^-139 S."""
+    row sees it or not: a smaller scale's factor is off by 2^-150, that times 448
+    S, and 2^16 sums by steps of 2^-149 S over 2^7: 2^-139 S."""
     import deepseek_v4_kernel as dk
     kc, vc, ks, vs, table, ctx = dev
     b, s_q, h, d = q.shape
@@ -62,6 +62,7 @@ def check_decode_on_gpu(dev, q, scale=None):
     pieces = torch.cuda.get_device_properties(0).multi_processor_count * 8
     steps = 2.0 ** -23 * (4 * -(-units // pieces) + 32)
     u = U[q.dtype]
+    least = 2.0 ** -25 if q.dtype == torch.float16 else 1e-30  # fp16 has steps of 2^-24 at zero
     for i, n in enumerate(lens):
         if n == 0:
             assert (got[i] == 0).all() and torch.isneginf(lse[i]).all()
@@ -79,7 +80,8 @@ def check_decode_on_gpu(dev, q, scale=None):
             want, mag, rest = p @ v, p @ v.abs(), p.clamp(max=2.0 ** -25) @ v.abs()
             most = vs[blk, kvh].double().max()
             e = 2.0 ** -19 * size + 2.0 ** -20 + steps
-            tol = u * want.abs() + (2.0 ** -11 + 2 * e)[..., None] * mag + rest + 2.0 ** -139 * most + 1e-30
+            err = (2.0 ** -11 + 2 * e)[..., None] * mag + rest + 2.0 ** -139 * most
+            tol = u * (want.abs() + err) + err + least  # (what is rounded is off already)
             o, l = got[i, :, kvh * g:(kvh + 1) * g].double(), lse[i, kvh * g:(kvh + 1) * g].T.double()
             off = (o - want).abs()
             assert (off <= tol).all(), (i, kvh, off.max().item(), int((~(off <= tol)).sum()))
@@ -118,6 +120,28 @@ def test_decode_value_scales_far_apart(kind, h, d, page, s_q):
     vc.view(torch.uint8)[zero.cuda()] = 0
     ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
     check_decode_on_gpu((kc, vc, ks, vs, table.cuda(), ctx), rand(g, len(lens), s_q, h, d))
+
+
+@pytest.mark.parametrize("exps", [[-8, Z, 119, -8], [-44, Z, 57, Z], [0, -60, 119, Z], [-30, Z, 119, 119]])
+@pytest.mark.parametrize("h,d", [(3, 128), (12, 64)])
+def test_decode_zeros_before_large_values_out_of_sight(exps, h, d):
+    """The largest blocks have weights of 2^-261; zeros or small values stand
+    between them and those that make the output."""
+    lens = [64, 50, 700] * 40
+    kc, vc, ks, vs = pool(44 * len(lens), 16, 1, d, 44)
+    kc.zero_()
+    ks.fill_(1.0)
+    where = torch.arange(44 * len(lens), device="cuda") % 4
+    top = max(x for x in exps if x != Z)
+    for i, x in enumerate(exps):
+        vs[where == i] = 2.0 ** (-100 if x == Z else x)
+        if x == Z:
+            vc.view(torch.uint8)[where == i] = 0
+        elif x == top:
+            kc.view(torch.uint8)[where == i] = 0x38  # 1.0
+    table = torch.arange(44 * len(lens), dtype=torch.int32, device="cuda").view(len(lens), 44)
+    q = torch.full((len(lens), 1, h, d), -16.0 * 128 / d, dtype=torch.bfloat16, device="cuda")
+    check_decode_on_gpu((kc, vc, ks, vs, table, torch.tensor(lens, dtype=torch.int32, device="cuda")), q, scale=128 ** -0.5)
 
 
 @pytest.mark.parametrize("exps", [[-80, 40], [118, -8], [-8, -8, 118, 60], [0, 100, -30]])
