@@ -217,7 +217,7 @@ _PAGES = (16, 32, 64, 128, 256, 512, 1024)
 
 def _scale(sm_scale: Optional[float], d: int) -> float:
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale < _MAX_FP32:
+    if not 0.0 < scale <= _MAX_FP32:
         raise RuntimeError(f"sm_scale must be positive, in fp32 too, got {scale}")
     return scale
 
