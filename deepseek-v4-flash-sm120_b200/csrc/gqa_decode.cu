@@ -23,7 +23,7 @@
 // register or an issue slot spent on them.
 //
 // Measured, d = 128, against 6.5 TB/s of a copy: 16 sequences of 131,072
-// positions, 8 KV heads of 16 rows (4.1 GB) 728 us, 5.6 TB/s (835 where it runs
+// positions, 8 KV heads of 16 rows (4.1 GB) 728 us, 5.6 TB/s (855 where it runs
 // for long, at the power limit's 1.7 GHz); 32 of 1,000 to 32,768 with 8 rows
 // (554 MB) 126 us, 4.4 TB/s; one of 4,096 (8.4 MB) 16.6.  The last is what a
 // call takes whatever its size (launch, the list, the first tiles behind their
